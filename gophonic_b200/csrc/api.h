@@ -49,6 +49,35 @@ struct AttnParamsX : AttnParams {
                            // plane (the values are the first dv channels of the keys) has the keys' stride d.
 };
 
+// Attention that reads a part of its cache: the extremes of every key channel of the full pages (page_bounds), the pages of a row and
+// kv head chosen by them (select_pages), and attention over the listed pages (attention_pages).  Rows are those of a step, packed
+// sequence by sequence, as in AttnParams.
+struct PagesParams {
+    const void* q;          // select_pages, attention_pages: [rows, q_row_stride], heads x d
+    int64_t q_row_stride;
+    void* out;              // attention_pages: [rows, out_row_stride], heads x d
+    int64_t out_row_stride;
+    const void* k_plane;    // page_bounds (planes of them), attention_pages: [pages][kv_heads][64][d]
+    const void* v_plane;
+    void* bounds;           // page_bounds (planes of them), select_pages: [pages][kv_heads][2][d], the lowest values, then the highest
+    const int* block_table;
+    int bt_stride;
+    const int* seq_slot;
+    const int* seq_q_start;
+    const int* seq_q_len;
+    const int* seq_kv_len;
+    int nseq, heads, kv_heads, d;
+    int max_q_len;
+    float scale;
+    int* list;              // [rows][kv_heads][top]: logical pages; negative entries name none
+    int top;
+    int first, last;        // select_pages: pages at the sequence's start, and up to the row's own, that are always chosen
+    int planes;             // page_bounds: planes that lie behind one another, pages apart
+    int pages;              // pages of each cache plane, and slots (rows) of the block table
+    int max_slots;
+    int rows;               // rows of q
+};
+
 // Per-head q/k RMSNorm, rotary embedding and cache write on the rows of a fused q|k|v buffer.
 struct QkRopeParams {
     void* qkv;
@@ -468,3 +497,6 @@ struct GatedDeltaParams {
 };
 GB_API int gb_gated_delta(const GatedDeltaParams* p, cudaStream_t stream);
 GB_API int gb_gelu(void* z, int64_t n, int dtype, cudaStream_t stream);
+GB_API int gb_page_bounds(const PagesParams* p, int dtype, cudaStream_t stream);
+GB_API int gb_select_pages(const PagesParams* p, int dtype, cudaStream_t stream);
+GB_API int gb_attention_pages(const PagesParams* p, int dtype, cudaStream_t stream);

@@ -1,0 +1,504 @@
+// Attention over listed pages of the cache: every (row, kv head) has a list of logical pages, and the row attends to the keys of
+// those pages at positions up to its own.  Entries that name no page of the row's past are passed over; a row whose list holds
+// nothing it can see leaves zeros.
+//
+// Single rows.  A cluster of CTAs owns one (row, kv head): the CTAs take equal stretches of the list's pages, each with a running
+// softmax of its own, and join their results through distributed shared memory, so there is neither scratch memory nor a second
+// kernel.  The query heads of the group are the rows of the tiles and share every key and value that is read.
+//   bfloat16: both products on mma.sync, a page of 64 keys at a time, 16 keys a warp, pages asked for three deep by cp.async;
+//   float32:  CUDA cores, pages staged in shared memory; a thread has a key's scores first and some channels' sums after.
+// Scores, the softmax and the sums are float32; with bfloat16 the probabilities are rounded to bfloat16 for the second product, as
+// the values are.
+#include "mma.cuh"
+#include "api.h"
+
+#include <cooperative_groups.h>
+#include <math.h>
+
+namespace {
+
+namespace cg = cooperative_groups;
+typedef __nv_bfloat16 bf16;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int THREADS = 128;
+constexpr int MAX_TOP = 1024;     // entries of a list
+constexpr int MAX_PIECES = 8;     // CTAs of a cluster: the portable most
+
+// The row's listed pages that it can see, in the list's order, packed into `to`; how many there are.  Every thread of the CTA.
+__device__ __forceinline__ int pack_list(const PagesParams& p, const int* list, int own_page, int* to, int* counts) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int n = 0;
+    for (int base = 0; base < p.top; base += THREADS) {
+        const int i = base + tid;
+        const int lp = i < p.top ? list[i] : -1;
+        const bool ok = lp >= 0 && lp <= own_page;
+        const unsigned who = __ballot_sync(0xffffffffu, ok);
+        if (lane == 0) counts[warp] = __popc(who);
+        __syncthreads();
+        int at = n + __popc(who & ((1u << lane) - 1u));
+        for (int w = 0; w < THREADS / 32; w++) {
+            if (w < warp) at += counts[w];
+            n += counts[w];
+        }
+        if (ok) to[at] = lp;
+        __syncthreads();
+    }
+    return n;
+}
+
+// What the CTAs of a cluster leave for one another: per head of the chunk its maximum, sum and weighted values.
+// Joined by all of them: CTA r of the cluster writes every pieces-th four channels.
+template <typename T>
+__device__ __forceinline__ void join(const PagesParams& p, const float* ml, const float* os, int nh, int hd, T* out) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int pieces = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    cluster.sync();
+    const int quads = hd / 4;
+    for (int idx = threadIdx.x * pieces + rank; idx < nh * quads; idx += THREADS * pieces) {
+        const int r = idx / quads, c = (idx - r * quads) * 4;
+        float m[MAX_PIECES], M = -INFINITY;
+        for (int w = 0; w < pieces; w++) {
+            m[w] = cluster.map_shared_rank(ml, w)[2 * r];
+            M = fmaxf(M, m[w]);
+        }
+        float L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (M != -INFINITY) {
+            for (int w = 0; w < pieces; w++) {
+                const float e = exp2f(m[w] - M);
+                L += e * cluster.map_shared_rank(ml, w)[2 * r + 1];
+                const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(os, w) + (size_t)r * hd + c);
+                acc.x += e * x.x;
+                acc.y += e * x.y;
+                acc.z += e * x.z;
+                acc.w += e * x.w;
+            }
+        }
+        T* op = out + (int64_t)r * hd + c;
+        const float inv = M == -INFINITY ? 0.f : 1.f / L;     // nothing seen: zeros
+        op[0] = from_f32<T>(acc.x * inv);
+        op[1] = from_f32<T>(acc.y * inv);
+        op[2] = from_f32<T>(acc.z * inv);
+        op[3] = from_f32<T>(acc.w * inv);
+    }
+    cluster.sync();     // a CTA's shared memory outlives its readers
+}
+
+// The place of a CTA: its row, kv head, first head and number of heads; false: nothing to do (for the whole cluster).
+struct Place {
+    int row, pos, kvh, h0, nh;
+    const int* bt;
+    __device__ __forceinline__ bool find(const PagesParams& p, int GC) {
+        const int pieces = (int)cg::this_cluster().num_blocks();
+        const int unit = (int)blockIdx.x / pieces, seq = unit / p.max_q_len, qi = unit % p.max_q_len;
+        const int q_len = p.seq_q_len[seq];
+        if (qi >= q_len) return false;
+        const int G = p.heads / p.kv_heads, chunks = (G + GC - 1) / GC;
+        kvh = (int)blockIdx.y / chunks;
+        const int chunk = (int)blockIdx.y % chunks;
+        row = p.seq_q_start[seq] + qi;
+        pos = p.seq_kv_len[seq] - q_len + qi;
+        h0 = kvh * G + chunk * GC;
+        nh = min(GC, G - chunk * GC);
+        bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
+        return true;
+    }
+};
+
+// ---- bfloat16 ------------------------------------------------------------------------------------
+constexpr int STAGES = 3;
+
+template <int HD>
+__global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) {
+    constexpr bool QREG = HD <= 128;
+    constexpr int SD = HD + 8, KS = HD / 16, NF = HD / 8, CH = HD / 8;
+    constexpr int STAGE = 2 * 64 * SD;   // elements: keys, then values
+    extern __shared__ __align__(16) unsigned char raw[];
+    bf16* Qs = reinterpret_cast<bf16*>(raw);       // [16][SD]
+    bf16* KV = Qs + 16 * SD;                       // [STAGES][2][64][SD]
+    int* pages = reinterpret_cast<int*>(KV + STAGES * STAGE);   // [top]
+    __shared__ int counts[THREADS / 32];
+    __shared__ float ml[16][2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    pdl_wait();
+    pdl_trigger();
+    Place at;
+    const int G = p.heads / p.kv_heads, GC = G < 16 ? G : 16;
+    if (!at.find(p, GC)) return;
+    const int pieces = (int)cg::this_cluster().num_blocks(), piece = (int)cg::this_cluster().block_rank();
+    {
+        const bf16* qsrc = (const bf16*)p.q + (int64_t)at.row * p.q_row_stride + (int64_t)at.h0 * HD;
+        for (int idx = tid; idx < 16 * CH; idx += THREADS) {
+            const int r = idx / CH, c = idx - r * CH;
+            const bool ok = r < at.nh;
+            cp_async16(Qs + r * SD + c * 8, ok ? qsrc + (int64_t)r * HD + c * 8 : qsrc, ok ? 16 : 0);
+        }
+        cp_async_commit();
+    }
+    const int n_all = pack_list(p, p.list + ((int64_t)at.row * p.kv_heads + at.kvh) * p.top, at.pos / GB_PAGE, pages, counts);
+    const int lo = (int)((int64_t)n_all * piece / pieces), n = (int)((int64_t)n_all * (piece + 1) / pieces) - lo;
+
+    const bf16* kbase = (const bf16*)p.k_plane;
+    const bf16* vbase = (const bf16*)p.v_plane;
+    auto load_tile = [&](int i) {
+        const int64_t off = (page_of(at.bt, pages[lo + i] * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + at.kvh) * (int64_t)(GB_PAGE * HD);
+        bf16* st = KV + (i % STAGES) * STAGE;
+        for (int idx = tid; idx < 64 * CH; idx += THREADS) {
+            const int r = idx / CH, c = idx - r * CH;
+            cp_async16(st + r * SD + c * 8, kbase + off + r * HD + c * 8, 16);
+        }
+        for (int idx = tid; idx < 64 * CH; idx += THREADS) {
+            const int r = idx / CH, c = idx - r * CH;
+            cp_async16(st + 64 * SD + r * SD + c * 8, vbase + off + r * HD + c * 8, 16);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++) {
+        if (s < n) load_tile(s);
+        cp_async_commit();
+    }
+    const float sc = p.scale * LOG2E;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float o[NF][4];
+#pragma unroll
+    for (int j = 0; j < NF; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[j][e] = 0.f;
+    uint32_t qf[QREG ? KS : 1][4];
+    for (int i = 0; i < n; i++) {
+        cp_async_wait<STAGES - 2>();   // page i has landed, and the queries before it
+        __syncthreads();
+        if (i + STAGES - 1 < n) load_tile(i + STAGES - 1);
+        cp_async_commit();
+        if (QREG && i == 0) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                ldmatrix_x4(qf[QREG ? ks : 0], Qs + ((lane & 7) + ((lane >> 3) & 1) * 8) * SD + ks * 16 + (lane >> 4) * 8);
+        }
+        const bf16* kt = KV + (i % STAGES) * STAGE;
+        const bf16* vt = kt + 64 * SD;
+        const int key0 = pages[lo + i] * GB_PAGE + warp * 16;
+        if (pages[lo + i] * GB_PAGE + GB_PAGE - 1 > at.pos) {
+            // The row's own page: what stands behind its position gets probabilities of zero, and zero times an Inf or NaN
+            // that was left there would not be zero.
+            const int seen = at.pos + 1 - pages[lo + i] * GB_PAGE;
+            for (int idx = tid; idx < (64 - seen) * CH; idx += THREADS)
+                *reinterpret_cast<uint4*>(KV + (i % STAGES) * STAGE + (64 + seen + idx / CH) * SD + idx % CH * 8) = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+        }
+        float s[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[j][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            uint32_t a[4], b[4];
+            if (QREG) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] = qf[QREG ? ks : 0][e];
+            } else {
+                ldmatrix_x4(a, Qs + ((lane & 7) + ((lane >> 3) & 1) * 8) * SD + ks * 16 + (lane >> 4) * 8);
+            }
+            ldmatrix_x4(b, kt + (warp * 16 + (lane & 7) + (lane >> 4) * 8) * SD + ks * 16 + ((lane >> 3) & 1) * 8);
+            mma_bf16_16816(s[0], a[0], a[1], a[2], a[3], b[0], b[1]);
+            mma_bf16_16816(s[1], a[0], a[1], a[2], a[3], b[2], b[3]);
+        }
+        float mx0 = m0, mx1 = m1;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool ok = key0 + j * 8 + t4 * 2 + (e & 1) <= at.pos;
+                const float v = ok ? s[j][e] * sc : -INFINITY;
+                s[j][e] = v;
+                if (e & 2) mx1 = fmaxf(mx1, v); else mx0 = fmaxf(mx0, v);
+            }
+        }
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+        const float base0 = mx0 == -INFINITY ? 0.f : mx0, base1 = mx1 == -INFINITY ? 0.f : mx1;
+        const float c0 = exp2f(m0 - base0), c1 = exp2f(m1 - base1);
+        m0 = mx0;
+        m1 = mx1;
+        l0 *= c0;
+        l1 *= c1;
+#pragma unroll
+        for (int j = 0; j < NF; j++) {
+            o[j][0] *= c0;
+            o[j][1] *= c0;
+            o[j][2] *= c1;
+            o[j][3] *= c1;
+        }
+        uint32_t pa[4];
+        {
+            const float p00 = exp2f(s[0][0] - base0), p01 = exp2f(s[0][1] - base0), p02 = exp2f(s[0][2] - base1), p03 = exp2f(s[0][3] - base1);
+            const float p10 = exp2f(s[1][0] - base0), p11 = exp2f(s[1][1] - base0), p12 = exp2f(s[1][2] - base1), p13 = exp2f(s[1][3] - base1);
+            l0 += p00 + p01 + p10 + p11;
+            l1 += p02 + p03 + p12 + p13;
+            pa[0] = pack_bf16(p00, p01);
+            pa[1] = pack_bf16(p02, p03);
+            pa[2] = pack_bf16(p10, p11);
+            pa[3] = pack_bf16(p12, p13);
+        }
+#pragma unroll
+        for (int c = 0; c < KS; c++) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, vt + (warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * SD + c * 16 + (lane >> 4) * 8);
+            mma_bf16_16816(o[c * 2], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+            mma_bf16_16816(o[c * 2 + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+        }
+    }
+    cp_async_wait<0>();
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    __syncthreads();   // every warp is done with the pages: their memory takes the warps' results
+
+    float* Ms = reinterpret_cast<float*>(KV);   // [4][16]
+    float* Ls = Ms + 64;                        // [4][16]
+    float* Os = Ls + 64;                        // [4][16][HD]; the CTA's own over the first warp's
+    if (t4 == 0) {
+        Ms[warp * 16 + g] = m0;
+        Ms[warp * 16 + g + 8] = m1;
+        Ls[warp * 16 + g] = l0;
+        Ls[warp * 16 + g + 8] = l1;
+    }
+#pragma unroll
+    for (int j = 0; j < NF; j++) {
+        float* o0 = Os + ((size_t)warp * 16 + g) * HD + j * 8 + t4 * 2;
+        if (g < at.nh) *reinterpret_cast<float2*>(o0) = make_float2(o[j][0], o[j][1]);
+        if (g + 8 < at.nh) *reinterpret_cast<float2*>(o0 + 8 * HD) = make_float2(o[j][2], o[j][3]);
+    }
+    __syncthreads();
+    for (int idx = tid; idx < at.nh * HD / 4; idx += THREADS) {
+        const int r = idx / (HD / 4), c = (idx - r * (HD / 4)) * 4;
+        const float M = fmaxf(fmaxf(Ms[r], Ms[16 + r]), fmaxf(Ms[32 + r], Ms[48 + r]));
+        float L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (M != -INFINITY) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float e = exp2f(Ms[w * 16 + r] - M);
+                const float4 x = *reinterpret_cast<const float4*>(Os + ((size_t)w * 16 + r) * HD + c);
+                L += e * Ls[w * 16 + r];
+                acc.x += e * x.x;
+                acc.y += e * x.y;
+                acc.z += e * x.z;
+                acc.w += e * x.w;
+            }
+        }
+        *reinterpret_cast<float4*>(Os + (size_t)r * HD + c) = acc;
+        if (c == 0) {
+            ml[r][0] = M;
+            ml[r][1] = L;
+        }
+    }
+    join<bf16>(p, &ml[0][0], Os, at.nh, HD, (bf16*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * HD);
+}
+
+// ---- float32 -------------------------------------------------------------------------------------
+constexpr int F_HEADS = 8;       // heads of a group that a CTA takes at most
+constexpr int F_CH = 2;          // channels a thread sums at most: head_dim up to 256
+
+__global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) {
+    extern __shared__ __align__(16) float sm[];
+    const int d = p.d, sd = d + 4;                 // rows of 16-byte chunks that start four banks further each
+    float* Qs = sm;                                // [F_HEADS][d], scaled
+    float* Ks = Qs + F_HEADS * d;                  // [64][sd]
+    float* Vs = Ks + GB_PAGE * sd;                 // [64][d]
+    float* Ps = Vs + GB_PAGE * d;                  // [F_HEADS][64]
+    float* Os = Ps + F_HEADS * GB_PAGE;            // [F_HEADS][d]
+    int* pages = reinterpret_cast<int*>(Os + F_HEADS * d);
+    __shared__ int counts[THREADS / 32];
+    __shared__ float ml[F_HEADS][2], corr[F_HEADS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    Place at;
+    const int G = p.heads / p.kv_heads, GC = G < F_HEADS ? G : F_HEADS;
+    if (!at.find(p, GC)) return;
+    const int pieces = (int)cg::this_cluster().num_blocks(), piece = (int)cg::this_cluster().block_rank();
+    const float* qsrc = (const float*)p.q + (int64_t)at.row * p.q_row_stride + (int64_t)at.h0 * d;
+    const float sc = p.scale * LOG2E;
+    for (int i = tid; i < at.nh * d; i += THREADS) Qs[i] = qsrc[i] * sc;
+    if (tid < F_HEADS) {
+        ml[tid][0] = -INFINITY;
+        ml[tid][1] = 0.f;
+    }
+    const int n_all = pack_list(p, p.list + ((int64_t)at.row * p.kv_heads + at.kvh) * p.top, at.pos / GB_PAGE, pages, counts);
+    const int lo = (int)((int64_t)n_all * piece / pieces), n = (int)((int64_t)n_all * (piece + 1) / pieces) - lo;
+    float o[F_HEADS][F_CH];
+#pragma unroll
+    for (int h = 0; h < F_HEADS; h++)
+#pragma unroll
+        for (int c = 0; c < F_CH; c++) o[h][c] = 0.f;
+    const int CH = d / 4;
+    for (int i = 0; i < n; i++) {
+        const int64_t off = (page_of(at.bt, pages[lo + i] * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + at.kvh) * (int64_t)(GB_PAGE * d);
+        const float* k = (const float*)p.k_plane + off;
+        const float* v = (const float*)p.v_plane + off;
+        __syncthreads();       // the page before is done with
+        for (int idx = tid; idx < GB_PAGE * CH; idx += THREADS) {
+            const int r = idx / CH, c = (idx - r * CH) * 4;
+            cp_async16(Ks + r * sd + c, k + (int64_t)r * d + c, 16);
+            cp_async16(Vs + r * d + c, v + (int64_t)r * d + c, 16);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncthreads();
+        {
+            // a thread: one key, every second head
+            const int key = tid & 63;
+            const bool ok = pages[lo + i] * GB_PAGE + key <= at.pos;
+            float s[F_HEADS / 2];
+#pragma unroll
+            for (int h = 0; h < F_HEADS / 2; h++) s[h] = 0.f;
+            for (int c = 0; c < d; c += 4) {
+                const float4 kk = *reinterpret_cast<const float4*>(Ks + key * sd + c);
+#pragma unroll
+                for (int h = 0; h < F_HEADS / 2; h++) {
+                    const int head = 2 * h + (tid >> 6);
+                    if (head < at.nh) {
+                        const float4 qq = *reinterpret_cast<const float4*>(Qs + head * d + c);
+                        s[h] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[h]))));
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < F_HEADS / 2; h++) {
+                const int head = 2 * h + (tid >> 6);
+                if (head < at.nh) Ps[head * GB_PAGE + key] = ok ? s[h] : -INFINITY;
+            }
+        }
+        __syncthreads();
+        for (int h = warp; h < at.nh; h += THREADS / 32) {
+            const float a = Ps[h * GB_PAGE + lane], b = Ps[h * GB_PAGE + 32 + lane];
+            const float old = ml[h][0], m = fmaxf(old, warp_max(fmaxf(a, b))), base = m == -INFINITY ? 0.f : m;
+            const float pa = exp2f(a - base), pb = exp2f(b - base), sum = warp_sum(pa + pb);
+            Ps[h * GB_PAGE + lane] = pa;
+            Ps[h * GB_PAGE + 32 + lane] = pb;
+            __syncwarp();
+            if (lane == 0) {
+                corr[h] = exp2f(old - base);
+                ml[h][0] = m;
+                ml[h][1] = ml[h][1] * corr[h] + sum;
+            }
+        }
+        __syncthreads();
+        const int keys = min(GB_PAGE, at.pos + 1 - pages[lo + i] * GB_PAGE);   // the others are not touched: they may hold Inf or NaN
+#pragma unroll
+        for (int c = 0; c < F_CH; c++) {
+            const int ch = tid + c * THREADS;
+            if (ch < d) {
+                float acc[F_HEADS];
+#pragma unroll
+                for (int h = 0; h < F_HEADS; h++) acc[h] = h < at.nh ? o[h][c] * corr[h] : 0.f;
+                for (int key = 0; key < keys; key++) {
+                    const float vv = Vs[key * d + ch];
+#pragma unroll
+                    for (int h = 0; h < F_HEADS; h++)
+                        if (h < at.nh) acc[h] = fmaf(Ps[h * GB_PAGE + key], vv, acc[h]);
+                }
+#pragma unroll
+                for (int h = 0; h < F_HEADS; h++) o[h][c] = acc[h];
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < F_HEADS; h++)
+#pragma unroll
+        for (int c = 0; c < F_CH; c++)
+            if (h < at.nh && tid + c * THREADS < d) Os[h * d + tid + c * THREADS] = o[h][c];
+    __syncthreads();
+    join<float>(p, &ml[0][0], Os, at.nh, d, (float*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * d);
+}
+
+// Into how many pieces a row's list is cut: the CTAs of a cluster.
+int pieces_for(const PagesParams& p, int chunks, int per_sm) {
+    const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads * chunks;
+    int pieces = 1;
+    while (pieces < MAX_PIECES && units * pieces * 2 <= (int64_t)gb_sm_count() * per_sm && p.top >= 4 * pieces) pieces *= 2;
+    return pieces;
+}
+
+template <typename K>
+int launch(K kernel, const PagesParams& p, int chunks, int pieces, int smem, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    const int64_t x = (int64_t)p.nseq * p.max_q_len * pieces;
+    if (x > 0x7fffffff || p.kv_heads * chunks > 65535) GB_REFUSE("attention_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
+    cfg.gridDim = dim3((unsigned)x, p.kv_heads * chunks);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = pieces;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, p);
+    GB_CHECK_LAUNCH("attention_pages");
+    return 0;
+}
+
+template <int HD>
+int launch_mma(const PagesParams& p, cudaStream_t stream) {
+    constexpr int SD = HD + 8;
+    constexpr int base = (16 * SD + STAGES * 2 * 64 * SD) * 2;
+    static_assert(base >= (128 + 64 * HD) * 4 + 16 * SD * 2, "the warps' results fit where the pages were");
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(attn_pages_mma_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, base + MAX_TOP * 4);
+        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", base + MAX_TOP * 4, cudaGetErrorString(e));
+        configured = true;
+    }
+    const int G = p.heads / p.kv_heads, chunks = (G + 15) / 16;
+    return launch(attn_pages_mma_kernel<HD>, p, chunks, pieces_for(p, chunks, HD <= 128 ? 2 : 1), base + p.top * 4, stream);
+}
+
+int launch_f32(const PagesParams& p, cudaStream_t stream) {
+    const auto bytes = [](int d, int top) { return (F_HEADS * d * 2 + GB_PAGE * (2 * d + 4) + F_HEADS * GB_PAGE) * 4 + top * 4; };
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(attn_pages_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(256, MAX_TOP));
+        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", bytes(256, MAX_TOP), cudaGetErrorString(e));
+        configured = true;
+    }
+    const int G = p.heads / p.kv_heads, chunks = (G + F_HEADS - 1) / F_HEADS;
+    return launch(attn_pages_f32_kernel, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1), bytes(p.d, p.top), stream);
+}
+
+}  // namespace
+
+GB_API int gb_attention_pages(const PagesParams* pp, int dtype, cudaStream_t stream) {
+    const PagesParams p = *pp;
+    const char* who = "attention_pages";
+    if (p.nseq <= 0 || p.max_q_len <= 0) return 0;
+    if (dtype != GB_F32 && dtype != GB_BF16) GB_REFUSE("%s: dtype code %d", who, dtype);
+    if (p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads) GB_REFUSE("%s: %d heads over %d kv heads", who, p.heads, p.kv_heads);
+    if (p.top <= 0 || p.top > MAX_TOP) GB_REFUSE("%s: lists of %d pages; this kernel takes 1 to %d", who, p.top, MAX_TOP);
+    if (p.pages <= 0 || p.bt_stride <= 0 || p.max_slots <= 0) GB_REFUSE("%s: %d pages, block table %d x %d", who, p.pages, p.max_slots, p.bt_stride);
+    if (((uintptr_t)p.k_plane | (uintptr_t)p.v_plane) & 15) GB_REFUSE("%s: the planes must be 16-byte aligned", who);
+    if (dtype == GB_F32) {
+        if (p.d <= 0 || p.d % 4 || p.d > 256) GB_REFUSE("%s: head_dim %d is not a multiple of 4 up to 256", who, p.d);
+        return launch_f32(p, stream);
+    }
+    if (((uintptr_t)p.q & 15) || (p.q_row_stride & 7)) GB_REFUSE("%s: query rows must be 16-byte aligned", who);
+    switch (p.d) {
+        case 16: return launch_mma<16>(p, stream);
+        case 32: return launch_mma<32>(p, stream);
+        case 48: return launch_mma<48>(p, stream);
+        case 64: return launch_mma<64>(p, stream);
+        case 80: return launch_mma<80>(p, stream);
+        case 96: return launch_mma<96>(p, stream);
+        case 112: return launch_mma<112>(p, stream);
+        case 128: return launch_mma<128>(p, stream);
+        case 256: return launch_mma<256>(p, stream);
+    }
+    GB_REFUSE("%s: bfloat16 heads of %d are not one of 16, 32, ..., 128, 256", who, p.d);
+}
+
+// the checked build's record of the first index this file's kernels found out of bounds
+GB_CHECK_READER(gb_checked_status_attention_pages)

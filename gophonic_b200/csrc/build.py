@@ -48,6 +48,8 @@ SOURCES = [
     "attention_simt.cu",
     "attention_mma.cu",
     "attention_tc5.cu",
+    "attention_pages.cu",
+    "page_select.cu",
     "linear_state.cu",
     "delta_state.cu",
     "attention_sigmoid.cu",

@@ -526,7 +526,7 @@ def checked_status():
     Always None in the ordinary build, whose kernels carry no checks.  Synchronises."""
     out = (c_int * 4)()
     for name in ("rows", "cache", "attention_simt", "attention_mma", "attention_tc5", "linear_state", "delta_state", "attention_sigmoid", "hyper", "postnorm", "attention_latent", "sandwich",
-                 "short_conv", "gated_delta"):
+                 "short_conv", "gated_delta", "page_select", "attention_pages"):
         code = int(getattr(_lib, "gb_checked_status_" + name)(out))
         if code or out[3]:
             return name, _CHECK_NAMES.get(code, f"code {code}"), out[1], out[2], out[3]
@@ -800,6 +800,110 @@ def attention_decode_rope(qkv: torch.Tensor, out: torch.Tensor, rope_args: tuple
     r = _rope_params(qkv, *rope_args)
     a = _attn_params(qkv[:, :r.heads * r.d], out, *attn_args)
     _check(_lib.gb_attention_decode_mma_rope(byref(a), byref(r), _stream()), 2 if a.num_splits > 1 else 1)
+
+
+# ---- attention that reads a part of its cache ----------------------------------------------------
+class _PagesParams(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_row_stride", c_int64), ("out", c_void_p), ("out_row_stride", c_int64), ("k_plane", c_void_p), ("v_plane", c_void_p),
+        ("bounds", c_void_p), ("block_table", c_void_p), ("bt_stride", c_int), ("seq_slot", c_void_p), ("seq_q_start", c_void_p),
+        ("seq_q_len", c_void_p), ("seq_kv_len", c_void_p), ("nseq", c_int), ("heads", c_int), ("kv_heads", c_int), ("d", c_int),
+        ("max_q_len", c_int), ("scale", c_float), ("list", c_void_p), ("top", c_int), ("first", c_int), ("last", c_int), ("planes", c_int),
+        ("pages", c_int), ("max_slots", c_int), ("rows", c_int),
+    ]
+
+
+MAX_LISTED_PAGES = 1024          # entries of a row's list of pages
+MAX_SELECTABLE_PAGES = 32768     # pages of a sequence that a row's may be selected from: 2,097,152 tokens
+
+
+def _need_sequences(who: str, block_table: torch.Tensor, nseq: int, **lists: torch.Tensor) -> None:
+    _need(block_table, "block table", torch.int32, 2)
+    for name, t in lists.items():
+        _need(t, name, torch.int32, 1)
+        if t.numel() < nseq:
+            raise KernelError(f"{who}: {name} has {t.numel()} entries for {nseq} sequences")
+
+
+def _need_rows(who: str, name: str, t: torch.Tensor, dtype, width: int) -> None:
+    _need(t, f"{who}: {name}", dtype, 2, contiguous=False)
+    if t.stride(1) != 1 or t.shape[1] < width or (t.shape[0] > 1 and t.stride(0) < width):
+        raise KernelError(f"{who}: {name} {tuple(t.shape)} with strides {tuple(t.stride())} for rows of {width}")
+
+
+def page_bounds(k_planes: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_slot: torch.Tensor, seq_q_len: torch.Tensor,
+                seq_kv_len: torch.Tensor, nseq: int, max_q_len: int) -> None:
+    """The extremes of every key channel of the pages that a step has filled: for each sequence's pages whose last position is among
+    its ``seq_q_len`` newest, bounds[page, kv head, 0] = the lowest values of the page's 64 keys and bounds[page, kv head, 1] the
+    highest (exact; NaN if one of them is).  ``k_planes`` [pages, kv_heads, 64, head_dim] with ``bounds`` [pages, kv_heads, 2,
+    head_dim] of the same dtype, or several such planes in one leading dimension.  Nothing else of ``bounds`` changes.  To be called
+    behind what writes the step's keys; ``select_pages`` scores the pages of earlier tokens by it."""
+    if k_planes.dim() not in (4, 5):
+        raise KernelError(f"page_bounds: key planes {tuple(k_planes.shape)}")
+    _need(k_planes, "key planes")
+    _need(bounds, "page bounds", k_planes.dtype)
+    d = k_planes.shape[-1]
+    if k_planes.shape[-2] != PAGE or tuple(bounds.shape) != tuple(k_planes.shape[:-2]) + (2, d):
+        raise KernelError(f"page_bounds: key planes {tuple(k_planes.shape)}, bounds {tuple(bounds.shape)}")
+    _need_sequences("page_bounds", block_table, nseq, seq_slot=seq_slot, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
+    planes = k_planes.shape[0] if k_planes.dim() == 5 else 1
+    p = _PagesParams(k_plane=k_planes.data_ptr(), bounds=bounds.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
+                     seq_slot=seq_slot.data_ptr(), seq_q_len=seq_q_len.data_ptr(), seq_kv_len=seq_kv_len.data_ptr(), nseq=nseq,
+                     kv_heads=k_planes.shape[-3], d=d, max_q_len=max_q_len, planes=planes, pages=k_planes.shape[-4], max_slots=block_table.shape[0])
+    _check(_lib.gb_page_bounds(byref(p), _code(k_planes.dtype), _stream()))
+
+
+def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_slot: torch.Tensor, seq_q_start: torch.Tensor,
+                 seq_q_len: torch.Tensor, seq_kv_len: torch.Tensor, nseq: int, max_q_len: int, heads: int, kv_heads: int, head_dim: int,
+                 pages: torch.Tensor, first: int = 1, last: int = 2) -> None:
+    """For every row of the step and kv head, which pages of 64 tokens of its sequence it should read: ``pages`` int32 [rows, kv_heads,
+    top] receives logical page numbers in ascending order, then -1.  The first ``first`` pages and the ``last`` (at least one) up to
+    the row's own are always among them, and of the others those with the highest scores
+    sum over the group's query heads and channels of max(q lo, q hi), lo and hi the page's bounds (``page_bounds``): an upper bound of
+    what any of its keys can score.  The choice is the one of 64-bit arithmetic; pages that tie go by their number, a score that
+    is NaN counts as the lowest.  A row that sees no more than ``top`` pages gets all of them.  q is a [rows, >= heads * head_dim]
+    view (row stride free); the bounds of full pages must hold lo <= hi, as ``page_bounds`` leaves them; rows of no sequence keep
+    what they had.  Sequences of up to ``MAX_SELECTABLE_PAGES`` pages."""
+    _need_rows("select_pages", "q", q, None, heads * head_dim)
+    _need(bounds, "page bounds", q.dtype, 4)
+    _need(pages, "page lists", torch.int32, 3)
+    if bounds.shape[1:] != (kv_heads, 2, head_dim):
+        raise KernelError(f"select_pages: bounds {tuple(bounds.shape)} for {kv_heads} kv heads of {head_dim}")
+    if pages.shape[0] != q.shape[0] or pages.shape[1] != kv_heads:
+        raise KernelError(f"select_pages: lists {tuple(pages.shape)} for {q.shape[0]} rows and {kv_heads} kv heads")
+    _need_sequences("select_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
+    p = _PagesParams(q=q.data_ptr(), q_row_stride=q.stride(0), bounds=bounds.data_ptr(), block_table=block_table.data_ptr(),
+                     bt_stride=block_table.stride(0), seq_slot=seq_slot.data_ptr(), seq_q_start=seq_q_start.data_ptr(),
+                     seq_q_len=seq_q_len.data_ptr(), seq_kv_len=seq_kv_len.data_ptr(), nseq=nseq, heads=heads, kv_heads=kv_heads, d=head_dim,
+                     max_q_len=max_q_len, list=pages.data_ptr(), top=pages.shape[2], first=first, last=last, pages=bounds.shape[0],
+                     max_slots=block_table.shape[0], rows=q.shape[0])
+    _check(_lib.gb_select_pages(byref(p), _code(q.dtype), _stream()))
+
+
+def attention_pages(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, block_table: torch.Tensor,
+                    seq_slot: torch.Tensor, seq_q_start: torch.Tensor, seq_q_len: torch.Tensor, seq_kv_len: torch.Tensor, nseq: int,
+                    max_q_len: int, heads: int, kv_heads: int, head_dim: int, scale: float, pages: torch.Tensor) -> None:
+    """Causal GQA over a part of the paged cache: row r's heads of kv head g attend to the keys, at positions up to the row's own, of
+    the logical pages that ``pages[r, g]`` lists (int32 [rows, kv_heads, top], top up to ``MAX_LISTED_PAGES``; ascending and each
+    once, as ``select_pages`` leaves them; negative entries and pages behind the row's own name nothing).  A row that sees no key
+    gives zeros; rows of no sequence keep what they had.  q and out are [rows, >= heads * head_dim] views (row strides free)."""
+    _need_rows("attention_pages", "q", q, None, heads * head_dim)
+    _need_rows("attention_pages", "out", out, q.dtype, heads * head_dim)
+    _need(k_plane, "key plane", q.dtype, 4)
+    _need(v_plane, "value plane", q.dtype, 4)
+    for t, nm in ((k_plane, "key plane"), (v_plane, "value plane")):
+        if t.shape[1:] != (kv_heads, PAGE, head_dim) or t.shape != k_plane.shape:
+            raise KernelError(f"attention_pages: {nm} {tuple(t.shape)} for {kv_heads} kv heads of {head_dim}")
+    _need(pages, "page lists", torch.int32, 3)
+    if pages.shape[0] != q.shape[0] or out.shape[0] != q.shape[0] or pages.shape[1] != kv_heads:
+        raise KernelError(f"attention_pages: q {tuple(q.shape)}, out {tuple(out.shape)}, lists {tuple(pages.shape)} for {kv_heads} kv heads")
+    _need_sequences("attention_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
+    p = _PagesParams(q=q.data_ptr(), q_row_stride=q.stride(0), out=out.data_ptr(), out_row_stride=out.stride(0), k_plane=k_plane.data_ptr(),
+                     v_plane=v_plane.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
+                     seq_slot=seq_slot.data_ptr(), seq_q_start=seq_q_start.data_ptr(), seq_q_len=seq_q_len.data_ptr(),
+                     seq_kv_len=seq_kv_len.data_ptr(), nseq=nseq, heads=heads, kv_heads=kv_heads, d=head_dim, max_q_len=max_q_len, scale=scale,
+                     list=pages.data_ptr(), top=pages.shape[2], pages=k_plane.shape[0], max_slots=block_table.shape[0], rows=q.shape[0])
+    _check(_lib.gb_attention_pages(byref(p), _code(q.dtype), _stream()))
 
 
 # ---- mixers with a matrix state ------------------------------------------------------------
