@@ -15,6 +15,9 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
+int gb_attention_pages_tc5_accepts(const PagesParams& p);
+int gb_attention_pages_tc5(const PagesParams& p, int pieces, cudaStream_t stream);
+
 namespace {
 
 namespace cg = cooperative_groups;
@@ -23,6 +26,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int THREADS = 128;
 constexpr int MAX_TOP = 1024;     // entries of a list
 constexpr int MAX_PIECES = 8;     // CTAs of a cluster: the portable most
+constexpr int TC5_MIN_ROWS = 16;  // rows of a sequence from which on its tiles run on tcgen05 (attention_pages_tc5.cu)
 
 // The row's listed pages that it can see, in the list's order, packed into `to`; how many there are.  Every thread of the CTA.
 __device__ __forceinline__ int pack_list(const PagesParams& p, const int* list, int own_page, int* to, int* counts) {
@@ -63,19 +67,18 @@ __device__ __forceinline__ void join(const PagesParams& p, const float* ml, cons
         }
         float L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (M != -INFINITY) {
-            for (int w = 0; w < pieces; w++) {
-                const float e = exp2f(m[w] - M);
-                L += e * cluster.map_shared_rank(ml, w)[2 * r + 1];
-                const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(os, w) + (size_t)r * hd + c);
-                acc.x += e * x.x;
-                acc.y += e * x.y;
-                acc.z += e * x.z;
-                acc.w += e * x.w;
-            }
+        const float base = M == -INFINITY ? 0.f : M;
+        for (int w = 0; w < pieces; w++) {
+            const float e = exp2f(m[w] - base);        // a NaN score leaves no maximum but a NaN sum, which stays one
+            L += e * cluster.map_shared_rank(ml, w)[2 * r + 1];
+            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(os, w) + (size_t)r * hd + c);
+            acc.x += e * x.x;
+            acc.y += e * x.y;
+            acc.z += e * x.z;
+            acc.w += e * x.w;
         }
         T* op = out + (int64_t)r * hd + c;
-        const float inv = M == -INFINITY ? 0.f : 1.f / L;     // nothing seen: zeros
+        const float inv = L == 0.f ? 0.f : 1.f / L;     // nothing seen: zeros
         op[0] = from_f32<T>(acc.x * inv);
         op[1] = from_f32<T>(acc.y * inv);
         op[2] = from_f32<T>(acc.z * inv);
@@ -279,17 +282,16 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
         const float M = fmaxf(fmaxf(Ms[r], Ms[16 + r]), fmaxf(Ms[32 + r], Ms[48 + r]));
         float L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (M != -INFINITY) {
+        const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float e = exp2f(Ms[w * 16 + r] - M);
-                const float4 x = *reinterpret_cast<const float4*>(Os + ((size_t)w * 16 + r) * HD + c);
-                L += e * Ls[w * 16 + r];
-                acc.x += e * x.x;
-                acc.y += e * x.y;
-                acc.z += e * x.z;
-                acc.w += e * x.w;
-            }
+        for (int w = 0; w < 4; w++) {
+            const float e = exp2f(Ms[w * 16 + r] - base);
+            const float4 x = *reinterpret_cast<const float4*>(Os + ((size_t)w * 16 + r) * HD + c);
+            L += e * Ls[w * 16 + r];
+            acc.x += e * x.x;
+            acc.y += e * x.y;
+            acc.z += e * x.z;
+            acc.w += e * x.w;
         }
         *reinterpret_cast<float4*>(Os + (size_t)r * HD + c) = acc;
         if (c == 0) {
@@ -486,6 +488,13 @@ GB_API int gb_attention_pages(const PagesParams* pp, int dtype, cudaStream_t str
         return launch_f32(p, stream);
     }
     if (((uintptr_t)p.q & 15) || (p.q_row_stride & 7)) GB_REFUSE("%s: query rows must be 16-byte aligned", who);
+    if (p.max_q_len >= TC5_MIN_ROWS && gb_attention_pages_tc5_accepts(p)) {
+        int gp = 1, pieces = 1;
+        while (gp < p.heads / p.kv_heads) gp *= 2;
+        const int64_t tiles = (int64_t)p.nseq * ceil_div(p.max_q_len, 256 / gp) * p.kv_heads;
+        while (pieces < MAX_PIECES && tiles * pieces * 2 <= gb_sm_count()) pieces *= 2;
+        return gb_attention_pages_tc5(p, pieces, stream);
+    }
     switch (p.d) {
         case 16: return launch_mma<16>(p, stream);
         case 32: return launch_mma<32>(p, stream);

@@ -1,0 +1,660 @@
+// Attention over listed pages for runs of rows, on the fifth-generation tensor cores (bfloat16, head_dim 128).
+//
+// Every row has a list of pages of its own, but rows that follow one another list nearly the same ones.  A CTA owns a tile of one
+// sequence and kv head, 256 rows of (token, query head of the group) in two groups of 128, and walks the pages that any of its
+// tokens lists, each once: its keys and values are fetched once for the tile.  For each of these pages a word of bits says which
+// tokens list it.  A group's products are issued for the pages its own tokens list; a warp none of whose tokens lists the
+// page writes zero weights without looking at the scores; a row that does not list it takes none of what its warp finds.
+//     S_g = Q_g K^T   (M 128, N 64 keys, K 128)   -> two S buffers of 64 columns per group
+//     O_g += P_g V    (M 128, N 128, K 64 keys)    -> one O buffer of 128 columns per group
+// Roles by warp: warp 0 loads queries and keys by TMA, the one behind the softmax warps the values, four pages deep each; one
+// thread each of warps 1-2 issues the scores products of group A and B, one each of warps 3-4 their values products; warps 5-8
+// and 9-12 are the softmax of group A and B (a thread a row, probabilities back into tensor memory as the second product's A
+// operand, O rescaled only when a row's maximum has grown by more than 2^8 since the scale in use was chosen).
+//
+// The heads of a group are rows of the tile (a group of G heads takes the next power of two: a tensor map of three dimensions
+// brings token after token, head after head), so that they share every page too.
+//
+// A weight of zero times an infinite or NaN value would not be zero.  The last warp looks through every page's values; if it
+// meets one that is not finite, the tile's rows are computed once more at the end, each over its own keys alone.
+//
+// Where there are few tiles, a cluster of CTAs shares one: each takes a stretch of the pages, and they join their rows through
+// distributed shared memory.  All barrier waits are bounded; one that gives up sets a status word and the CTA runs out.
+#include "tc5.cuh"
+#include "api.h"
+
+#include <cooperative_groups.h>
+#include <math.h>
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+__device__ int g_status;
+
+typedef __nv_bfloat16 bf16;
+constexpr int HD = 128, BQ = 128, GROUPS = 2, ROWS = GROUPS * BQ, BKV = 64, STAGES = 4;
+constexpr int FIRST_SOFTMAX_WARP = 1 + 2 * GROUPS;
+constexpr int VALUE_LOADER_WARP = FIRST_SOFTMAX_WARP + 4 * GROUPS, CHECKER_WARP = VALUE_LOADER_WARP + 1;
+constexpr int WARPS = CHECKER_WARP + 1, THREADS = WARPS * 32;
+constexpr int QPANEL = 128 * 128;               // 128 rows of 128 bytes (64 channels)
+constexpr int KPANEL = 64 * 128;                // 64 keys of 128 bytes
+constexpr int Q_BYTES = 2 * QPANEL, K_BYTES = 2 * KPANEL, V_BYTES = 2 * KPANEL, STAGE_BYTES = K_BYTES + V_BYTES;
+constexpr int TILE_BYTES = GROUPS * Q_BYTES + STAGES * STAGE_BYTES;
+constexpr int LIST_BYTES = 232448 - 3072 - 1024 - TILE_BYTES;   // for the tile's pages and their bits, beside the static part and the alignment
+constexpr int MAX_TABLE = 32768;                // pages of a sequence: their bitmap is made where the pages will go
+constexpr int TMEM_COLS = 512;                  // S: 2 groups x 2 buffers x 64; O: 2 groups x 128
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_AT = 8.0f;
+constexpr int MAX_PIECES = 8;
+static_assert(ROWS * HD * 4 <= STAGES * STAGE_BYTES, "a tile's sums fit where the pages were");
+
+// The tile: tokens, bits of a page's entry.
+__host__ __device__ inline int padded_group(int G) {
+    int gp = 1;
+    while (gp < G) gp *= 2;
+    return gp;
+}
+__host__ __device__ inline int tile_tokens(int gp) { return ROWS / gp; }
+__host__ __device__ inline int mask_words(int gp) { return tile_tokens(gp) > 32 ? tile_tokens(gp) / 32 : 1; }
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(s32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(s32(smem_dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(s32(bar))
+        : "memory");
+}
+// MN-major operand: the values' rows are keys, the second half of the head one panel further
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(KPANEL >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// D (+)= A B with A in tensor memory
+__device__ __forceinline__ void umma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+}
+
+// One (token, head) over its own keys alone, by a warp: the way of rows whose tile met a value that is not finite.
+__device__ __noinline__ void row_alone(const PagesParams& p, const int* bt, int row, int pos, int head, int kvh, int lane) {
+    const int* list = p.list + ((int64_t)row * p.kv_heads + kvh) * p.top;
+    const bf16* q = (const bf16*)p.q + (int64_t)row * p.q_row_stride + (int64_t)head * HD;
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < p.top; i++) {
+        const int lp = list[i];
+        if (lp < 0 || lp > pos / BKV) continue;
+        const int64_t off = (page_of(bt, lp * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * (int64_t)(BKV * HD);
+        const bf16 *k = (const bf16*)p.k_plane + off, *v = (const bf16*)p.v_plane + off;
+        const int n = min(BKV, pos + 1 - lp * BKV);
+        for (int half = 0; half < n; half += 32) {
+            float s = -INFINITY;
+            if (half + lane < n) {
+                s = 0.f;
+                for (int c = 0; c < HD; c++) s = fmaf(__bfloat162float(q[c]), __bfloat162float(k[(half + lane) * HD + c]), s);
+                s *= p.scale * LOG2E;
+            }
+            // A maximum that does not lose a NaN score.
+            float big = s;
+            for (int d = 16; d > 0; d >>= 1) {
+                const float other = __shfl_xor_sync(0xffffffffu, big, d);
+                big = other != other || big != big ? NAN : fmaxf(big, other);
+            }
+            const float now = big != big || m != m ? NAN : fmaxf(m, big);
+            const float base = now == -INFINITY ? 0.f : now, corr = exp2f(m - base), w = exp2f(s - base);
+            l = l * corr + warp_sum(w);
+            for (int e = 0; e < 4; e++) o[e] *= corr;
+            for (int t = 0; t < min(32, n - half); t++) {
+                const float wt = __shfl_sync(0xffffffffu, w, t);
+                for (int e = 0; e < 4; e++) o[e] = fmaf(wt, __bfloat162float(v[(half + t) * HD + lane * 4 + e]), o[e]);
+            }
+            m = now;
+        }
+    }
+    bf16* to = (bf16*)p.out + (int64_t)row * p.out_row_stride + (int64_t)head * HD + lane * 4;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    for (int e = 0; e < 4; e++) to[e] = __float2bfloat16_rn(o[e] * inv);
+}
+
+__global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                 const __grid_constant__ CUtensorMap map_v, PagesParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* Qs = base;                          // [GROUPS][Q_BYTES]
+    unsigned char* KVs = Qs + GROUPS * Q_BYTES;        // [STAGES][K | V]
+    __shared__ uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES];
+    __shared__ uint64_t s_full[GROUPS][2], p_full[GROUPS][2], o_done[GROUPS][2];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s, bad_s, n_s;
+    __shared__ float row_m[ROWS], row_l[ROWS];         // of a tile that several CTAs share
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int pieces = (int)cluster.num_blocks(), piece = (int)cluster.block_rank();
+    const int G = p.heads / p.kv_heads, GP = padded_group(G), TOK = tile_tokens(GP), TOKG = TOK / GROUPS, MW = mask_words(GP);
+    const int seq = blockIdx.z, kvh = blockIdx.y;
+    const int q_len = p.seq_q_len[seq], kv_len = p.seq_kv_len[seq];
+    const int q0 = ((int)blockIdx.x / pieces) * TOK;
+    if (q0 >= q_len) return;                           // the whole cluster leaves before anything is allocated
+    const int past = kv_len - q_len, q_start = p.seq_q_start[seq];
+    const int tokens = min(TOK, q_len - q0);
+    const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
+    int* entry = reinterpret_cast<int*>(KVs + STAGES * STAGE_BYTES);    // page | bit 30: group A lists it | bit 31: group B
+    const int cap = min(TOK * p.top, p.bt_stride);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(entry + cap);          // [entry][MW]: the tokens that list it
+
+    if (threadIdx.x == 0) {
+        mbar_init(&q_full, 1);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&k_empty[s], GROUPS);
+            mbar_init(&v_empty[s], GROUPS + 1);        // the values issuers and the checker
+        }
+        for (int g = 0; g < GROUPS; g++) {
+            for (int b = 0; b < 2; b++) {
+                mbar_init(&s_full[g][b], 1);
+                mbar_init(&p_full[g][b], 4);
+                mbar_init(&o_done[g][b], 1);
+            }
+        }
+        abort_s = bad_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        mbar_expect_tx(&q_full, GROUPS * Q_BYTES);
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) tma_load_3d(Qs + g * Q_BYTES + h * QPANEL, &map_q, h * 64, kvh * G, q_start + q0 + g * TOKG, &q_full);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(s32(&tmem_base_s)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    // The tile's pages in ascending order, and who lists them: a bitmap of the sequence's pages, the number of pages ahead of
+    // each of its words, then every list once more to set its token's bit.  The bitmap stands where the pages will go.
+    {
+        uint32_t* map = reinterpret_cast<uint32_t*>(KVs);
+        int* ahead = reinterpret_cast<int*>(map + MAX_TABLE / 32);
+        const int words = (p.bt_stride + 31) / 32;
+        const int* lists = p.list + ((int64_t)(q_start + q0) * p.kv_heads + kvh) * p.top;
+        auto each = [&](auto use) {
+            for (int i = threadIdx.x; i < tokens * p.top; i += THREADS) {
+                const int tok = i / p.top;
+                const int lp = lists[(int64_t)tok * p.kv_heads * p.top + (i - tok * p.top)];
+                if (lp >= 0 && lp <= (past + q0 + tok) / BKV && lp < p.bt_stride) use(tok, lp);
+            }
+        };
+        for (int i = threadIdx.x; i < words; i += THREADS) map[i] = 0;
+        __syncthreads();
+        each([&](int, int lp) { atomicOr(&map[lp >> 5], 1u << (lp & 31)); });
+        __syncthreads();
+        if (warp == 0) {
+            const int per = (words + 31) / 32, a = min(words, lane * per), b = min(words, a + per);
+            int own = 0;
+            for (int i = a; i < b; i++) own += __popc(map[i]);
+            int to = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, to, o);
+                if (lane >= o) to += v;
+            }
+            if (lane == 31) n_s = to;
+            to -= own;
+            for (int i = a; i < b; i++) {
+                ahead[i] = to;
+                to += __popc(map[i]);
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_s * MW; i += THREADS) bits[i] = 0;
+        for (int i = threadIdx.x; i < words; i += THREADS) {
+            int at = ahead[i];
+            for (uint32_t m = map[i]; m; m &= m - 1) entry[at++] = i * 32 + __ffs(m) - 1;
+        }
+        __syncthreads();
+        each([&](int tok, int lp) {
+            const int at = ahead[lp >> 5] + __popc(map[lp >> 5] & ((1u << (lp & 31)) - 1u));
+            atomicOr(&bits[at * MW + (tok >> 5)], 1u << (tok & 31));
+        });
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_s; i += THREADS) {
+            uint32_t a = 0, b = 0;
+            for (int w = 0; w < MW; w++) {
+                const uint32_t m = bits[i * MW + w];
+                if (MW > 1) {
+                    if (w < MW / 2) a |= m; else b |= m;
+                } else {
+                    const uint32_t low = (1u << TOKG) - 1u;    // a tile of at most 32 tokens: TOKG is at most 16
+                    a |= m & low;
+                    b |= m & ~low;
+                }
+            }
+            entry[i] |= (a ? 1 << 30 : 0) | (b ? (int)0x80000000u : 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const uint32_t tmem_base = tmem_base_s;
+    const int lo = (int)((int64_t)n_s * piece / pieces), n = (int)((int64_t)n_s * (piece + 1) / pieces) - lo;
+    entry += lo;
+    bits += lo * MW;
+    auto lists_it = [&](int j, int g) { return g ? entry[j] < 0 : (entry[j] & (1 << 30)) != 0; };
+
+    if (warp == 0 || warp == VALUE_LOADER_WARP) {
+        if (lane == 0) {
+            const bool keys = warp == 0;
+            uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+            int issued = 0;
+            for (int j = 0; j < n; j++) {
+                const int s = j % STAGES;
+                if (!mbar_wait_relaxed(&empty[s], ((uint32_t)(j / STAGES) & 1u) ^ 1u)) {
+                    atomicCAS(&g_status, 0, 1);
+                    abort_s = 1;
+                }
+                if (*(volatile int*)&abort_s) break;
+                mbar_expect_tx(&full[s], K_BYTES);
+                unsigned char* to = KVs + (size_t)s * STAGE_BYTES + (keys ? 0 : K_BYTES);
+                const int row = ((int)page_of(bt, (entry[j] & 0x3fffffff) * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * BKV;
+#pragma unroll
+                for (int h = 0; h < 2; h++) tma_load_2d(to + h * KPANEL, keys ? &map_k : &map_v, h * 64, row, &full[s]);
+                issued = j + 1;
+            }
+            if (*(volatile int*)&abort_s) {
+                for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; j++) mbar_wait(&full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+                if (keys) mbar_wait(&q_full, 0);
+            }
+        }
+    } else if (warp < FIRST_SOFTMAX_WARP) {
+        if (lane == 0) {
+            const int g = (warp - 1) % GROUPS;
+            const bool scores_role = warp - 1 < GROUPS;
+            bool ok = true;
+            int i = 0;        // pages of the group so far
+            if (scores_role) {
+                const uint32_t idesc = instr_desc(BQ, BKV);
+                ok = mbar_wait(&q_full, 0);
+                const uint64_t q_desc = smem_desc(s32(Qs + g * Q_BYTES)), k_desc = smem_desc(s32(KVs));
+                for (int j = 0; j < n && ok; j++) {
+                    ok = mbar_wait_relaxed(&k_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+                    if (ok && lists_it(j, g)) {
+                        const int b = i & 1;
+                        // the probabilities of the page before last lie in this buffer's columns until their product has read them
+                        if (i >= 2) ok = mbar_wait_relaxed(&o_done[g][b], (uint32_t)((i - 2) >> 1) & 1u);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                        const uint64_t kd = k_desc + (uint64_t)((j % STAGES) * (STAGE_BYTES >> 4));
+                        const uint32_t d_tmem = tmem_base + (uint32_t)(g * 128 + b * 64);
+#pragma unroll
+                        for (int ks = 0; ks < 8; ks++)
+                            umma(d_tmem, q_desc + (uint64_t)((ks >> 2) * (QPANEL >> 4) + (ks & 3) * 2),
+                                 kd + (uint64_t)((ks >> 2) * (KPANEL >> 4) + (ks & 3) * 2), idesc, ks > 0 ? 1u : 0u);
+                        umma_commit(&s_full[g][b]);
+                        i++;
+                    }
+                    if (ok) umma_commit(&k_empty[j % STAGES]);
+                }
+            } else {
+                const uint32_t idesc = instr_desc(BQ, HD) | (1u << 16);  // values enter MN-major
+                const uint64_t v_desc = smem_desc_mn(s32(KVs + K_BYTES));
+                for (int j = 0; j < n && ok; j++) {
+                    ok = mbar_wait_relaxed(&v_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+                    if (ok && lists_it(j, g)) {
+                        const int b = i & 1;
+                        ok = mbar_wait(&p_full[g][b], (uint32_t)(i >> 1) & 1u);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                        const uint64_t vd = v_desc + (uint64_t)((j % STAGES) * (STAGE_BYTES >> 4));
+                        const uint32_t d_tmem = tmem_base + (uint32_t)(256 + g * 128);
+#pragma unroll
+                        for (int kk = 0; kk < BKV / 16; kk++)
+                            umma_ta(d_tmem, tmem_base + (uint32_t)(g * 128 + b * 64 + kk * 8), vd + (uint64_t)(kk * ((16 * 128) >> 4)), idesc,
+                                    (i > 0 || kk > 0) ? 1u : 0u);
+                        umma_commit(&o_done[g][b]);
+                        i++;
+                    }
+                    if (ok) umma_commit(&v_empty[j % STAGES]);
+                }
+            }
+            if (!ok) {
+                atomicCAS(&g_status, 0, 3);
+                abort_s = 1;
+            }
+        }
+    } else if (warp == CHECKER_WARP) {
+        bool ok = true;
+        for (int j = 0; j < n && ok; j++) {
+            ok = mbar_wait_relaxed(&v_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+            if (!ok) break;
+            const uint4* v = reinterpret_cast<const uint4*>(KVs + (size_t)(j % STAGES) * STAGE_BYTES + K_BYTES);
+            __nv_bfloat162 most = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll 4
+            for (int c = lane; c < V_BYTES / 16; c += 32) {
+                const uint4 x = v[c];
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t a = w[e] & 0x7fff7fffu;
+                    most = __hmax2_nan(most, *reinterpret_cast<const __nv_bfloat162*>(&a));
+                }
+            }
+            const uint32_t m = *reinterpret_cast<const uint32_t*>(&most);
+            if ((m & 0x7fffu) >= 0x7f80u || ((m >> 16) & 0x7fffu) >= 0x7f80u) bad_s = 1;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_empty[j % STAGES]);
+        }
+        if (!ok && lane == 0) {
+            atomicCAS(&g_status, 0, 2);
+            abort_s = 1;
+        }
+    }
+    const int g = warp >= FIRST_SOFTMAX_WARP && warp < VALUE_LOADER_WARP ? (warp - FIRST_SOFTMAX_WARP) >> 2 : -1;   // a softmax warp's group
+    const int quad = warp & 3, r = quad * 32 + lane;          // row within the group
+    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+    const uint32_t o_addr = tmem_base + lane_addr + (uint32_t)(256 + (g > 0 ? g : 0) * 128);
+    const int tok = (g > 0 ? g : 0) * TOKG + r / GP, h = r % GP;
+    const bool row_ok = g >= 0 && tok < tokens && h < G;
+    float m_used = -INFINITY, l = 0.f;
+    int i = 0;             // pages of the group so far
+    if (g >= 0) {
+        const int pos = past + q0 + tok;
+        const float sc = p.scale * LOG2E;    // > 0
+        float m_run = -INFINITY;
+        bool ok = true;
+        for (int j = 0; j < n && ok; j++) {
+            if (!lists_it(j, g)) continue;
+            const int b = i & 1, key0 = (entry[j] & 0x3fffffff) * BKV;
+            const bool mine = (bits[j * MW + (tok >> 5)] >> (tok & 31)) & 1u;
+            const bool any = __any_sync(0xffffffffu, mine);
+            if (!mbar_wait(&s_full[g][b], (uint32_t)(i >> 1) & 1u)) {
+                ok = false;
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)(g * 128 + b * 64);
+            uint32_t pw[32];
+            if (!any) {
+                // scores of this buffer were issued behind the product of two pages ago: it may be written
+#pragma unroll
+                for (int e = 0; e < 32; e++) pw[e] = 0u;
+                tmem_st32(s_addr, pw);
+            } else {
+                uint32_t v0[32], v1[32];
+                tmem_ld32_nowait(s_addr, v0);
+                tmem_ld32_nowait(s_addr + 32u, v1);
+                tmem_wait_ld();
+                if (key0 + BKV - 1 > pos) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        if (key0 + e > pos) v0[e] = 0xff800000u;  // -inf
+                        if (key0 + 32 + e > pos) v1[e] = 0xff800000u;
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+#pragma unroll
+                    for (int f = 0; f < 4; f++) mx[f] = max3(mx[f], __uint_as_float(v0[e + f]), __uint_as_float(v1[e + f]));
+                const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+                if (mine) m_run = fmaxf(m_run, tile_max);
+                const bool grow = m_run > m_used + RESCALE_AT || (m_used == -INFINITY && m_run != -INFINITY);
+                if (__any_sync(0xffffffffu, grow && i > 0)) {
+                    // O_g may only be touched between products: wait for the previous page's
+                    if (!mbar_wait(&o_done[g][(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    const float f = (grow && i > 0) ? fast_exp2(m_used - m_run) : 1.f;  // m_used = -inf gives 0: O is all zeros then
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o_addr + (uint32_t)c0, o);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(o_addr + (uint32_t)c0, o);
+                    }
+                    l *= f;
+                }
+                if (grow) m_used = m_run;
+                const float mbase = m_used == -INFINITY ? 0.f : m_used;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 32; c++) {
+                    const uint32_t a = c < 16 ? v0[(c & 15) * 2] : v1[(c & 15) * 2], bb = c < 16 ? v0[(c & 15) * 2 + 1] : v1[(c & 15) * 2 + 1];
+                    const float p0 = fast_exp2(fmaf(__uint_as_float(a), sc, -mbase)), p1 = fast_exp2(fmaf(__uint_as_float(bb), sc, -mbase));
+                    sum[c & 3] += p0 + p1;
+                    const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
+                    pw[c] = mine ? *reinterpret_cast<const uint32_t*>(&h2) : 0u;
+                }
+                tmem_st32(s_addr, pw);
+                if (mine) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[g][b]);
+            i++;
+        }
+        if (ok && i > 0 && !mbar_wait(&o_done[g][(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) ok = false;
+        if (!ok) {
+            atomicCAS(&g_status, 0, 4);
+            abort_s = 1;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    }
+    __syncthreads();      // every role is done with the pages, and whether a value was not finite is known
+    const bool aborted = *(volatile int*)&abort_s != 0;
+    if (pieces == 1) {
+        if (g >= 0 && !aborted && !bad_s) {
+            const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;       // nothing seen: zeros; a NaN stays one
+            bf16* op = (bf16*)p.out + (int64_t)(q_start + q0 + tok) * p.out_row_stride + (int64_t)(kvh * G + h) * HD;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                uint32_t o[32];
+                if (i > 0) {
+                    tmem_ld32(o_addr + (uint32_t)c0, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0u;
+                }
+                if (row_ok) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int f = 0; f < 4; f++) {
+                            const __nv_bfloat162 a = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * f]) * inv, __uint_as_float(o[e + 2 * f + 1]) * inv);
+                            w[f] = *reinterpret_cast<const uint32_t*>(&a);
+                        }
+                        *reinterpret_cast<uint4*>(op + c0 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+        if (bad_s && !aborted)
+            for (int t = warp; t < tokens * G; t += WARPS)
+                row_alone(p, bt, q_start + q0 + t / G, past + q0 + t / G, kvh * G + t % G, kvh, lane);
+    } else {
+        // A row's 32 chunks of four channels stand in an order of their own (the chunk's number xor the row's), so that the
+        // threads of a warp, a row each, write to different banks.
+        float* sums = reinterpret_cast<float*>(KVs);
+        if (g >= 0) {
+            const int at = g * BQ + r;
+            row_m[at] = m_used;
+            row_l[at] = l;
+            if (i > 0) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + (uint32_t)c0, o);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        *reinterpret_cast<uint4*>(sums + (size_t)at * HD + (((c0 >> 2) + e) ^ (at & 31)) * 4) =
+                            make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+            }
+        }
+        cluster.sync();
+        bool bad = false, gone = false;
+        for (int w = 0; w < pieces; w++) {
+            bad |= *cluster.map_shared_rank(&bad_s, w) != 0;
+            gone |= *cluster.map_shared_rank(&abort_s, w) != 0;
+        }
+        for (int at = piece + warp * pieces; at < ROWS && !gone; at += WARPS * pieces) {
+            const int tk = (at / BQ) * TOKG + (at % BQ) / GP, hh = (at % BQ) % GP;
+            if (tk >= tokens || hh >= G) continue;
+            if (bad) {
+                row_alone(p, bt, q_start + q0 + tk, past + q0 + tk, kvh * G + hh, kvh, lane);
+                continue;
+            }
+            float m[MAX_PIECES], M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < MAX_PIECES; w++) {
+                if (w >= pieces) break;
+                m[w] = *cluster.map_shared_rank(&row_m[at], w);
+                M = fmaxf(M, m[w]);
+            }
+            float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < MAX_PIECES; w++) {
+                if (w >= pieces) break;
+                const float lw = *cluster.map_shared_rank(&row_l[at], w);
+                if (m[w] == -INFINITY && lw == 0.f) continue;      // this row saw nothing there (a NaN score leaves a NaN sum)
+                const float f = m[w] == -INFINITY ? 1.f : fast_exp2(m[w] - M);
+                const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums, w) + (size_t)at * HD + (lane ^ (at & 31)) * 4);
+                L += f * lw;
+                o[0] += f * x.x;
+                o[1] += f * x.y;
+                o[2] += f * x.z;
+                o[3] += f * x.w;
+            }
+            const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+            const __nv_bfloat162 a = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), b = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
+            bf16* op = (bf16*)p.out + (int64_t)(q_start + q0 + tk) * p.out_row_stride + (int64_t)(kvh * G + hh) * HD + lane * 4;
+            *reinterpret_cast<uint2*>(op) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        }
+        cluster.sync();     // a CTA's shared memory outlives its readers
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    Tc5EncodeTiledFn fn = tc5_encode_fn();
+    if (!fn) GB_REFUSE("attention_pages: the driver offers no cuTensorMapEncodeTiled");
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) GB_REFUSE("attention_pages: cuTensorMapEncodeTiled failed with code %d", (int)r);
+    return 0;
+}
+
+int list_bytes(const PagesParams& p) {
+    const int gp = padded_group(p.heads / p.kv_heads);
+    const int64_t most = (int64_t)tile_tokens(gp) * p.top;
+    const int cap = (int)(most < p.bt_stride ? most : p.bt_stride);
+    return cap * 4 * (1 + mask_words(gp));
+}
+
+}  // namespace
+
+// Whether this kernel takes the call: heads of 128 in groups of up to 128, 16-byte aligned rows, a positive scale, and a tile's
+// pages (those its tokens can list together) within the shared memory there is for them.
+int gb_attention_pages_tc5_accepts(const PagesParams& p) {
+    return p.d == HD && p.heads / p.kv_heads <= BQ && p.scale > 0.f && !((uintptr_t)p.q & 15) && !(p.q_row_stride & 7) && !((uintptr_t)p.out & 15) &&
+           !(p.out_row_stride & 7) && p.rows > 0 && p.bt_stride <= MAX_TABLE && (int64_t)p.pages * p.kv_heads * BKV <= 0x7fffffff &&
+           list_bytes(p) <= LIST_BYTES;
+}
+
+int gb_attention_pages_tc5(const PagesParams& p, int pieces, cudaStream_t stream) {
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(attn_pages_tc5_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_BYTES + 1024 + LIST_BYTES);
+        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", TILE_BYTES + LIST_BYTES, cudaGetErrorString(e));
+        configured = true;
+    }
+    const int G = p.heads / p.kv_heads, gp = padded_group(G), tok = tile_tokens(gp);
+    CUtensorMap map_q, map_k, map_v;
+    {
+        const cuuint64_t dims[3] = {HD, (cuuint64_t)p.heads, (cuuint64_t)p.rows}, strides[2] = {HD * 2, (cuuint64_t)p.q_row_stride * 2};
+        const cuuint32_t box[3] = {64, (cuuint32_t)gp, (cuuint32_t)(tok / GROUPS)};
+        if (int rc = make_map(&map_q, p.q, 3, dims, strides, box)) return rc;
+    }
+    {
+        const cuuint64_t dims[2] = {HD, (cuuint64_t)p.pages * p.kv_heads * BKV}, strides[1] = {HD * 2};
+        const cuuint32_t box[2] = {64, 64};
+        if (int rc = make_map(&map_k, p.k_plane, 2, dims, strides, box)) return rc;
+        if (int rc = make_map(&map_v, p.v_plane, 2, dims, strides, box)) return rc;
+    }
+    const dim3 grid(ceil_div(p.max_q_len, tok) * pieces, p.kv_heads, p.nseq);
+    if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("attention_pages: grid (%u, %u, %u) exceeds one launch", grid.x, grid.y, grid.z);
+    cudaError_t e = launch_pdl_cluster(attn_pages_tc5_kernel, grid, dim3(THREADS), (size_t)(TILE_BYTES + 1024 + list_bytes(p)), stream, pieces, 1, map_q, map_k, map_v, p);
+    if (e != cudaSuccess) GB_REFUSE("attention_pages: launch failed: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+GB_API int gb_attention_pages_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) cudaMemcpyToSymbol(g_status, &zero, sizeof(int));
+    return v;
+}
+
+// the checked build's record of the first index this file's kernels found out of bounds
+GB_CHECK_READER(gb_checked_status_attention_pages_tc5)

@@ -49,6 +49,7 @@ SOURCES = [
     "attention_mma.cu",
     "attention_tc5.cu",
     "attention_pages.cu",
+    "attention_pages_tc5.cu",
     "page_select.cu",
     "linear_state.cu",
     "delta_state.cu",

@@ -526,7 +526,8 @@ def checked_status():
     Always None in the ordinary build, whose kernels carry no checks.  Synchronises."""
     out = (c_int * 4)()
     for name in ("rows", "cache", "attention_simt", "attention_mma", "attention_tc5", "linear_state", "delta_state", "attention_sigmoid", "hyper", "postnorm", "attention_latent", "sandwich",
-                 "short_conv", "gated_delta", "page_select", "attention_pages"):
+                 "short_conv", "gated_delta", "page_select", "attention_pages",
+                 "attention_pages_tc5"):
         code = int(getattr(_lib, "gb_checked_status_" + name)(out))
         if code or out[3]:
             return name, _CHECK_NAMES.get(code, f"code {code}"), out[1], out[2], out[3]
@@ -536,7 +537,7 @@ def checked_status():
 def tc5_status() -> int:
     """0, or which role of a tcgen05 kernel gave up waiting on a barrier since the last call."""
     code = 0
-    for name in ("gb_gemm_tc5_status", "gb_gemm_tc5_decode_status", "gb_attention_tc5_status"):
+    for name in ("gb_gemm_tc5_status", "gb_gemm_tc5_decode_status", "gb_attention_tc5_status", "gb_attention_pages_status"):
         code = code or int(getattr(_lib, name)())
     return code
 

@@ -292,6 +292,27 @@ def test_attention_pages_passes_over_entries_that_name_nothing(ops, dtype):
     check_attention(s, out, plain)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=names)
+@pytest.mark.parametrize("top", [4, 24])
+def test_attention_pages_single_rows_beside_what_is_not_finite(ops, dtype, top):
+    """NaN keys and infinite values of listed pages come through, also where a row sees nothing else; those of others do not."""
+    s = Step([(1500, 1), (1500, 1), (1500, 1), (1500, 1)], 4, 2, 64, dtype, seed=6)
+    pages = torch.full((4, 2, top), -1, dtype=torch.int32)
+    pages[0, :, 0] = 5
+    pages[1, :, :4] = torch.tensor([1, 5, 7, 23])
+    pages[2, :, :4] = torch.tensor([1, 9, 11, 23])
+    pages[3, :, :2] = torch.tensor([2, 3])
+    for i, (plane, page, value) in enumerate([("k_plane", 5, math.nan), ("k_plane", 5, math.nan), ("v_plane", 9, -math.inf), ("v_plane", 4, math.nan)]):
+        s.dev[plane][s.table[s.slots[i], page]] = value
+    # behind the row's position, in its own page
+    for i in range(4):
+        s.dev["v_plane"][s.table[s.slots[i], 23], :, 1500 % PAGE + 1:] = math.nan
+        s.dev["k_plane"][s.table[s.slots[i], 23], :, 1500 % PAGE + 1:] = math.nan
+    out = s.attend(ops, pages.to(DEV)).cpu()
+    assert out[0].isnan().all() and out[1].isnan().all() and (out[2] == -math.inf).all() and out[3].isfinite().all()
+    check_attention(s, out, pages, rows={3})
+
+
 def test_all_pages_equal_full_attention(ops):
     """Lists of everything: what the attention over the whole cache gives, up to the rounding of the weights."""
     s = Step([(500, 1), (63, 1), (1000, 1)], 8, 2, 128, BF, seed=3)
@@ -302,6 +323,82 @@ def test_all_pages_equal_full_attention(ops):
     slot, start, q_len, kv_len = s.seq
     ops.attention(s.q_dev, full, s.dev["k_plane"], s.dev["v_plane"], s.dev["table"], slot, start, q_len, kv_len, s.nseq, 1, 8, 2, 128, 128 ** -0.5)
     assert float((out.float() - full.float()).abs().max()) <= 2 * 2.0 ** -8 * float(s.v_plane.float().abs().max())
+
+
+# ---- runs of rows on the tcgen05 kernel ---------------------------------------------------------
+def like_lists(s, top, seed, span, pool):
+    """Lists of rows that follow one another, nearly alike: every ``span`` rows a new set of ``pool`` pages, of which a row takes some."""
+    g = torch.Generator().manual_seed(seed)
+    pages = torch.full((s.q.shape[0], s.kvh, top), -1, dtype=torch.int32)
+    sets = {}
+    for i, pos, row in s.each_row():
+        own = pos // PAGE
+        for h in range(s.kvh):
+            key = (i, h, row // span)
+            if key not in sets:
+                sets[key] = torch.randperm(own + 1, generator=g)[:pool]
+            some = sets[key][torch.rand(len(sets[key]), generator=g) < 0.6].tolist()
+            pick = sorted(set([own] + some))[-top:]
+            pages[row, h, :len(pick)] = torch.tensor(pick, dtype=torch.int32)
+    return pages
+
+
+@pytest.mark.parametrize("heads,kvh", [(2, 2), (4, 2), (3, 1), (4, 1), (7, 1), (16, 2), (20, 1), (128, 1)])
+@pytest.mark.parametrize("seqs,top", [([(0, 16)], 4), ([(0, 150)], 5), ([(900, 70), (333, 1), (0, 33)], 9), ([(63, 2), (2000, 17)], 12)],
+                         ids=["least", "prompt", "three", "behind"])
+def test_attention_pages_runs(ops, heads, kvh, seqs, top):
+    s = Step(seqs, heads, kvh, 128, BF, seed=heads, more_rows=2, room=1)
+    pages = like_lists(s, top, heads, 12, 10)
+    out = s.attend(ops, pages.to(DEV))
+    assert ops.tc5_status() == 0
+    check_attention(s, out, pages, rows=set(range(0, s.rows, 3 if s.rows * heads > 500 else 1)) | {s.rows - 1})
+    assert (out[s.rows:] == 9.0).all()
+
+
+def test_attention_pages_runs_with_empty_lists(ops):
+    s = Step([(500, 40), (0, 20)], 4, 1, 128, BF, seed=1)
+    pages = random_lists(s, 6, 3, empty=True)
+    pages[5:30] = -1
+    out = s.attend(ops, pages.to(DEV))
+    check_attention(s, out, pages)
+    assert (out[5:30] == 0).all()
+    out = s.attend(ops, torch.full_like(pages, -1).to(DEV))
+    assert (out == 0).all() and ops.tc5_status() == 0
+
+
+@pytest.mark.parametrize("heads,kvh,new", [(4, 1, 150), (16, 8, 700)], ids=["shared tiles", "whole tiles"])
+@pytest.mark.parametrize("where", ["unlisted page", "another row's page", "behind the last token", "later token", "keys"])
+def test_attention_pages_runs_beside_values_that_are_not_finite(ops, heads, kvh, new, where):
+    """What a row does not see does not reach it, be it Inf or NaN; what it sees does."""
+    s = Step([(1000, new)], heads, kvh, 128, BF, seed=2, junk=math.nan if where == "behind the last token" else 0.0)
+    pages = like_lists(s, 8, 5, 12, 9)
+    clean = s.attend(ops, pages.to(DEV)).clone()
+    if where == "behind the last token":
+        assert (1000 + new) % PAGE
+        check_attention(s, clean, pages, rows={0, 3, new - 1, new - 2})
+        return
+    target = s.dev["k_plane"] if where == "keys" else s.dev["v_plane"]
+    mine = s.table[s.slots[0]]
+    if where == "later token":
+        pos = 1000 + new - 1
+        target[mine[pos // PAGE], :, pos % PAGE] = math.nan
+        sees = torch.zeros((new, kvh), dtype=torch.bool)
+        sees[new - 1] = (pages[new - 1] == pos // PAGE).any(-1)
+    else:
+        page = 3 if where != "unlisted page" else 1
+        if where == "unlisted page":
+            pages[pages == page] = -1
+            clean = s.attend(ops, pages.to(DEV)).clone()
+        target[mine[page]] = math.inf if where == "another row's page" else math.nan
+        sees = (pages == page).any(-1)
+        assert where == "unlisted page" or (sees.any() and not sees.all())
+    out = s.attend(ops, pages.to(DEV))
+    G = heads // kvh
+    got, ref = out.cpu().float().reshape(new, kvh, G * 128), clean.cpu().float().reshape(new, kvh, G * 128)
+    assert not got[sees].isfinite().any()
+    # the others: the same up to the rounding of the weights
+    assert float((got[~sees] - ref[~sees]).abs().max()) <= 4 * 2.0 ** -8 * float(s.v_plane.float().abs().max())
+    assert got[~sees].isfinite().all() and ops.tc5_status() == 0
 
 
 # ---- the three together ------------------------------------------------------------------------
