@@ -12,13 +12,17 @@
 // of them, a page above tau + 2 e is among the k best and one below tau - 2 e is not, whatever the errors were, and only the
 // pages between (as a rule the one at the border) are summed again in 64 bits, where a product of two bfloat16 values and
 // most of their sums are exact.  Pages that tie go by their number.
-#include "common.cuh"
+#include "mma.cuh"
 #include "api.h"
 
+#include <cooperative_groups.h>
 #include <math.h>
+
+#include <utility>
 
 namespace {
 
+namespace cg = cooperative_groups;
 typedef __nv_bfloat16 bf16;
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -99,275 +103,533 @@ __global__ void __launch_bounds__(BOUND_THREADS) page_bounds_kernel(PagesParams 
 }
 
 // ---- selection ---------------------------------------------------------------------------------
-constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
-constexpr int BAND = 512;              // pages near the border that are kept with their 64-bit scores
-
 __device__ __forceinline__ uint32_t order_key(float s) {
     const uint32_t b = __float_as_uint(s);
     return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ uint64_t order_key(double s) {
     const uint64_t b = (uint64_t)__double_as_longlong(s == 0.0 ? 0.0 : s);   // the two zeros are one score
     return b ^ ((b >> 63) ? 0xffffffffffffffffull : 0x8000000000000000ull);
 }
 
+// A row's candidates: pages c0 .. c0 + nc - 1 of its sequence, of which the k highest are wanted.
 template <typename T>
-struct SelectSmem {
-    double coef_d[2 * 256];      // [N | P], in the order of a page's bounds
-    double band_s[BAND];
-    float coef[2 * 256];
-    int band_i[BAND];
-    int hist[256];
-    int warp_a[SELECT_WARPS], warp_b[SELECT_WARPS];
-    float warp_e[SELECT_WARPS];
-    int digit, rest, above, n_band, unsafe;
+struct Row {
+    const T* q;              // the group's heads
+    int* list;
+    const int* bt;
+    int n, c0, nc, k;        // pages the row sees; candidates; wanted of them (fewer)
+    int kvh;
+    __device__ __forceinline__ const T* bounds(const PagesParams& p, int i) const {
+        return (const T*)p.bounds + (page_of(bt, (c0 + i) * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + kvh) * (2 * p.d);
+    }
+    // false: the row sees no more than `top` pages
+    __device__ __forceinline__ bool find(const PagesParams& p, int seq, int qi, int q_len, int head) {
+        kvh = head;
+        const int row = p.seq_q_start[seq] + qi, pos = p.seq_kv_len[seq] - q_len + qi;
+        list = p.list + ((int64_t)row * p.kv_heads + kvh) * p.top;
+        q = (const T*)p.q + (int64_t)row * p.q_row_stride + (int64_t)kvh * (p.heads / p.kv_heads) * p.d;
+        bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
+        n = pos / GB_PAGE + 1;
+        c0 = p.first;
+        nc = n - p.first - p.last;
+        k = p.top - p.first - p.last;
+        return n > p.top;
+    }
 };
 
-// Sum over a page's 2 d bounds in 64 bits by one warp; NaN counts as the lowest score.
-template <typename T>
-__device__ __forceinline__ double page_score(const T* b, const double* coef, int d2, int lane) {
-    double s = 0.0;
-    for (int i = lane; i < d2; i += 32)
-        if (coef[i] != 0.0) s += coef[i] * (double)to_f32<T>(b[i]);   // no head looks that way: nothing, also where the bound is infinite
+// P and N in 64 bits, in the registers of a warp: lane l holds channels l, l + 32, ...
+struct Coef64 {
+    double up[8], down[8];
+    template <typename T>
+    __device__ __forceinline__ void load(const PagesParams& p, const T* q, int lane) {
+        const int G = p.heads / p.kv_heads;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s == s ? s : -INFINITY;
-}
-
-// hist holds how many keys have each digit: the digit of the `want`-th highest key, and how many are wanted of those that have it
-__device__ __forceinline__ void pick_digit(int* hist, int want, int& digit, int& rest) {
-    // by the first warp: each lane sums 8 digits, from the highest down
-    const int lane = threadIdx.x;
-    int own = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) own += hist[255 - (lane * 8 + j)];
-    int before = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-    }
-    before -= own;
-    if (before < want && want <= before + own) {
-        int left = want - before;
         for (int j = 0; j < 8; j++) {
-            const int v = hist[255 - (lane * 8 + j)];
-            if (left <= v) {
-                digit = 255 - (lane * 8 + j);
-                rest = left;
-                break;
+            const int c = lane + 32 * j;
+            up[j] = down[j] = 0.0;
+            if (c >= p.d) break;
+            for (int h = 0; h < G; h++) {
+                const double x = (double)to_f32<T>(q[(int64_t)h * p.d + c]);
+                up[j] += x <= 0.0 ? 0.0 : x;      // a NaN is in both
+                down[j] += x >= 0.0 ? 0.0 : x;
             }
-            left -= v;
         }
     }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(SELECT_THREADS) select_pages_kernel(PagesParams p) {
-    constexpr int E = Chunk<T>::E, MOST = 16 / E;     // chunks a lane holds: 16 channels at most
-    extern __shared__ __align__(16) unsigned char raw[];
-    SelectSmem<T>& s = *reinterpret_cast<SelectSmem<T>*>(raw);
-    uint32_t* key = reinterpret_cast<uint32_t*>(raw + sizeof(SelectSmem<T>));   // [candidates]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_wait();
-    pdl_trigger();
-    const int seq = blockIdx.x / p.max_q_len, qi = blockIdx.x % p.max_q_len, kvh = blockIdx.y;
-    const int q_len = p.seq_q_len[seq];
-    if (qi >= q_len) return;
-    const int row = p.seq_q_start[seq] + qi, pos = p.seq_kv_len[seq] - q_len + qi;
-    int* list = p.list + ((int64_t)row * p.kv_heads + kvh) * p.top;
-    const int n = pos / GB_PAGE + 1;                      // pages that the row can see
-    if (n <= p.top) {
-        for (int i = tid; i < p.top; i += SELECT_THREADS) list[i] = i < n ? i : -1;
-        return;
-    }
-    const int c0 = p.first, nc = n - p.first - p.last, k = p.top - p.first - p.last;   // candidates; wanted of them: fewer
-    const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
-    const int d2 = 2 * p.d, G = p.heads / p.kv_heads;
-    const T* bounds = (const T*)p.bounds;
-    auto bounds_of = [&](int i) { return bounds + (page_of(bt, (c0 + i) * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + kvh) * d2; };
-
-    const T* q = (const T*)p.q + (int64_t)row * p.q_row_stride + (int64_t)kvh * G * p.d;
-    for (int c = tid; c < p.d; c += SELECT_THREADS) {
-        double up = 0.0, down = 0.0;
-        for (int h = 0; h < G; h++) {
-            const double x = (double)to_f32<T>(q[(int64_t)h * p.d + c]);
-            up += x <= 0.0 ? 0.0 : x;      // a NaN is in both
-            down += x >= 0.0 ? 0.0 : x;
+    // A page's score, the same in every lane; NaN counts as the lowest.  Where no head looks one way there is nothing to add, also
+    // where the bound is infinite.
+    template <typename T>
+    __device__ __forceinline__ double score(const T* b, int d, int lane) const {
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int c = lane + 32 * j;
+            if (c >= d) break;
+            if (down[j] != 0.0) s += down[j] * (double)to_f32<T>(b[c]);
+            if (up[j] != 0.0) s += up[j] * (double)to_f32<T>(b[d + c]);
         }
-        s.coef_d[c] = down;
-        s.coef_d[p.d + c] = up;
-        s.coef[c] = (float)down;
-        s.coef[p.d + c] = (float)up;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        return s == s ? s : -INFINITY;
     }
-    if (tid == 0) s.n_band = s.unsafe = 0;
-    __syncthreads();
-    // A page's 2 d values are 16-byte chunks; LP lanes share a page and hold their coefficients in registers.
-    {
-        const int NC = d2 / E;
-        int LP = 1;
-        while (LP < 32 && LP < NC) LP *= 2;
-        const int sub = lane / LP, l = lane % LP, per_warp = 32 / LP;
-        float cf[MOST][E];
+};
+
+// The choice from float32 scores, by a group of W warps.
+template <int W, int BAND>
+struct Chooser {
+    double band_s[BAND];
+    int band_i[BAND];        // pages near the border, kept with their 64-bit scores
+    int hist[256];
+    int warp_a[W], warp_b[W];
+    int digit, rest, above, n_band;
+
+    static __device__ __forceinline__ void sync() {
+        if (W == 1) __syncwarp(); else __syncthreads();
+    }
+    // hist holds how many keys have each digit: the digit of the `want`-th highest key, and how many are wanted of those that have it
+    __device__ __forceinline__ void pick(int want, int lane) {
+        int v[8], own = 0;      // each lane: 8 digits, from the highest down
 #pragma unroll
-        for (int j = 0; j < MOST; j++)
+        for (int j = 0; j < 8; j++) own += v[j] = hist[255 - (lane * 8 + j)];
+        int before = own;
 #pragma unroll
-            for (int e = 0; e < E; e++) cf[j][e] = l + j * LP < NC ? s.coef[(l + j * LP) * E + e] : 0.f;
-        float most = 0.f;     // of this lane's share of a page's sum of |terms|
-        bool odd = false;
-        for (int i0 = warp * per_warp; i0 < nc; i0 += SELECT_WARPS * per_warp) {
-            const int i = i0 + sub;
-            float acc = 0.f, mag = 0.f;
-            if (i < nc) {
-                const uint4* b = reinterpret_cast<const uint4*>(bounds_of(i));
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
+        }
+        before -= own;
+        if (before < want && want <= before + own) {
+            int left = want - before;
 #pragma unroll
-                for (int j = 0; j < MOST; j++) {
-                    if (l + j * LP >= NC) break;
-                    float x[E];
-                    unpack(b[l + j * LP], x);
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        acc = fmaf(cf[j][e], x[e], acc);
-                        mag = fmaf(fabsf(cf[j][e]), fabsf(x[e]), mag);
-                    }
+            for (int j = 0; j < 8; j++) {
+                if (left > 0 && left <= v[j]) {
+                    digit = 255 - (lane * 8 + j);
+                    rest = left;
+                }
+                left -= v[j];
+            }
+        }
+    }
+
+    // key[i]: the ordered float32 score of candidate i, off by no more than err; unsafe: they cannot be relied on.
+    template <typename T>
+    __device__ void run(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, bool unsafe, int tid) {
+        const int warp = tid >> 5, lane = tid & 31, NT = W * 32, nc = r.nc, k = r.k;
+        int ties_wanted = 0;
+        if (tid == 0) n_band = above = 0;
+        if (k > 0 && !unsafe) {
+            // tau: the k-th highest float32 score, digit by digit
+            uint32_t prefix = 0;
+            int want = k;
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                for (int i = tid; i < 256; i += NT) hist[i] = 0;
+                sync();
+                for (int i = tid; i < nc; i += NT) {
+                    const uint32_t v = key[i];
+                    if (shift == 24 || (v >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(v >> shift) & 255], 1);
+                }
+                sync();
+                if (warp == 0) pick(want, lane);
+                sync();
+                prefix |= (uint32_t)digit << shift;
+                want = rest;
+            }
+            const float tau = of_key(prefix);
+            const float hi = tau + 2.f * err + fabsf(tau) * 2.4e-7f, lo = tau - 2.f * err - fabsf(tau) * 2.4e-7f;
+            for (int i = tid; i < nc; i += NT) {
+                const float v = of_key(key[i]);
+                uint32_t mark = 0;
+                if (v > hi) {
+                    mark = 2;
+                    atomicAdd(&above, 1);
+                } else if (v >= lo) {
+                    const int at = atomicAdd(&n_band, 1);
+                    if (at < BAND) band_i[at] = i;
+                    mark = 2;      // until the band is settled
+                }
+                key[i] = mark;
+            }
+            sync();
+            const int m = n_band, wanted = k - above;
+            if (m > wanted && m <= BAND) {
+                Coef64 c;
+                c.load(p, r.q, lane);
+                for (int j = warp; j < m; j += W) {
+                    const double v = c.score(r.bounds(p, band_i[j]), p.d, lane);
+                    if (lane == 0) band_s[j] = v;
+                }
+                sync();
+                for (int j = tid; j < m; j += NT) {
+                    int better = 0;
+                    for (int o = 0; o < m; o++) better += band_s[o] > band_s[j] || (band_s[o] == band_s[j] && band_i[o] < band_i[j]);
+                    key[band_i[j]] = better < wanted ? 2 : 0;
                 }
             }
-            most = fmaxf(most, mag);
-            for (int o = LP / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-            odd = odd || !(fabsf(acc) <= 3.0e38f);
-            if (i < nc && l == 0) key[i] = order_key(acc);
+            sync();
         }
-        for (int o = LP / 2; o > 0; o >>= 1) most += __shfl_xor_sync(0xffffffffu, most, o);
-        most = warp_max(most);
-        if (lane == 0) s.warp_e[warp] = most;
-        if (odd || !(most <= 3.0e38f)) s.unsafe = 1;
+        if (k > 0 && (unsafe || n_band > BAND)) {
+            // Scores beyond float32, or hundreds that tie: the k-th highest of the 64-bit scores, which are summed anew for
+            // every digit.  Rare, and right for any input.
+            Coef64 c;
+            c.load(p, r.q, lane);
+            uint64_t prefix = 0;
+            int want = k;
+            for (int shift = 56; shift >= 0; shift -= 8) {
+                for (int i = tid; i < 256; i += NT) hist[i] = 0;
+                sync();
+                for (int i = warp; i < nc; i += W) {
+                    const uint64_t v = order_key(c.score(r.bounds(p, i), p.d, lane));
+                    if (lane == 0 && (shift == 56 || (v >> (shift + 8)) == (prefix >> (shift + 8)))) atomicAdd(&hist[(int)(v >> shift) & 255], 1);
+                }
+                sync();
+                if (warp == 0) pick(want, lane);
+                sync();
+                prefix |= (uint64_t)digit << shift;
+                want = rest;
+            }
+            for (int i = warp; i < nc; i += W) {
+                const uint64_t v = order_key(c.score(r.bounds(p, i), p.d, lane));
+                if (lane == 0) key[i] = v > prefix ? 2 : v == prefix ? 1 : 0;
+            }
+            ties_wanted = want;
+            sync();
+        }
+        // the chosen pages in order, a page a thread at a time; of those that tie the first
+        int sure_to = 0, tie_to = 0;
+        for (int i0 = 0; i0 < r.n; i0 += NT) {
+            const int i = i0 + tid, ci = i - r.c0;
+            const uint32_t m = i >= r.n ? 0u : ci < 0 || ci >= nc ? 2u : k > 0 ? key[ci] : 0u;
+            const unsigned sure = __ballot_sync(0xffffffffu, m == 2), tie = __ballot_sync(0xffffffffu, m == 1), below = (1u << lane) - 1u;
+            int s_at = sure_to, t_at = tie_to;
+            if (W > 1) {
+                if (lane == 0) {
+                    warp_a[warp] = __popc(sure);
+                    warp_b[warp] = __popc(tie);
+                }
+                sync();
+                for (int w = 0; w < W; w++) {
+                    if (w < warp) {
+                        s_at += warp_a[w];
+                        t_at += warp_b[w];
+                    }
+                    sure_to += warp_a[w];
+                    tie_to += warp_b[w];
+                }
+                sync();
+            } else {
+                sure_to += __popc(sure);
+                tie_to += __popc(tie);
+            }
+            s_at += __popc(sure & below);
+            t_at += __popc(tie & below);
+            if (m == 2 || (m == 1 && t_at < ties_wanted)) r.list[s_at + min(t_at, ties_wanted)] = i;
+        }
+        sync();     // before the group's next row
     }
-    __syncthreads();
-    float err = 0.f;
+};
+
+// Single rows ----------------------------------------------------------------------------------
+// A cluster of CTAs scores one (row, kv head): each takes a stretch of the pages and leaves their scores in the first one's shared
+// memory, which then chooses.  A page's 2 d bounds are 16-byte chunks, LP lanes share them, CPL chunks a lane, and hold their
+// coefficients in registers; a warp asks for eight chunks a lane before it adds anything up.
+constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
+constexpr int MAX_PIECES = 8;
+constexpr int ROW_BAND = 512;
+
+struct SelectSmem {
+    Chooser<SELECT_WARPS, ROW_BAND> choose;
+    float coef[2 * 256];                        // [N | P], in the order of a page's bounds
+    float err[MAX_PIECES * SELECT_WARPS];       // of every warp of the cluster; a NaN: unsafe
+};
+
+template <int N, int LP>
+__device__ __forceinline__ float sum_many(float (&v)[N], int lane) {
+    // The sums of N values over LP lanes (both powers of two): half of the values go to the other half of the lanes, until a
+    // lane has one; lane l ends with value l / (LP / N) of the group's (N <= LP)
+    if constexpr (N == 1) {
 #pragma unroll
-    for (int w = 0; w < SELECT_WARPS; w++) err = fmaxf(err, s.warp_e[w]);
-    // A float32 sum of at most 16 products a lane and 5 steps between lanes, of coefficients rounded once: 22 half steps of 2^-23
-    // relative to the sum of the terms' sizes, itself known to 2^-18; products below the normal range add next to nothing.
-    err = err * (24.f * 5.9604645e-8f) + 1.0e-42f;
-    const bool unsafe = s.unsafe != 0;
-    int ties_wanted = 0;
-    if (k > 0 && !unsafe) {
-        // tau: the k-th highest float32 score, digit by digit
-        uint32_t prefix = 0;
-        int want = k;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            s.hist[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < nc; i += SELECT_THREADS)
-                if (shift == 24 || (key[i] >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s.hist[(key[i] >> shift) & 255], 1);
-            __syncthreads();
-            if (warp == 0) pick_digit(s.hist, want, s.digit, s.rest);
-            __syncthreads();
-            prefix |= (uint32_t)s.digit << shift;
-            want = s.rest;
-        }
-        const float tau = __uint_as_float(prefix ^ ((prefix >> 31) ? 0x80000000u : 0xffffffffu));
-        const float hi = tau + 2.f * err + fabsf(tau) * 2.4e-7f, lo = tau - 2.f * err - fabsf(tau) * 2.4e-7f;
-        if (tid == 0) s.above = 0;
-        __syncthreads();
-        for (int i = tid; i < nc; i += SELECT_THREADS) {
-            const uint32_t kb = key[i];
-            const float v = __uint_as_float(kb ^ ((kb >> 31) ? 0x80000000u : 0xffffffffu));
-            uint32_t mark = 0;
-            if (v > hi) {
-                mark = 2;
-                atomicAdd(&s.above, 1);
-            } else if (v >= lo) {
-                const int at = atomicAdd(&s.n_band, 1);
-                if (at < BAND) s.band_i[at] = i;
-                mark = 2;      // until the band is settled
-            }
-            key[i] = mark;
-        }
-        __syncthreads();
-        const int m = s.n_band, wanted = k - s.above;
-        if (m > wanted && m <= BAND) {
-            for (int j = warp; j < m; j += SELECT_WARPS) {
-                const double v = page_score<T>(bounds_of(s.band_i[j]), s.coef_d, d2, lane);
-                if (lane == 0) s.band_s[j] = v;
-            }
-            __syncthreads();
-            for (int j = tid; j < m; j += SELECT_THREADS) {
-                int better = 0;
-                for (int o = 0; o < m; o++)
-                    better += s.band_s[o] > s.band_s[j] || (s.band_s[o] == s.band_s[j] && s.band_i[o] < s.band_i[j]);
-                key[s.band_i[j]] = better < wanted ? 2 : 0;
-            }
-        }
-        __syncthreads();
-    }
-    if (k > 0 && (unsafe || s.n_band > BAND)) {
-        // Scores beyond float32, or hundreds that tie: the k-th highest of the 64-bit scores, which are summed anew for
-        // every digit.  Rare, and right for any input.
-        uint64_t prefix = 0;
-        int want = k;
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            s.hist[tid] = 0;
-            __syncthreads();
-            for (int i = warp; i < nc; i += SELECT_WARPS) {
-                const uint64_t v = order_key(page_score<T>(bounds_of(i), s.coef_d, d2, lane));
-                if (lane == 0 && (shift == 56 || (v >> (shift + 8)) == (prefix >> (shift + 8)))) atomicAdd(&s.hist[(int)(v >> shift) & 255], 1);
-            }
-            __syncthreads();
-            if (warp == 0) pick_digit(s.hist, want, s.digit, s.rest);
-            __syncthreads();
-            prefix |= (uint64_t)s.digit << shift;
-            want = s.rest;
-        }
-        for (int i = warp; i < nc; i += SELECT_WARPS) {
-            const uint64_t v = order_key(page_score<T>(bounds_of(i), s.coef_d, d2, lane));
-            if (lane == 0) key[i] = v > prefix ? 2 : v == prefix ? 1 : 0;
-        }
-        ties_wanted = want;
-        __syncthreads();
-    }
-    // the chosen pages in order: each thread counts a stretch of the pages
-    auto kind = [&](int page) -> uint32_t {
-        if (page < c0 || page >= c0 + nc) return 2;
-        return k > 0 ? key[page - c0] : 0;
-    };
-    const int per = (n + SELECT_THREADS - 1) / SELECT_THREADS;
-    const int a = min(n, tid * per), b = min(n, a + per);
-    int sure = 0, tie = 0;
-    for (int i = a; i < b; i++) {
-        const uint32_t m = kind(i);
-        sure += m == 2;
-        tie += m == 1;
-    }
-    int sure_to = sure, tie_to = tie;
+        for (int o = LP / 2; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+        return v[0];
+    } else {
+        float half[N / 2];
+        const bool upper = lane & (LP / 2);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, sure_to, o), y = __shfl_up_sync(0xffffffffu, tie_to, o);
-        if (lane >= o) {
-            sure_to += x;
-            tie_to += y;
+        for (int j = 0; j < N / 2; j++) {
+            const float give = upper ? v[j] : v[j + N / 2], keep = upper ? v[j + N / 2] : v[j];
+            half[j] = keep + __shfl_xor_sync(0xffffffffu, give, LP / 2);
         }
-    }
-    if (lane == 31) {
-        s.warp_a[warp] = sure_to;
-        s.warp_b[warp] = tie_to;
-    }
-    __syncthreads();
-    sure_to -= sure;
-    tie_to -= tie;
-    for (int w = 0; w < warp; w++) {
-        sure_to += s.warp_a[w];
-        tie_to += s.warp_b[w];
-    }
-    for (int i = a; i < b; i++) {
-        const uint32_t m = kind(i);
-        if (m == 2 || (m == 1 && tie_to < ties_wanted)) list[sure_to + min(tie_to, ties_wanted)] = i;
-        sure_to += m == 2;
-        tie_to += m == 1;
+        return sum_many<N / 2, LP / 2>(half, lane);
     }
 }
 
-constexpr int MAX_PAGES = 32768;   // of a sequence: their scores stand in shared memory
+template <typename T, int LP, int CPL>
+__global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams p) {
+    constexpr int E = Chunk<T>::E, U = 8 / CPL, PER_WARP = 32 / LP;     // pages a group of LP lanes takes at a time
+    extern __shared__ __align__(16) unsigned char raw[];
+    SelectSmem& s = *reinterpret_cast<SelectSmem*>(raw);
+    uint32_t* key = reinterpret_cast<uint32_t*>(raw + sizeof(SelectSmem));   // [candidates]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int pieces = (int)cluster.num_blocks(), piece = (int)cluster.block_rank();
+    pdl_wait();
+    pdl_trigger();
+    const int unit = blockIdx.x / pieces, seq = unit / p.max_q_len, qi = unit % p.max_q_len;
+    const int q_len = p.seq_q_len[seq];
+    if (qi >= q_len) return;                    // the whole cluster
+    Row<T> r;
+    if (!r.find(p, seq, qi, q_len, blockIdx.y)) {
+        if (piece == 0)
+            for (int i = tid; i < p.top; i += SELECT_THREADS) r.list[i] = i < r.n ? i : -1;
+        return;
+    }
+    auto started = cluster.barrier_arrive();    // waited for before the first CTA's memory is written
+    const int d2 = 2 * p.d, G = p.heads / p.kv_heads;
+    for (int c = tid; c < p.d; c += SELECT_THREADS) {
+        float up = 0.f, down = 0.f;
+        for (int h = 0; h < G; h++) {
+            const float x = to_f32<T>(r.q[(int64_t)h * p.d + c]);
+            up += x <= 0.f ? 0.f : x;      // a NaN is in both
+            down += x >= 0.f ? 0.f : x;
+        }
+        s.coef[c] = down;
+        s.coef[p.d + c] = up;
+    }
+    __syncthreads();
+    cluster.barrier_wait(std::move(started));
+    const int NC = d2 / E, sub = lane / LP, l = lane % LP;
+    float cf[CPL][E], mx[CPL][E];
+#pragma unroll
+    for (int j = 0; j < CPL; j++)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            cf[j][e] = l + j * LP < NC ? s.coef[(l + j * LP) * E + e] : 0.f;
+            mx[j][e] = 0.f;
+        }
+    uint32_t* keys0 = cluster.map_shared_rank(key, 0);
+    bool odd = false;
+    const T* plane = (const T*)p.bounds;
+    constexpr int BATCH = U * PER_WARP;
+    for (int i0 = (piece * SELECT_WARPS + warp) * BATCH; i0 < r.nc; i0 += pieces * SELECT_WARPS * BATCH) {
+        int64_t page = 0;
+        if (lane < BATCH && i0 + lane < r.nc) page = page_of(r.bt, (r.c0 + i0 + lane) * GB_PAGE, p.bt_stride, p.pages);
+        uint4 x[U][CPL];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            // pages beyond the last are the sequence's last once more
+            const int at = min(sub * U + u, r.nc - 1 - i0);
+            const int64_t pg = __shfl_sync(0xffffffffu, page, at);
+            const uint4* b = reinterpret_cast<const uint4*>(plane + (pg * p.kv_heads + r.kvh) * d2);
+#pragma unroll
+            for (int j = 0; j < CPL; j++)
+                if (l + j * LP < NC) x[u][j] = b[l + j * LP];
+        }
+        float acc[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            acc[u] = 0.f;
+#pragma unroll
+            for (int j = 0; j < CPL; j++) {
+                if (l + j * LP >= NC) break;
+                float f[E];
+                unpack(x[u][j], f);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    acc[u] = fmaf(cf[j][e], f[e], acc[u]);
+                    mx[j][e] = fmaxf(mx[j][e], fabsf(f[e]));
+                }
+            }
+        }
+        const float sum = sum_many<U, LP>(acc, lane);
+        constexpr int SHARE = LP / U;                     // lanes that end with the same page
+        const int i = i0 + sub * U + l / SHARE;
+        odd = odd || !(fabsf(sum) <= 3.0e38f);
+        if (l % SHARE == 0 && i < r.nc) keys0[i] = order_key(sum);
+    }
+    float most = 0.f;      // the sum of the terms' sizes is no more than that of the coefficients times the channels' largest bounds
+#pragma unroll
+    for (int j = 0; j < CPL; j++)
+#pragma unroll
+        for (int e = 0; e < E; e++) most = fmaf(fabsf(cf[j][e]), mx[j][e], most);
+    if (odd || !(most <= 3.0e38f)) most = NAN;
+#pragma unroll
+    for (int o = LP / 2; o > 0; o >>= 1) most += __shfl_xor_sync(0xffffffffu, most, o);
+#pragma unroll
+    for (int o = 16; o >= LP; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, most, o);
+        most = most <= other || other != other ? other : most;
+    }
+    if (lane == 0) cluster.map_shared_rank(s.err, 0)[piece * SELECT_WARPS + warp] = most;
+    cluster.sync();
+    if (piece != 0) return;
+    float err = 0.f;
+    bool unsafe = false;
+    for (int w = 0; w < pieces * SELECT_WARPS; w++) {
+        err = fmaxf(err, s.err[w]);
+        unsafe = unsafe || !(s.err[w] <= 3.0e38f);
+    }
+    // A float32 sum of at most 16 products a lane and 5 steps between lanes, of coefficients that are sums of G values: 22 + G half steps
+    // of 2^-23 relative to the sum of the terms' sizes, itself known to 2^-18; products below the normal range add next to nothing.
+    err = err * ((24.f + (float)G) * 5.9604645e-8f) + 1.0e-42f;
+    s.choose.run(p, r, key, err, unsafe, tid);
+}
+
+// Runs of rows -----------------------------------------------------------------------------------
+// A CTA takes RT rows of one sequence and kv head and scores all their candidate pages as one product on mma.sync: the rows'
+// coefficients, each as the sum of two bfloat16 values (2^-17 relative), against the pages' bounds, which come from the cache
+// straight into the fragments.  The channels of a block of 32 are dealt to the k steps so that a lane's share of a page is 16
+// consecutive bytes; the coefficients are read in the same order.  The scores stand in shared memory, a warp chooses for a row.
+constexpr int TILE_THREADS = 512, TILE_WARPS = TILE_THREADS / 32, TILE_BAND = 48;
+
+struct alignas(16) TileSmem {
+    Chooser<1, TILE_BAND> choose[TILE_WARPS];
+    float size[64];          // per chunk of 8 bounds: their largest size, over all pages
+};
+
+__host__ __device__ inline int tile_coef_stride(int d) { return 2 * d + 32; }        // elements: rows 64 bytes of banks apart
+__host__ __device__ inline int tile_key_stride(int pages) { return (pages + 31) / 32 * 32 + 8; }
+
+template <int MT>
+__global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParams p) {
+    constexpr int RT = MT * 16;
+    extern __shared__ __align__(16) unsigned char raw[];
+    TileSmem& s = *reinterpret_cast<TileSmem*>(raw);
+    const int CS = tile_coef_stride(p.d), KS = tile_key_stride(p.bt_stride);
+    bf16* coef = reinterpret_cast<bf16*>(raw + sizeof(TileSmem));                    // [2][RT][CS]
+    uint32_t* keys = reinterpret_cast<uint32_t*>(coef + 2 * RT * CS);                // [RT][KS]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    pdl_wait();
+    pdl_trigger();
+    const int seq = blockIdx.z, kvh = blockIdx.y, q0 = blockIdx.x * RT;
+    const int q_len = p.seq_q_len[seq];
+    if (q0 >= q_len) return;
+    const int rows = min(RT, q_len - q0), d = p.d, G = p.heads / p.kv_heads;
+    const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
+    // candidates of the last row, which has the most
+    const int nc = (p.seq_kv_len[seq] - q_len + q0 + rows - 1) / GB_PAGE + 1 - p.first - p.last;
+    {
+        const bf16* q = (const bf16*)p.q + (int64_t)(p.seq_q_start[seq] + q0) * p.q_row_stride + (int64_t)kvh * G * d;
+        for (int i = tid; i < RT * (d / 2); i += TILE_THREADS) {
+            const int row = i / (d / 2), c = (i - row * (d / 2)) * 2;
+            float up[2] = {0.f, 0.f}, down[2] = {0.f, 0.f};
+            if (row < rows)
+                for (int h = 0; h < G; h++) {
+                    const bf16* at = q + (int64_t)row * p.q_row_stride + h * d + c;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float x = __bfloat162float(at[e]);
+                        up[e] += x <= 0.f ? 0.f : x;
+                        down[e] += x >= 0.f ? 0.f : x;
+                    }
+                }
+            bf16* to = coef + row * CS + c;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const bf16 dh = __float2bfloat16_rn(down[e]), uh = __float2bfloat16_rn(up[e]);
+                to[e] = dh;
+                to[d + e] = uh;
+                to[RT * CS + e] = __float2bfloat16_rn(down[e] - __bfloat162float(dh));
+                to[RT * CS + d + e] = __float2bfloat16_rn(up[e] - __bfloat162float(uh));
+            }
+        }
+        for (int i = tid; i < 64; i += TILE_THREADS) s.size[i] = 0.f;
+    }
+    __syncthreads();
+    const int KB = d / 16;             // blocks of 32 bounds
+    const bf16* plane = (const bf16*)p.bounds;
+    __nv_bfloat162 size[16];           // of each block: the largest this lane has met in its chunk of 8
+#pragma unroll
+    for (int kb = 0; kb < 16; kb++) size[kb] = __floats2bfloat162_rn(0.f, 0.f);
+    for (int i0 = warp * 16; i0 < nc; i0 += TILE_WARPS * 16) {
+        const bf16* b[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int i = min(i0 + t * 8 + g, nc - 1);         // pages beyond the last are the last once more
+            b[t] = plane + (page_of(bt, (p.first + i) * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + kvh) * (2 * d) + t4 * 8;
+        }
+        float acc[MT][2][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[m][t][e] = 0.f;
+#pragma unroll
+        for (int half = 0; half < 4; half++) {                 // blocks in fours: what a lane asks for at once
+            if (half * 4 >= KB) break;
+            uint4 x[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    if (half * 4 + j < KB) x[j][t] = *reinterpret_cast<const uint4*>(b[t] + (half * 4 + j) * 32);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int kb = half * 4 + j;
+                if (kb >= KB) break;
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const uint32_t w[4] = {x[j][t].x, x[j][t].y, x[j][t].z, x[j][t].w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t a = w[e] & 0x7fff7fffu;
+                        size[kb] = __hmax2_nan(size[kb], *reinterpret_cast<const __nv_bfloat162*>(&a));
+                    }
+                }
+#pragma unroll
+                for (int term = 0; term < 2; term++)
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        const bf16* a = coef + (term * RT + m * 16 + g) * CS + kb * 32 + t4 * 8;
+                        const uint4 a0 = *reinterpret_cast<const uint4*>(a), a1 = *reinterpret_cast<const uint4*>(a + 8 * CS);
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            mma_bf16_16816(acc[m][t], a0.x, a1.x, a0.y, a1.y, x[j][t].x, x[j][t].y);
+                            mma_bf16_16816(acc[m][t], a0.z, a1.z, a0.w, a1.w, x[j][t].z, x[j][t].w);
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int i = i0 + t * 8 + t4 * 2;             // KS has room for whole blocks of 16
+                *reinterpret_cast<uint2*>(keys + (m * 16 + g) * KS + i) = make_uint2(order_key(acc[m][t][0]), order_key(acc[m][t][1]));
+                *reinterpret_cast<uint2*>(keys + (m * 16 + g + 8) * KS + i) = make_uint2(order_key(acc[m][t][2]), order_key(acc[m][t][3]));
+            }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 16; kb++) {
+        if (kb >= KB) break;
+        const float lo = __low2float(size[kb]), hi = __high2float(size[kb]);
+        float v = lo != lo || hi != hi ? INFINITY : fmaxf(lo, hi);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (g == 0) atomicMax(reinterpret_cast<int*>(&s.size[kb * 4 + t4]), __float_as_int(v));   // not negative: ordered as integers
+    }
+    __syncthreads();
+    for (int row = warp; row < rows; row += TILE_WARPS) {
+        Row<bf16> r;
+        if (!r.find(p, seq, q0 + row, q_len, kvh)) {
+            for (int i = lane; i < p.top; i += 32) r.list[i] = i < r.n ? i : -1;
+            continue;
+        }
+        // The coefficients are good to 2^-18 (3.9e-6) and G half steps of 2^-23, their products' sums on the tensor cores to 6 units of 2^-23
+        // for each of 4 d / 16 steps (16 products and the sum so far, cut off behind 25 bits of the largest of them, and the result).
+        // All relative to the sum of the terms' sizes; what is below the normal range of a coefficient's second part is let in by 1e-35.
+        float most = 0.f;
+        for (int c = lane; c < 2 * d; c += 32) most = fmaf(fabsf(__bfloat162float(coef[row * CS + c])) + 1.0e-35f, s.size[c >> 3], most);
+        most = warp_sum(most);
+        const bool unsafe = !(most <= 1.0e38f);
+        const float err = most * (1.02f * (3.9e-6f + (float)d * 1.8e-7f + (float)G * 5.9604645e-8f)) + 1.0e-42f;
+        s.choose[warp].run(p, r, keys + row * KS, err, unsafe, lane);
+    }
+}
+
+constexpr int MAX_PAGES = 32768;        // of a sequence: their scores stand in shared memory
+constexpr int MAX_TILE_SMEM = 232448;   // what a CTA can have
+constexpr int TILE_MIN_ROWS = 8;        // rows of a sequence from which on they are scored as tiles
 
 int check(const PagesParams& p, int dtype, const char* who) {
     if (dtype != GB_F32 && dtype != GB_BF16) GB_REFUSE("%s: dtype code %d", who, dtype);
@@ -397,18 +659,42 @@ GB_API int gb_page_bounds(const PagesParams* pp, int dtype, cudaStream_t stream)
     return 0;
 }
 
-template <typename T>
-static int launch_select(const PagesParams& p, cudaStream_t stream) {
-    const size_t smem = sizeof(SelectSmem<T>) + (size_t)p.bt_stride * sizeof(uint32_t);
+template <typename T, int LP, int CPL>
+static int launch_rows(const PagesParams& p, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(select_pages_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)(sizeof(SelectSmem<T>) + MAX_PAGES * sizeof(uint32_t)));
+        const cudaError_t e = cudaFuncSetAttribute(select_row_kernel<T, LP, CPL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)(sizeof(SelectSmem) + MAX_PAGES * sizeof(uint32_t)));
         if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
         configured = true;
     }
-    if (p.kv_heads > 65535 || (int64_t)p.nseq * p.max_q_len > 0x7fffffff) GB_REFUSE("select_pages: %d sequences of up to %d rows exceed one launch", p.nseq, p.max_q_len);
-    launch_pdl(select_pages_kernel<T>, dim3(p.nseq * p.max_q_len, p.kv_heads), dim3(SELECT_THREADS), smem, stream, p);
+    // pieces of no fewer pages than the CTA's warps take at a time, while they all run at once
+    const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads;
+    int pieces = 1;
+    while (pieces < MAX_PIECES && units * pieces * 2 <= 4 * gb_sm_count() && p.bt_stride > pieces * SELECT_WARPS * 8) pieces *= 2;
+    const int64_t x = (int64_t)p.nseq * p.max_q_len * pieces;
+    if (p.kv_heads > 65535 || x > 0x7fffffff) GB_REFUSE("select_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
+    launch_pdl_cluster(select_row_kernel<T, LP, CPL>, dim3((unsigned)x, p.kv_heads), dim3(SELECT_THREADS), sizeof(SelectSmem) + (size_t)p.bt_stride * sizeof(uint32_t),
+                       stream, pieces, 1, p);
+    GB_CHECK_LAUNCH("select_pages");
+    return 0;
+}
+
+static int64_t tile_smem(const PagesParams& p, int rt) {
+    return (int64_t)sizeof(TileSmem) + 2 * rt * tile_coef_stride(p.d) * 2 + (int64_t)rt * tile_key_stride(p.bt_stride) * 4;
+}
+
+template <int MT>
+static int launch_tiles(const PagesParams& p, cudaStream_t stream) {
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(select_tile_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_TILE_SMEM);
+        if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
+        configured = true;
+    }
+    const dim3 grid(ceil_div(p.max_q_len, MT * 16), p.kv_heads, p.nseq);
+    if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("select_pages: %d kv heads, %d sequences exceed one launch", p.kv_heads, p.nseq);
+    launch_pdl(select_tile_kernel<MT>, grid, dim3(TILE_THREADS), (size_t)tile_smem(p, MT * 16), stream, p);
     GB_CHECK_LAUNCH("select_pages");
     return 0;
 }
@@ -420,7 +706,20 @@ GB_API int gb_select_pages(const PagesParams* pp, int dtype, cudaStream_t stream
     if (p.heads <= 0 || p.heads % p.kv_heads) GB_REFUSE("select_pages: %d heads over %d kv heads", p.heads, p.kv_heads);
     if (p.first < 0 || p.last < 1 || p.first + p.last > p.top) GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
     if (p.bt_stride > MAX_PAGES) GB_REFUSE("select_pages: sequences of up to %d pages; this kernel takes %d", p.bt_stride, MAX_PAGES);
-    return dtype == GB_F32 ? launch_select<float>(p, stream) : launch_select<bf16>(p, stream);
+    if (dtype == GB_BF16 && p.max_q_len >= TILE_MIN_ROWS && p.d % 16 == 0) {
+        if (p.max_q_len > 16 && tile_smem(p, 32) <= MAX_TILE_SMEM) return launch_tiles<2>(p, stream);
+        if (tile_smem(p, 16) <= MAX_TILE_SMEM) return launch_tiles<1>(p, stream);
+    }
+    const int chunks = 2 * p.d / (dtype == GB_F32 ? 4 : 8);
+    if (dtype == GB_F32) {
+        if (chunks <= 16) return launch_rows<float, 16, 1>(p, stream);
+        if (chunks <= 32) return launch_rows<float, 32, 1>(p, stream);
+        if (chunks <= 64) return launch_rows<float, 32, 2>(p, stream);
+        return launch_rows<float, 32, 4>(p, stream);
+    }
+    if (chunks <= 16) return launch_rows<bf16, 16, 1>(p, stream);
+    if (chunks <= 32) return launch_rows<bf16, 32, 1>(p, stream);
+    return launch_rows<bf16, 32, 2>(p, stream);
 }
 
 // the checked build's record of the first index this file's kernels found out of bounds

@@ -176,20 +176,21 @@ def wide_step(dtype, pages, heads=2, kvh=1, d=128, new=2):
     return Step([(pages * PAGE - new + 1, new)], heads, kvh, d, dtype, seed=pages)
 
 
-@pytest.mark.parametrize("dtype", [BF, F32], ids=names)
-@pytest.mark.parametrize("pages", [300, 1400])
-def test_select_pages_long(ops, dtype, pages):
-    s = wide_step(dtype, pages)
+@pytest.mark.parametrize("dtype,new", [(BF, 2), (F32, 2), (BF, 40), (BF, 12)], ids=names)
+@pytest.mark.parametrize("pages", [300, 1400, 3300])
+def test_select_pages_long(ops, dtype, new, pages):
+    """Clusters of single rows; tiles of 32 rows, of 16, and contexts too long for either."""
+    s = wide_step(dtype, pages, new=new)
     bounds = s.bounds_plane()
     check_selection(s, s.select(ops, bounds, 33), bounds, 33, 1, 2)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=names)
 @pytest.mark.parametrize("kind", ["equal", "few kinds", "zero query", "one ulp", "nan", "inf", "huge", "tiny", "nan query", "inf query", "cancel"])
-@pytest.mark.parametrize("pages", [40, 700])
-def test_select_pages_near_the_border(ops, dtype, kind, pages):
+@pytest.mark.parametrize("pages,new", [(40, 2), (700, 2), (40, 21), (300, 9)])
+def test_select_pages_near_the_border(ops, dtype, kind, pages, new):
     """Scores that tie, that differ in the last place of one channel, that float32 cannot hold: the choice is the 64-bit one."""
-    s = wide_step(dtype, pages)
+    s = wide_step(dtype, pages, new=new)
     g = torch.Generator().manual_seed(pages)
     bounds = s.bounds_plane()
     n = s.table.shape[1]
