@@ -125,12 +125,11 @@ struct Row {
         return (const T*)p.bounds + (page_of(bt, (c0 + i) * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + kvh) * (2 * p.d);
     }
     // false: the row sees no more than `top` pages
-    __device__ __forceinline__ bool find(const PagesParams& p, int seq, int qi, int q_len, int head) {
+    __device__ __forceinline__ bool find(const PagesParams& p, const int* table_row, int row, int pos, int head) {
         kvh = head;
-        const int row = p.seq_q_start[seq] + qi, pos = p.seq_kv_len[seq] - q_len + qi;
         list = p.list + ((int64_t)row * p.kv_heads + kvh) * p.top;
         q = (const T*)p.q + (int64_t)row * p.q_row_stride + (int64_t)kvh * (p.heads / p.kv_heads) * p.d;
-        bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
+        bt = table_row;
         n = pos / GB_PAGE + 1;
         c0 = p.first;
         nc = n - p.first - p.last;
@@ -146,28 +145,41 @@ struct Coef64 {
     __device__ __forceinline__ void load(const PagesParams& p, const T* q, int lane) {
         const int G = p.heads / p.kv_heads;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int c = lane + 32 * j;
-            up[j] = down[j] = 0.0;
-            if (c >= p.d) break;
-            for (int h = 0; h < G; h++) {
-                const double x = (double)to_f32<T>(q[(int64_t)h * p.d + c]);
-                up[j] += x <= 0.0 ? 0.0 : x;      // a NaN is in both
-                down[j] += x >= 0.0 ? 0.0 : x;
-            }
+        for (int j = 0; j < 8; j++) up[j] = down[j] = 0.0;
+        for (int h0 = 0; h0 < G; h0 += 4) {      // four heads' values are asked for together
+            T v[4][8];
+#pragma unroll
+            for (int h = 0; h < 4; h++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[h][j] = h0 + h < G && lane + 32 * j < p.d ? q[(int64_t)(h0 + h) * p.d + lane + 32 * j] : from_f32<T>(0.f);
+#pragma unroll
+            for (int h = 0; h < 4; h++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (32 * j >= p.d) break;
+                    const float x = to_f32<T>(v[h][j]);
+                    up[j] += (double)(x <= 0.f ? 0.f : x);      // a NaN is in both
+                    down[j] += (double)(x >= 0.f ? 0.f : x);
+                }
         }
     }
     // A page's score, the same in every lane; NaN counts as the lowest.  Where no head looks one way there is nothing to add, also
     // where the bound is infinite.
     template <typename T>
     __device__ __forceinline__ double score(const T* b, int d, int lane) const {
-        double s = 0.0;
+        T lo[8], hi[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int c = lane + 32 * j;
-            if (c >= d) break;
-            if (down[j] != 0.0) s += down[j] * (double)to_f32<T>(b[c]);
-            if (up[j] != 0.0) s += up[j] * (double)to_f32<T>(b[d + c]);
+            lo[j] = c < d ? b[c] : from_f32<T>(0.f);
+            hi[j] = c < d ? b[d + c] : from_f32<T>(0.f);
+        }
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (32 * j >= d) break;
+            if (down[j] != 0.0) s += down[j] * (double)to_f32<T>(lo[j]);
+            if (up[j] != 0.0) s += up[j] * (double)to_f32<T>(hi[j]);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -175,17 +187,42 @@ struct Coef64 {
     }
 };
 
-// The choice from float32 scores, by a group of W warps.
+// The choice from float32 scores, by a group of W warps.  key[i] is the ordered float32 score of candidate i, off by no more than
+// `err`.  Warp w has the candidates from w * seg on, 32 at a time; where there are few enough (R > 0: up to 32 R a warp) they stay in
+// registers: every step of the search for the border is a loop over them, and from shared memory it took 670 cycles for 500
+// scores where it takes a tenth.
 template <int W, int BAND>
 struct Chooser {
     double band_s[BAND];
     int band_i[BAND];        // pages near the border, kept with their 64-bit scores
     int hist[256];
     int warp_a[W], warp_b[W];
-    int digit, rest, above, n_band;
+    int digit, rest;
 
     static __device__ __forceinline__ void sync() {
         if (W == 1) __syncwarp(); else __syncthreads();
+    }
+    // Sums over the group.  `at` alternates between two arrays, so that one barrier a call is enough.
+    __device__ __forceinline__ int total(int v, int* at, int warp, int lane) {
+        v = __reduce_add_sync(0xffffffffu, v);
+        if (W > 1) {
+            if (lane == 0) at[warp] = v;
+            sync();
+            v = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++) v += at[w];
+        }
+        return v;
+    }
+    __device__ __forceinline__ uint32_t least(uint32_t v, int* at, int warp, int lane) {
+        v = __reduce_min_sync(0xffffffffu, v);
+        if (W > 1) {
+            if (lane == 0) at[warp] = (int)v;
+            sync();
+#pragma unroll
+            for (int w = 0; w < W; w++) v = min(v, (uint32_t)at[w]);
+        }
+        return v;
     }
     // hist holds how many keys have each digit: the digit of the `want`-th highest key, and how many are wanted of those that have it
     __device__ __forceinline__ void pick(int want, int lane) {
@@ -212,118 +249,164 @@ struct Chooser {
         }
     }
 
-    // key[i]: the ordered float32 score of candidate i, off by no more than err; unsafe: they cannot be relied on.
-    template <typename T>
-    __device__ void run(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, bool unsafe, int tid) {
-        const int warp = tid >> 5, lane = tid & 31, NT = W * 32, nc = r.nc, k = r.k;
-        int ties_wanted = 0;
-        if (tid == 0) n_band = above = 0;
-        if (k > 0 && !unsafe) {
-            // tau: the k-th highest float32 score, digit by digit
-            uint32_t prefix = 0;
-            int want = k;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256; i += NT) hist[i] = 0;
-                sync();
-                for (int i = tid; i < nc; i += NT) {
-                    const uint32_t v = key[i];
-                    if (shift == 24 || (v >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(v >> shift) & 255], 1);
-                }
-                sync();
-                if (warp == 0) pick(want, lane);
-                sync();
-                prefix |= (uint32_t)digit << shift;
-                want = rest;
-            }
-            const float tau = of_key(prefix);
-            const float hi = tau + 2.f * err + fabsf(tau) * 2.4e-7f, lo = tau - 2.f * err - fabsf(tau) * 2.4e-7f;
-            for (int i = tid; i < nc; i += NT) {
-                const float v = of_key(key[i]);
-                uint32_t mark = 0;
-                if (v > hi) {
-                    mark = 2;
-                    atomicAdd(&above, 1);
-                } else if (v >= lo) {
-                    const int at = atomicAdd(&n_band, 1);
-                    if (at < BAND) band_i[at] = i;
-                    mark = 2;      // until the band is settled
-                }
-                key[i] = mark;
-            }
-            sync();
-            const int m = n_band, wanted = k - above;
-            if (m > wanted && m <= BAND) {
-                Coef64 c;
-                c.load(p, r.q, lane);
-                for (int j = warp; j < m; j += W) {
-                    const double v = c.score(r.bounds(p, band_i[j]), p.d, lane);
-                    if (lane == 0) band_s[j] = v;
-                }
-                sync();
-                for (int j = tid; j < m; j += NT) {
-                    int better = 0;
-                    for (int o = 0; o < m; o++) better += band_s[o] > band_s[j] || (band_s[o] == band_s[j] && band_i[o] < band_i[j]);
-                    key[band_i[j]] = better < wanted ? 2 : 0;
-                }
-            }
-            sync();
+    // false: too many pages near the border
+    template <typename T, int R>
+    __device__ __forceinline__ bool fast(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, int warp, int lane) {
+        const int nc = r.nc, k = r.k;
+        const int steps = R > 0 ? R : (nc + 32 * W - 1) / (32 * W), from = warp * steps * 32 + lane;
+        uint32_t reg[R > 0 ? R : 1];
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; j++) reg[j] = from + j * 32 < nc ? key[from + j * 32] : 0u;     // no finite score's key is 0
         }
-        if (k > 0 && (unsafe || n_band > BAND)) {
-            // Scores beyond float32, or hundreds that tie: the k-th highest of the 64-bit scores, which are summed anew for
-            // every digit.  Rare, and right for any input.
+        auto at = [&](int j) -> uint32_t {
+            if constexpr (R > 0) return reg[j];
+            return from + j * 32 < nc ? key[from + j * 32] : 0u;
+        };
+        auto each = [&](auto use) {
+            if constexpr (R > 0) {
+#pragma unroll
+                for (int j = 0; j < R; j++) use(j, at(j));
+            } else {
+                for (int j = 0; j < steps; j++) use(j, at(j));
+            }
+        };
+        // tau, the k-th highest float32 score: the keys from `lo` on are k or more, those from `hi` on fewer; halved until a border
+        // parts exactly k of them (a dozen steps for some hundred scores), or one value is left
+        uint32_t lo = 0xffffffffu, most = 0u;
+        each([&](int, uint32_t v) {
+            if (v) lo = min(lo, v);
+            most = max(most, v);
+        });
+        lo = least(lo, warp_a, warp, lane);
+        uint32_t hi = ~least(~most, warp_b, warp, lane) + 1u;
+        for (bool odd = false; hi - lo > 1u; odd = !odd) {
+            const uint32_t mid = lo + (hi - lo) / 2u;
+            int c = 0;
+            each([&](int, uint32_t v) { c += v >= mid; });
+            c = total(c, odd ? warp_b : warp_a, warp, lane);
+            if (c >= k) lo = mid; else hi = mid;
+            if (c == k) break;
+        }
+        uint32_t border = 0xffffffffu;      // the least key that is `lo` or more
+        each([&](int, uint32_t v) {
+            if (v >= lo) border = min(border, v);
+        });
+        sync();
+        border = least(border, warp_a, warp, lane);
+        const float tau = of_key(border);
+        const float upper = tau + 2.f * err + fabsf(tau) * 2.4e-7f, lower = tau - 2.f * err - fabsf(tau) * 2.4e-7f;
+        const uint32_t sure_from = order_key(upper) + 1u, near_from = order_key(lower == 0.f ? -0.f : lower);
+        int sure = 0, near = 0;
+        each([&](int, uint32_t v) {
+            sure += v >= sure_from;
+            near += v >= near_from && v < sure_from;
+        });
+        const int near_mine = near;
+        const int wanted = k - total(sure, warp_b, warp, lane), m = total(near, warp_a, warp, lane);
+        if (m > BAND && m > wanted) return false;
+        const bool settle = m > wanted;
+        if (settle) {
+            // the pages near the border, in any order: their 64-bit scores, and which are among the best of them
+            if (W > 1) sync();
+            if (warp == 0 && lane == 0) rest = 0;
+            sync();
+            if (__any_sync(0xffffffffu, near_mine > 0))
+                each([&](int j, uint32_t v) {
+                    if (v >= near_from && v < sure_from) band_i[atomicAdd(&rest, 1)] = from + j * 32;
+                });
+            sync();
             Coef64 c;
             c.load(p, r.q, lane);
-            uint64_t prefix = 0;
-            int want = k;
-            for (int shift = 56; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256; i += NT) hist[i] = 0;
-                sync();
-                for (int i = warp; i < nc; i += W) {
-                    const uint64_t v = order_key(c.score(r.bounds(p, i), p.d, lane));
-                    if (lane == 0 && (shift == 56 || (v >> (shift + 8)) == (prefix >> (shift + 8)))) atomicAdd(&hist[(int)(v >> shift) & 255], 1);
-                }
-                sync();
-                if (warp == 0) pick(want, lane);
-                sync();
-                prefix |= (uint64_t)digit << shift;
-                want = rest;
+            for (int j = warp; j < m; j += W) {
+                const double v = c.score(r.bounds(p, band_i[j]), p.d, lane);
+                if (lane == 0) band_s[j] = v;
             }
-            for (int i = warp; i < nc; i += W) {
-                const uint64_t v = order_key(c.score(r.bounds(p, i), p.d, lane));
-                if (lane == 0) key[i] = v > prefix ? 2 : v == prefix ? 1 : 0;
+            sync();
+            for (int j = warp * 32 + lane; j < m; j += W * 32) {
+                int better = 0;
+                for (int o = 0; o < m; o++) better += band_s[o] > band_s[j] || (band_s[o] == band_s[j] && band_i[o] < band_i[j]);
+                key[band_i[j]] = better < wanted ? 0xffffffffu : 0u;
             }
-            ties_wanted = want;
             sync();
         }
-        // the chosen pages in order, a page a thread at a time; of those that tie the first
-        int sure_to = 0, tie_to = 0;
-        for (int i0 = 0; i0 < r.n; i0 += NT) {
-            const int i = i0 + tid, ci = i - r.c0;
-            const uint32_t m = i >= r.n ? 0u : ci < 0 || ci >= nc ? 2u : k > 0 ? key[ci] : 0u;
-            const unsigned sure = __ballot_sync(0xffffffffu, m == 2), tie = __ballot_sync(0xffffffffu, m == 1), below = (1u << lane) - 1u;
-            int s_at = sure_to, t_at = tie_to;
-            if (W > 1) {
-                if (lane == 0) {
-                    warp_a[warp] = __popc(sure);
-                    warp_b[warp] = __popc(tie);
-                }
-                sync();
-                for (int w = 0; w < W; w++) {
-                    if (w < warp) {
-                        s_at += warp_a[w];
-                        t_at += warp_b[w];
-                    }
-                    sure_to += warp_a[w];
-                    tie_to += warp_b[w];
-                }
-                sync();
-            } else {
-                sure_to += __popc(sure);
-                tie_to += __popc(tie);
+        auto taken = [&](int j, uint32_t v) -> bool {
+            if (settle && v >= near_from && v < sure_from) v = key[from + j * 32];
+            return v >= (settle ? sure_from : near_from);
+        };
+        int before = 0;
+        if (W > 1) {
+            int mine = 0;
+            each([&](int j, uint32_t v) { mine += taken(j, v); });
+            mine = __reduce_add_sync(0xffffffffu, mine);
+            if (lane == 0) warp_b[warp] = mine;
+            sync();
+            for (int w = 0; w < warp; w++) before += warp_b[w];
+        }
+        int* list = r.list + r.c0;
+        each([&](int j, uint32_t v) {
+            const bool yes = taken(j, v);
+            const unsigned who = __ballot_sync(0xffffffffu, yes);
+            if (yes) list[before + __popc(who & ((1u << lane) - 1u))] = r.c0 + from + j * 32;
+            before += __popc(who);
+        });
+        return true;
+    }
+
+    // Scores beyond float32, or hundreds that tie: the k-th highest of the 64-bit scores, which are summed anew for every digit.
+    // Rare, and right for any input.
+    template <typename T>
+    __device__ __noinline__ void slow(const PagesParams& p, const Row<T>& r, uint32_t* key, int warp, int lane) {
+        const int nc = r.nc, NT = W * 32, tid = warp * 32 + lane;
+        Coef64 c;
+        c.load(p, r.q, lane);
+        uint64_t prefix = 0;
+        int want = r.k;
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            sync();
+            for (int i = tid; i < 256; i += NT) hist[i] = 0;
+            sync();
+            for (int i = warp; i < nc; i += W) {
+                const uint64_t v = order_key(c.score(r.bounds(p, i), p.d, lane));
+                if (lane == 0 && (shift == 56 || (v >> (shift + 8)) == (prefix >> (shift + 8)))) atomicAdd(&hist[(int)(v >> shift) & 255], 1);
             }
-            s_at += __popc(sure & below);
-            t_at += __popc(tie & below);
-            if (m == 2 || (m == 1 && t_at < ties_wanted)) r.list[s_at + min(t_at, ties_wanted)] = i;
+            sync();
+            if (warp == 0) pick(want, lane);
+            sync();
+            prefix |= (uint64_t)digit << shift;
+            want = rest;
+        }
+        for (int i = warp; i < nc; i += W) {
+            const uint64_t v = order_key(c.score(r.bounds(p, i), p.d, lane));
+            if (lane == 0) key[i] = v > prefix ? 2 : v == prefix ? 1 : 0;
+        }
+        sync();
+        // in order, by one warp; of those that tie the first
+        if (warp == 0) {
+            int at = 0;
+            for (int i0 = 0; i0 < nc; i0 += 32) {
+                const uint32_t v = i0 + lane < nc ? key[i0 + lane] : 0u;
+                const unsigned sure = __ballot_sync(0xffffffffu, v == 2), tie = __ballot_sync(0xffffffffu, v == 1), below = (1u << lane) - 1u;
+                const int ties = __popc(tie & below);
+                if (v == 2 || (v == 1 && ties < want)) r.list[r.c0 + at + __popc(sure & below) + min(ties, want)] = r.c0 + i0 + lane;
+                at += __popc(sure) + min(__popc(tie), want);
+                want -= min(__popc(tie), want);
+            }
+        }
+    }
+
+    // unsafe: the float32 scores cannot be relied on.
+    template <typename T>
+    __device__ __forceinline__ void run(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, bool unsafe, int tid) {
+        constexpr int FEW = W == 1 ? 16 : 4;
+        const int warp = W == 1 ? 0 : tid >> 5, lane = tid & 31;
+        for (int i = tid; i < r.c0; i += W * 32) r.list[i] = i;
+        for (int i = tid; i < p.last; i += W * 32) r.list[p.top - p.last + i] = r.n - p.last + i;
+        if (r.k > 0) {
+            bool done = false;
+            if (!unsafe)
+                done = r.nc <= FEW * 32 * W ? fast<T, FEW>(p, r, key, err, warp, lane) : fast<T, 0>(p, r, key, err, warp, lane);
+            if (!done) slow(p, r, key, warp, lane);
         }
         sync();     // before the group's next row
     }
@@ -378,7 +461,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams 
     const int q_len = p.seq_q_len[seq];
     if (qi >= q_len) return;                    // the whole cluster
     Row<T> r;
-    if (!r.find(p, seq, qi, q_len, blockIdx.y)) {
+    if (!r.find(p, block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots), p.seq_q_start[seq] + qi, p.seq_kv_len[seq] - q_len + qi, blockIdx.y)) {
         if (piece == 0)
             for (int i = tid; i < p.top; i += SELECT_THREADS) r.list[i] = i < r.n ? i : -1;
         return;
@@ -489,7 +572,7 @@ struct alignas(16) TileSmem {
 __host__ __device__ inline int tile_coef_stride(int d) { return 2 * d + 32; }        // elements: rows 64 bytes of banks apart
 __host__ __device__ inline int tile_key_stride(int pages) { return (pages + 31) / 32 * 32 + 8; }
 
-template <int MT>
+template <int MT, int KB_MAX>
 __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParams p) {
     constexpr int RT = MT * 16;
     extern __shared__ __align__(16) unsigned char raw[];
@@ -506,30 +589,48 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParam
     const int rows = min(RT, q_len - q0), d = p.d, G = p.heads / p.kv_heads;
     const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
     // candidates of the last row, which has the most
-    const int nc = (p.seq_kv_len[seq] - q_len + q0 + rows - 1) / GB_PAGE + 1 - p.first - p.last;
+    const int past = p.seq_kv_len[seq] - q_len, q_start = p.seq_q_start[seq];
+    const int nc = (past + q0 + rows - 1) / GB_PAGE + 1 - p.first - p.last;
     {
-        const bf16* q = (const bf16*)p.q + (int64_t)(p.seq_q_start[seq] + q0) * p.q_row_stride + (int64_t)kvh * G * d;
-        for (int i = tid; i < RT * (d / 2); i += TILE_THREADS) {
-            const int row = i / (d / 2), c = (i - row * (d / 2)) * 2;
-            float up[2] = {0.f, 0.f}, down[2] = {0.f, 0.f};
-            if (row < rows)
+        const bf16* q = (const bf16*)p.q + (int64_t)(q_start + q0) * p.q_row_stride + (int64_t)kvh * G * d;
+        const bool whole = !(((uintptr_t)p.q & 15) | (p.q_row_stride & 7));     // rows of 16-byte chunks
+        const int CH = d / 8;
+        for (int i = tid; i < RT * CH; i += TILE_THREADS) {
+            const int row = i / CH, c = (i - row * CH) * 8;
+            float up[8], down[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) up[e] = down[e] = 0.f;
+            if (row < rows) {
+#pragma unroll 4
                 for (int h = 0; h < G; h++) {
                     const bf16* at = q + (int64_t)row * p.q_row_stride + h * d + c;
+                    float x[8];
+                    if (whole) {
+                        unpack(*reinterpret_cast<const uint4*>(at), x);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float x = __bfloat162float(at[e]);
-                        up[e] += x <= 0.f ? 0.f : x;
-                        down[e] += x >= 0.f ? 0.f : x;
+                        for (int e = 0; e < 8; e++) x[e] = __bfloat162float(at[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        up[e] += x[e] <= 0.f ? 0.f : x[e];
+                        down[e] += x[e] >= 0.f ? 0.f : x[e];
                     }
                 }
+            }
             bf16* to = coef + row * CS + c;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const bf16 dh = __float2bfloat16_rn(down[e]), uh = __float2bfloat16_rn(up[e]);
-                to[e] = dh;
-                to[d + e] = uh;
-                to[RT * CS + e] = __float2bfloat16_rn(down[e] - __bfloat162float(dh));
-                to[RT * CS + d + e] = __float2bfloat16_rn(up[e] - __bfloat162float(uh));
+            for (int side = 0; side < 2; side++) {
+                uint32_t first[4], second[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x0 = side ? up[2 * e] : down[2 * e], x1 = side ? up[2 * e + 1] : down[2 * e + 1];
+                    first[e] = pack_bf16(x0, x1);
+                    const float r0 = __uint_as_float(first[e] << 16), r1 = __uint_as_float(first[e] & 0xffff0000u);
+                    second[e] = pack_bf16(x0 - r0, x1 - r1);
+                }
+                *reinterpret_cast<uint4*>(to + side * d) = make_uint4(first[0], first[1], first[2], first[3]);
+                *reinterpret_cast<uint4*>(to + RT * CS + side * d) = make_uint4(second[0], second[1], second[2], second[3]);
             }
         }
         for (int i = tid; i < 64; i += TILE_THREADS) s.size[i] = 0.f;
@@ -537,9 +638,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParam
     __syncthreads();
     const int KB = d / 16;             // blocks of 32 bounds
     const bf16* plane = (const bf16*)p.bounds;
-    __nv_bfloat162 size[16];           // of each block: the largest this lane has met in its chunk of 8
+    __nv_bfloat162 size[KB_MAX];       // of each block: the largest this lane has met in its chunk of 8
 #pragma unroll
-    for (int kb = 0; kb < 16; kb++) size[kb] = __floats2bfloat162_rn(0.f, 0.f);
+    for (int kb = 0; kb < KB_MAX; kb++) size[kb] = __floats2bfloat162_rn(0.f, 0.f);
     for (int i0 = warp * 16; i0 < nc; i0 += TILE_WARPS * 16) {
         const bf16* b[2];
 #pragma unroll
@@ -555,7 +656,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParam
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[m][t][e] = 0.f;
 #pragma unroll
-        for (int half = 0; half < 4; half++) {                 // blocks in fours: what a lane asks for at once
+        for (int half = 0; half < KB_MAX / 4; half++) {        // blocks in fours: what a lane asks for at once
             if (half * 4 >= KB) break;
             uint4 x[4][2];
 #pragma unroll
@@ -600,7 +701,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParam
             }
     }
 #pragma unroll
-    for (int kb = 0; kb < 16; kb++) {
+    for (int kb = 0; kb < KB_MAX; kb++) {
         if (kb >= KB) break;
         const float lo = __low2float(size[kb]), hi = __high2float(size[kb]);
         float v = lo != lo || hi != hi ? INFINITY : fmaxf(lo, hi);
@@ -611,7 +712,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParam
     __syncthreads();
     for (int row = warp; row < rows; row += TILE_WARPS) {
         Row<bf16> r;
-        if (!r.find(p, seq, q0 + row, q_len, kvh)) {
+        if (!r.find(p, bt, q_start + q0 + row, past + q0 + row, kvh)) {
             for (int i = lane; i < p.top; i += 32) r.list[i] = i < r.n ? i : -1;
             continue;
         }
@@ -619,6 +720,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParam
         // for each of 4 d / 16 steps (16 products and the sum so far, cut off behind 25 bits of the largest of them, and the result).
         // All relative to the sum of the terms' sizes; what is below the normal range of a coefficient's second part is let in by 1e-35.
         float most = 0.f;
+#pragma unroll 8
         for (int c = lane; c < 2 * d; c += 32) most = fmaf(fabsf(__bfloat162float(coef[row * CS + c])) + 1.0e-35f, s.size[c >> 3], most);
         most = warp_sum(most);
         const bool unsafe = !(most <= 1.0e38f);
@@ -684,17 +786,17 @@ static int64_t tile_smem(const PagesParams& p, int rt) {
     return (int64_t)sizeof(TileSmem) + 2 * rt * tile_coef_stride(p.d) * 2 + (int64_t)rt * tile_key_stride(p.bt_stride) * 4;
 }
 
-template <int MT>
+template <int MT, int KB_MAX>
 static int launch_tiles(const PagesParams& p, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(select_tile_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_TILE_SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(select_tile_kernel<MT, KB_MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_TILE_SMEM);
         if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
         configured = true;
     }
     const dim3 grid(ceil_div(p.max_q_len, MT * 16), p.kv_heads, p.nseq);
     if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("select_pages: %d kv heads, %d sequences exceed one launch", p.kv_heads, p.nseq);
-    launch_pdl(select_tile_kernel<MT>, grid, dim3(TILE_THREADS), (size_t)tile_smem(p, MT * 16), stream, p);
+    launch_pdl(select_tile_kernel<MT, KB_MAX>, grid, dim3(TILE_THREADS), (size_t)tile_smem(p, MT * 16), stream, p);
     GB_CHECK_LAUNCH("select_pages");
     return 0;
 }
@@ -707,8 +809,8 @@ GB_API int gb_select_pages(const PagesParams* pp, int dtype, cudaStream_t stream
     if (p.first < 0 || p.last < 1 || p.first + p.last > p.top) GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
     if (p.bt_stride > MAX_PAGES) GB_REFUSE("select_pages: sequences of up to %d pages; this kernel takes %d", p.bt_stride, MAX_PAGES);
     if (dtype == GB_BF16 && p.max_q_len >= TILE_MIN_ROWS && p.d % 16 == 0) {
-        if (p.max_q_len > 16 && tile_smem(p, 32) <= MAX_TILE_SMEM) return launch_tiles<2>(p, stream);
-        if (tile_smem(p, 16) <= MAX_TILE_SMEM) return launch_tiles<1>(p, stream);
+        if (p.max_q_len > 16 && tile_smem(p, 32) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<2, 8>(p, stream) : launch_tiles<2, 16>(p, stream);
+        if (tile_smem(p, 16) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<1, 8>(p, stream) : launch_tiles<1, 16>(p, stream);
     }
     const int chunks = 2 * p.d / (dtype == GB_F32 ? 4 : 8);
     if (dtype == GB_F32) {
