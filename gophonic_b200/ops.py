@@ -8,6 +8,7 @@ torch fallback.  Importing this module builds the library if needed and fails if
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, Structure, byref, c_float, c_int, c_int64, c_uint64, c_void_p
 from typing import Optional
 
@@ -818,6 +819,29 @@ MAX_LISTED_PAGES = 1024          # entries of a row's list of pages
 MAX_SELECTABLE_PAGES = 32768     # pages of a sequence that a row's may be selected from: 2,097,152 tokens
 
 
+# PagesParams as bytes: filling a ctypes structure field by field takes the host longer than most of these kernels take
+_PAGES_LAYOUT = struct.Struct("@QqQqQQQQi4xQQQQ5ifQ7i4x")
+assert _PAGES_LAYOUT.size == ctypes.sizeof(_PagesParams)
+for _f in (_lib.gb_page_bounds, _lib.gb_select_pages, _lib.gb_attention_pages):
+    _f.argtypes = (c_void_p, c_int, c_void_p)
+
+
+def _is_index(t: torch.Tensor, n: int, dev: int) -> bool:
+    return t.dtype is torch.int32 and t.get_device() == dev and t.numel() >= n and t.is_contiguous()
+
+
+def _is_plane(t: torch.Tensor, dtype, dev: int) -> bool:
+    return t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
+
+
+def _pages_stream(who: str, dev: int) -> c_void_p:
+    """The stream of a call whose tensors are all on device ``dev``, which has to be the library's."""
+    stream = _stream()
+    if _device_index and _device_index[0] != dev:
+        raise KernelError(f"{who}: tensors on cuda:{dev}, the library serves cuda:{_device_index[0]}")
+    return stream
+
+
 def _need_sequences(who: str, block_table: torch.Tensor, nseq: int, **lists: torch.Tensor) -> None:
     _need(block_table, "block table", torch.int32, 2)
     for name, t in lists.items():
@@ -839,19 +863,21 @@ def page_bounds(k_planes: torch.Tensor, bounds: torch.Tensor, block_table: torch
     highest (exact; NaN if one of them is).  ``k_planes`` [pages, kv_heads, 64, head_dim] with ``bounds`` [pages, kv_heads, 2,
     head_dim] of the same dtype, or several such planes in one leading dimension.  Nothing else of ``bounds`` changes.  To be called
     behind what writes the step's keys; ``select_pages`` scores the pages of earlier tokens by it."""
-    if k_planes.dim() not in (4, 5):
-        raise KernelError(f"page_bounds: key planes {tuple(k_planes.shape)}")
-    _need(k_planes, "key planes")
-    _need(bounds, "page bounds", k_planes.dtype)
-    d = k_planes.shape[-1]
-    if k_planes.shape[-2] != PAGE or tuple(bounds.shape) != tuple(k_planes.shape[:-2]) + (2, d):
-        raise KernelError(f"page_bounds: key planes {tuple(k_planes.shape)}, bounds {tuple(bounds.shape)}")
-    _need_sequences("page_bounds", block_table, nseq, seq_slot=seq_slot, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
-    planes = k_planes.shape[0] if k_planes.dim() == 5 else 1
-    p = _PagesParams(k_plane=k_planes.data_ptr(), bounds=bounds.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
-                     seq_slot=seq_slot.data_ptr(), seq_q_len=seq_q_len.data_ptr(), seq_kv_len=seq_kv_len.data_ptr(), nseq=nseq,
-                     kv_heads=k_planes.shape[-3], d=d, max_q_len=max_q_len, planes=planes, pages=k_planes.shape[-4], max_slots=block_table.shape[0])
-    _check(_lib.gb_page_bounds(byref(p), _code(k_planes.dtype), _stream()))
+    shape, dtype, dev = k_planes.shape, k_planes.dtype, k_planes.get_device()
+    if len(shape) not in (4, 5):
+        raise KernelError(f"page_bounds: key planes {tuple(shape)}")
+    planes, (pages, kv_heads, tokens, d) = (shape[0], shape[1:]) if len(shape) == 5 else (1, shape)
+    table = block_table.shape
+    if not (dev >= 0 and k_planes.is_contiguous() and _is_plane(bounds, dtype, dev) and tokens == PAGE and tuple(bounds.shape) == (*shape[:-2], 2, d)
+            and len(table) == 2 and _is_index(block_table, 0, dev) and _is_index(seq_slot, nseq, dev) and _is_index(seq_q_len, nseq, dev)
+            and _is_index(seq_kv_len, nseq, dev)):
+        _need(k_planes, "key planes")
+        _need(bounds, "page bounds", dtype)
+        _need_sequences("page_bounds", block_table, nseq, seq_slot=seq_slot, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
+        raise KernelError(f"page_bounds: key planes {tuple(shape)}, bounds {tuple(bounds.shape)}, or tensors on different devices")
+    p = _PAGES_LAYOUT.pack(0, 0, 0, 0, k_planes.data_ptr(), 0, bounds.data_ptr(), block_table.data_ptr(), table[1], seq_slot.data_ptr(), 0,
+                           seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, 0, kv_heads, d, max_q_len, 0.0, 0, 0, 0, 0, planes, pages, table[0], 0)
+    _check(_lib.gb_page_bounds(p, _code(dtype), _pages_stream("page_bounds", dev)))
 
 
 def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_slot: torch.Tensor, seq_q_start: torch.Tensor,
@@ -865,46 +891,62 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
     is NaN counts as the lowest.  A row that sees no more than ``top`` pages gets all of them.  q is a [rows, >= heads * head_dim]
     view (row stride free); the bounds of full pages must hold lo <= hi, as ``page_bounds`` leaves them; rows of no sequence keep
     what they had.  Sequences of up to ``MAX_SELECTABLE_PAGES`` pages."""
-    _need_rows("select_pages", "q", q, None, heads * head_dim)
-    _need(bounds, "page bounds", q.dtype, 4)
-    _need(pages, "page lists", torch.int32, 3)
-    if bounds.shape[1:] != (kv_heads, 2, head_dim):
-        raise KernelError(f"select_pages: bounds {tuple(bounds.shape)} for {kv_heads} kv heads of {head_dim}")
-    if pages.shape[0] != q.shape[0] or pages.shape[1] != kv_heads:
-        raise KernelError(f"select_pages: lists {tuple(pages.shape)} for {q.shape[0]} rows and {kv_heads} kv heads")
-    _need_sequences("select_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
-    p = _PagesParams(q=q.data_ptr(), q_row_stride=q.stride(0), bounds=bounds.data_ptr(), block_table=block_table.data_ptr(),
-                     bt_stride=block_table.stride(0), seq_slot=seq_slot.data_ptr(), seq_q_start=seq_q_start.data_ptr(),
-                     seq_q_len=seq_q_len.data_ptr(), seq_kv_len=seq_kv_len.data_ptr(), nseq=nseq, heads=heads, kv_heads=kv_heads, d=head_dim,
-                     max_q_len=max_q_len, list=pages.data_ptr(), top=pages.shape[2], first=first, last=last, pages=bounds.shape[0],
-                     max_slots=block_table.shape[0], rows=q.shape[0])
-    _check(_lib.gb_select_pages(byref(p), _code(q.dtype), _stream()))
+    dtype, dev, wide = q.dtype, q.get_device(), heads * head_dim
+    table, listed, plane, shape = block_table.shape, pages.shape, bounds.shape, q.shape
+    ok = dev >= 0 and len(shape) == 2 and len(table) == 2 and len(listed) == 3
+    if ok:
+        rows, width = shape
+        row_stride, unit = q.stride()
+        ok = (unit == 1 and width >= wide and (rows <= 1 or row_stride >= wide) and _is_plane(bounds, dtype, dev)
+              and tuple(plane) == (plane[0], kv_heads, 2, head_dim) and _is_plane(pages, torch.int32, dev) and listed[0] == rows
+              and listed[1] == kv_heads and _is_index(block_table, 0, dev) and _is_index(seq_slot, nseq, dev)
+              and _is_index(seq_q_start, nseq, dev) and _is_index(seq_q_len, nseq, dev) and _is_index(seq_kv_len, nseq, dev))
+    if not ok:
+        _need_rows("select_pages", "q", q, None, wide)
+        _need(bounds, "page bounds", dtype, 4)
+        _need(pages, "page lists", torch.int32, 3)
+        _need_sequences("select_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
+        raise KernelError(f"select_pages: bounds {tuple(plane)}, lists {tuple(listed)} for q {tuple(shape)} of {heads} over {kv_heads} heads of "
+                          f"{head_dim}, or tensors on different devices")
+    p = _PAGES_LAYOUT.pack(q.data_ptr(), row_stride, 0, 0, 0, 0, bounds.data_ptr(), block_table.data_ptr(), table[1], seq_slot.data_ptr(),
+                           seq_q_start.data_ptr(), seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, heads, kv_heads, head_dim, max_q_len, 0.0,
+                           pages.data_ptr(), listed[2], first, last, 0, plane[0], table[0], rows)
+    _check(_lib.gb_select_pages(p, _code(dtype), _pages_stream("select_pages", dev)))
 
 
 def attention_pages(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, block_table: torch.Tensor,
                     seq_slot: torch.Tensor, seq_q_start: torch.Tensor, seq_q_len: torch.Tensor, seq_kv_len: torch.Tensor, nseq: int,
                     max_q_len: int, heads: int, kv_heads: int, head_dim: int, scale: float, pages: torch.Tensor) -> None:
     """Causal GQA over a part of the paged cache: row r's heads of kv head g attend to the keys, at positions up to the row's own, of
-    the logical pages that ``pages[r, g]`` lists (int32 [rows, kv_heads, top], top up to ``MAX_LISTED_PAGES``; ascending and each
-    once, as ``select_pages`` leaves them; negative entries and pages behind the row's own name nothing).  A row that sees no key
+    the logical pages that ``pages[r, g]`` lists (int32 [rows, kv_heads, top], top up to ``MAX_LISTED_PAGES``; each page once, as
+    ``select_pages`` leaves them; negative entries and pages behind the row's own name nothing).  A row that sees no key
     gives zeros; rows of no sequence keep what they had.  q and out are [rows, >= heads * head_dim] views (row strides free)."""
-    _need_rows("attention_pages", "q", q, None, heads * head_dim)
-    _need_rows("attention_pages", "out", out, q.dtype, heads * head_dim)
-    _need(k_plane, "key plane", q.dtype, 4)
-    _need(v_plane, "value plane", q.dtype, 4)
-    for t, nm in ((k_plane, "key plane"), (v_plane, "value plane")):
-        if t.shape[1:] != (kv_heads, PAGE, head_dim) or t.shape != k_plane.shape:
-            raise KernelError(f"attention_pages: {nm} {tuple(t.shape)} for {kv_heads} kv heads of {head_dim}")
-    _need(pages, "page lists", torch.int32, 3)
-    if pages.shape[0] != q.shape[0] or out.shape[0] != q.shape[0] or pages.shape[1] != kv_heads:
-        raise KernelError(f"attention_pages: q {tuple(q.shape)}, out {tuple(out.shape)}, lists {tuple(pages.shape)} for {kv_heads} kv heads")
-    _need_sequences("attention_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
-    p = _PagesParams(q=q.data_ptr(), q_row_stride=q.stride(0), out=out.data_ptr(), out_row_stride=out.stride(0), k_plane=k_plane.data_ptr(),
-                     v_plane=v_plane.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
-                     seq_slot=seq_slot.data_ptr(), seq_q_start=seq_q_start.data_ptr(), seq_q_len=seq_q_len.data_ptr(),
-                     seq_kv_len=seq_kv_len.data_ptr(), nseq=nseq, heads=heads, kv_heads=kv_heads, d=head_dim, max_q_len=max_q_len, scale=scale,
-                     list=pages.data_ptr(), top=pages.shape[2], pages=k_plane.shape[0], max_slots=block_table.shape[0], rows=q.shape[0])
-    _check(_lib.gb_attention_pages(byref(p), _code(q.dtype), _stream()))
+    dtype, dev, wide = q.dtype, q.get_device(), heads * head_dim
+    table, listed, plane, shape, to = block_table.shape, pages.shape, k_plane.shape, q.shape, out.shape
+    ok = dev >= 0 and len(shape) == 2 and len(to) == 2 and len(table) == 2 and len(listed) == 3
+    if ok:
+        rows, width = shape
+        row_stride, unit = q.stride()
+        out_stride, out_unit = out.stride()
+        ok = (unit == 1 and out_unit == 1 and width >= wide and to[1] >= wide and to[0] == rows
+              and (rows <= 1 or (row_stride >= wide and out_stride >= wide)) and out.dtype is dtype and out.get_device() == dev
+              and _is_plane(k_plane, dtype, dev) and _is_plane(v_plane, dtype, dev) and tuple(plane) == (plane[0], kv_heads, PAGE, head_dim)
+              and v_plane.shape == plane and _is_plane(pages, torch.int32, dev) and listed[0] == rows and listed[1] == kv_heads
+              and _is_index(block_table, 0, dev) and _is_index(seq_slot, nseq, dev) and _is_index(seq_q_start, nseq, dev)
+              and _is_index(seq_q_len, nseq, dev) and _is_index(seq_kv_len, nseq, dev))
+    if not ok:
+        _need_rows("attention_pages", "q", q, None, wide)
+        _need_rows("attention_pages", "out", out, dtype, wide)
+        _need(k_plane, "key plane", dtype, 4)
+        _need(v_plane, "value plane", dtype, 4)
+        _need(pages, "page lists", torch.int32, 3)
+        _need_sequences("attention_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
+        raise KernelError(f"attention_pages: q {tuple(shape)}, out {tuple(to)}, lists {tuple(listed)}, planes {tuple(plane)} and "
+                          f"{tuple(v_plane.shape)} for {heads} over {kv_heads} heads of {head_dim}, or tensors on different devices")
+    p = _PAGES_LAYOUT.pack(q.data_ptr(), row_stride, out.data_ptr(), out_stride, k_plane.data_ptr(), v_plane.data_ptr(), 0, block_table.data_ptr(),
+                           table[1], seq_slot.data_ptr(), seq_q_start.data_ptr(), seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, heads, kv_heads,
+                           head_dim, max_q_len, scale, pages.data_ptr(), listed[2], 0, 0, 0, plane[0], table[0], rows)
+    _check(_lib.gb_attention_pages(p, _code(dtype), _pages_stream("attention_pages", dev)))
 
 
 # ---- mixers with a matrix state ------------------------------------------------------------
