@@ -6,7 +6,7 @@
 // softmax of its own, and join their results through distributed shared memory, so there is neither scratch memory nor a second
 // kernel.  The query heads of the group are the rows of the tiles and share every key and value that is read.
 //   bfloat16: both products on mma.sync, a page of 64 keys at a time, 16 keys a warp, pages asked for three deep by cp.async;
-//   float32:  CUDA cores, pages staged in shared memory; a thread has a key's scores first and some channels' sums after.
+//   float32:  CUDA cores, half a page a stage, three deep by cp.async.
 // Scores, the softmax and the sums are float32; with bfloat16 the probabilities are rounded to bfloat16 for the second product, as
 // the values are.
 #include "mma.cuh"
@@ -303,84 +303,96 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
 }
 
 // ---- float32 -------------------------------------------------------------------------------------
-constexpr int F_HEADS = 8;       // heads of a group that a CTA takes at most
+// Half a page of keys and values a stage.  A tile's scores: each warp takes a quarter of the channels, a lane a key; the quarters are
+// added where a warp has the softmax of a head; then a thread sums its channels over the tile's keys.
+constexpr int F_KEYS = 32, F_STAGES = 3;
 constexpr int F_CH = 2;          // channels a thread sums at most: head_dim up to 256
 
+__host__ __device__ constexpr int f32_stage(int d) { return F_KEYS * (2 * d + 4); }   // floats: key rows start four banks further each
+__host__ __device__ constexpr int f32_floats(int d, int nh) { return nh * d * 2 + nh * F_KEYS * 5 + F_STAGES * f32_stage(d); }
+
+template <int NH>
 __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) {
     extern __shared__ __align__(16) float sm[];
-    const int d = p.d, sd = d + 4;                 // rows of 16-byte chunks that start four banks further each
-    float* Qs = sm;                                // [F_HEADS][d], scaled
-    float* Ks = Qs + F_HEADS * d;                  // [64][sd]
-    float* Vs = Ks + GB_PAGE * sd;                 // [64][d]
-    float* Ps = Vs + GB_PAGE * d;                  // [F_HEADS][64]
-    float* Os = Ps + F_HEADS * GB_PAGE;            // [F_HEADS][d]
-    int* pages = reinterpret_cast<int*>(Os + F_HEADS * d);
+    const int d = p.d, sd = d + 4;
+    float* KV = sm;                                // [F_STAGES][32][sd], then [32][d]
+    float* Qs = KV + F_STAGES * f32_stage(d);      // [NH][d], scaled
+    float* Os = Qs + NH * d;                       // [NH][d]
+    float* Part = Os + NH * d;                     // [4 warps][NH][32]
+    float* Ps = Part + 4 * NH * F_KEYS;            // [NH][32]
+    int* pages = reinterpret_cast<int*>(Ps + NH * F_KEYS);
     __shared__ int counts[THREADS / 32];
-    __shared__ float ml[F_HEADS][2], corr[F_HEADS];
+    __shared__ float ml[NH][2], corr[NH];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
     Place at;
-    const int G = p.heads / p.kv_heads, GC = G < F_HEADS ? G : F_HEADS;
+    const int G = p.heads / p.kv_heads, GC = G < NH ? G : NH;
     if (!at.find(p, GC)) return;
     const int pieces = (int)cg::this_cluster().num_blocks(), piece = (int)cg::this_cluster().block_rank();
     const float* qsrc = (const float*)p.q + (int64_t)at.row * p.q_row_stride + (int64_t)at.h0 * d;
     const float sc = p.scale * LOG2E;
-    for (int i = tid; i < at.nh * d; i += THREADS) Qs[i] = qsrc[i] * sc;
-    if (tid < F_HEADS) {
+    for (int i = tid; i < NH * d; i += THREADS) Qs[i] = i < at.nh * d ? qsrc[i] * sc : 0.f;
+    if (tid < NH) {
         ml[tid][0] = -INFINITY;
         ml[tid][1] = 0.f;
     }
     const int n_all = pack_list(p, p.list + ((int64_t)at.row * p.kv_heads + at.kvh) * p.top, at.pos / GB_PAGE, pages, counts);
-    const int lo = (int)((int64_t)n_all * piece / pieces), n = (int)((int64_t)n_all * (piece + 1) / pieces) - lo;
-    float o[F_HEADS][F_CH];
+    const int lo = (int)((int64_t)n_all * piece / pieces), n = 2 * ((int)((int64_t)n_all * (piece + 1) / pieces) - lo);   // half pages
+    const int CH = d / 4;
+    auto load_tile = [&](int i) {
+        const int64_t off = ((page_of(at.bt, pages[lo + i / 2] * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + at.kvh) * GB_PAGE + (i & 1) * F_KEYS) * (int64_t)d;
+        const float *k = (const float*)p.k_plane + off, *v = (const float*)p.v_plane + off;
+        float* st = KV + (i % F_STAGES) * f32_stage(d);
+        for (int idx = tid; idx < F_KEYS * CH; idx += THREADS) {
+            const int r = idx / CH, c = (idx - r * CH) * 4;
+            cp_async16(st + r * sd + c, k + (int64_t)r * d + c, 16);
+            cp_async16(st + F_KEYS * sd + r * d + c, v + (int64_t)r * d + c, 16);
+        }
+    };
 #pragma unroll
-    for (int h = 0; h < F_HEADS; h++)
+    for (int s = 0; s < F_STAGES - 1; s++) {
+        if (s < n) load_tile(s);
+        cp_async_commit();
+    }
+    float o[NH][F_CH];
+#pragma unroll
+    for (int h = 0; h < NH; h++)
 #pragma unroll
         for (int c = 0; c < F_CH; c++) o[h][c] = 0.f;
-    const int CH = d / 4;
+    const int quarter = (CH + 3) / 4, c_lo = warp * quarter, c_hi = min(CH, c_lo + quarter);    // the warp's chunks of four channels
     for (int i = 0; i < n; i++) {
-        const int64_t off = (page_of(at.bt, pages[lo + i] * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + at.kvh) * (int64_t)(GB_PAGE * d);
-        const float* k = (const float*)p.k_plane + off;
-        const float* v = (const float*)p.v_plane + off;
-        __syncthreads();       // the page before is done with
-        for (int idx = tid; idx < GB_PAGE * CH; idx += THREADS) {
-            const int r = idx / CH, c = (idx - r * CH) * 4;
-            cp_async16(Ks + r * sd + c, k + (int64_t)r * d + c, 16);
-            cp_async16(Vs + r * d + c, v + (int64_t)r * d + c, 16);
-        }
+        cp_async_wait<F_STAGES - 2>();
+        __syncthreads();               // the tile has landed, and the one before is done with
+        if (i + F_STAGES - 1 < n) load_tile(i + F_STAGES - 1);
         cp_async_commit();
-        cp_async_wait<0>();
-        __syncthreads();
+        const float *Ks = KV + (i % F_STAGES) * f32_stage(d), *Vs = Ks + F_KEYS * sd;
+        const int key0 = pages[lo + i / 2] * GB_PAGE + (i & 1) * F_KEYS, keys = min(F_KEYS, at.pos + 1 - key0);   // keys the row sees
+        if (keys <= 0) continue;
         {
-            // a thread: one key, every second head
-            const int key = tid & 63;
-            const bool ok = pages[lo + i] * GB_PAGE + key <= at.pos;
-            float s[F_HEADS / 2];
+            float s[NH];
 #pragma unroll
-            for (int h = 0; h < F_HEADS / 2; h++) s[h] = 0.f;
-            for (int c = 0; c < d; c += 4) {
-                const float4 kk = *reinterpret_cast<const float4*>(Ks + key * sd + c);
+            for (int h = 0; h < NH; h++) s[h] = 0.f;
+#pragma unroll 4
+            for (int c = c_lo; c < c_hi; c++) {
+                const float4 kk = *reinterpret_cast<const float4*>(Ks + lane * sd + c * 4);
 #pragma unroll
-                for (int h = 0; h < F_HEADS / 2; h++) {
-                    const int head = 2 * h + (tid >> 6);
-                    if (head < at.nh) {
-                        const float4 qq = *reinterpret_cast<const float4*>(Qs + head * d + c);
-                        s[h] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[h]))));
-                    }
+                for (int h = 0; h < NH; h++) {
+                    const float4 qq = *reinterpret_cast<const float4*>(Qs + h * d + c * 4);
+                    s[h] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[h]))));
                 }
             }
 #pragma unroll
-            for (int h = 0; h < F_HEADS / 2; h++) {
-                const int head = 2 * h + (tid >> 6);
-                if (head < at.nh) Ps[head * GB_PAGE + key] = ok ? s[h] : -INFINITY;
-            }
+            for (int h = 0; h < NH; h++) Part[(warp * NH + h) * F_KEYS + lane] = s[h];
         }
         __syncthreads();
         for (int h = warp; h < at.nh; h += THREADS / 32) {
-            const float a = Ps[h * GB_PAGE + lane], b = Ps[h * GB_PAGE + 32 + lane];
-            const float old = ml[h][0], m = fmaxf(old, warp_max(fmaxf(a, b))), base = m == -INFINITY ? 0.f : m;
-            const float pa = exp2f(a - base), pb = exp2f(b - base), sum = warp_sum(pa + pb);
-            Ps[h * GB_PAGE + lane] = pa;
-            Ps[h * GB_PAGE + 32 + lane] = pb;
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) s += Part[(w * NH + h) * F_KEYS + lane];
+            if (lane >= keys) s = -INFINITY;       // also where the key holds Inf or NaN
+            const float old = ml[h][0], m = fmaxf(old, warp_max(s)), base = m == -INFINITY ? 0.f : m;
+            const float w = exp2f(s - base), sum = warp_sum(w);
+            Ps[h * F_KEYS + lane] = w;
             __syncwarp();
             if (lane == 0) {
                 corr[h] = exp2f(old - base);
@@ -389,27 +401,38 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
             }
         }
         __syncthreads();
-        const int keys = min(GB_PAGE, at.pos + 1 - pages[lo + i] * GB_PAGE);   // the others are not touched: they may hold Inf or NaN
 #pragma unroll
         for (int c = 0; c < F_CH; c++) {
             const int ch = tid + c * THREADS;
             if (ch < d) {
-                float acc[F_HEADS];
 #pragma unroll
-                for (int h = 0; h < F_HEADS; h++) acc[h] = h < at.nh ? o[h][c] * corr[h] : 0.f;
-                for (int key = 0; key < keys; key++) {
-                    const float vv = Vs[key * d + ch];
+                for (int h = 0; h < NH; h++) o[h][c] *= corr[h];
+                if (keys == F_KEYS) {
+#pragma unroll 4
+                    for (int key = 0; key < F_KEYS; key += 4) {
+                        float v[4];
 #pragma unroll
-                    for (int h = 0; h < F_HEADS; h++)
-                        if (h < at.nh) acc[h] = fmaf(Ps[h * GB_PAGE + key], vv, acc[h]);
+                        for (int e = 0; e < 4; e++) v[e] = Vs[(key + e) * d + ch];
+#pragma unroll
+                        for (int h = 0; h < NH; h++) {
+                            const float4 w = *reinterpret_cast<const float4*>(Ps + h * F_KEYS + key);
+                            o[h][c] = fmaf(w.x, v[0], fmaf(w.y, v[1], fmaf(w.z, v[2], fmaf(w.w, v[3], o[h][c]))));
+                        }
+                    }
+                } else {
+                    // values behind the row's position are not touched: they may be Inf or NaN
+                    for (int key = 0; key < keys; key++) {
+                        const float v = Vs[key * d + ch];
+#pragma unroll
+                        for (int h = 0; h < NH; h++) o[h][c] = fmaf(Ps[h * F_KEYS + key], v, o[h][c]);
+                    }
                 }
-#pragma unroll
-                for (int h = 0; h < F_HEADS; h++) o[h][c] = acc[h];
             }
         }
     }
+    cp_async_wait<0>();
 #pragma unroll
-    for (int h = 0; h < F_HEADS; h++)
+    for (int h = 0; h < NH; h++)
 #pragma unroll
         for (int c = 0; c < F_CH; c++)
             if (h < at.nh && tid + c * THREADS < d) Os[h * d + tid + c * THREADS] = o[h][c];
@@ -427,20 +450,9 @@ int pieces_for(const PagesParams& p, int chunks, int per_sm) {
 
 template <typename K>
 int launch(K kernel, const PagesParams& p, int chunks, int pieces, int smem, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg = {};
     const int64_t x = (int64_t)p.nseq * p.max_q_len * pieces;
     if (x > 0x7fffffff || p.kv_heads * chunks > 65535) GB_REFUSE("attention_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
-    cfg.gridDim = dim3((unsigned)x, p.kv_heads * chunks);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = pieces;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, p);
+    launch_pdl_cluster(kernel, dim3((unsigned)x, p.kv_heads * chunks), dim3(THREADS), (size_t)smem, stream, pieces, 1, p);
     GB_CHECK_LAUNCH("attention_pages");
     return 0;
 }
@@ -460,16 +472,18 @@ int launch_mma(const PagesParams& p, cudaStream_t stream) {
     return launch(attn_pages_mma_kernel<HD>, p, chunks, pieces_for(p, chunks, HD <= 128 ? 2 : 1), base + p.top * 4, stream);
 }
 
+template <int NH>
 int launch_f32(const PagesParams& p, cudaStream_t stream) {
-    const auto bytes = [](int d, int top) { return (F_HEADS * d * 2 + GB_PAGE * (2 * d + 4) + F_HEADS * GB_PAGE) * 4 + top * 4; };
     static bool configured = false;
+    constexpr int most = f32_floats(256, NH) * 4 + MAX_TOP * 4;
+    static_assert(most <= 231000, "the widest heads' stages fit");
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_pages_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(256, MAX_TOP));
-        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", bytes(256, MAX_TOP), cudaGetErrorString(e));
+        const cudaError_t e = cudaFuncSetAttribute(attn_pages_f32_kernel<NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", most, cudaGetErrorString(e));
         configured = true;
     }
-    const int G = p.heads / p.kv_heads, chunks = (G + F_HEADS - 1) / F_HEADS;
-    return launch(attn_pages_f32_kernel, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1), bytes(p.d, p.top), stream);
+    const int G = p.heads / p.kv_heads, chunks = (G + NH - 1) / NH;
+    return launch(attn_pages_f32_kernel<NH>, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1), f32_floats(p.d, NH) * 4 + p.top * 4, stream);
 }
 
 }  // namespace
@@ -485,7 +499,8 @@ GB_API int gb_attention_pages(const PagesParams* pp, int dtype, cudaStream_t str
     if (((uintptr_t)p.k_plane | (uintptr_t)p.v_plane) & 15) GB_REFUSE("%s: the planes must be 16-byte aligned", who);
     if (dtype == GB_F32) {
         if (p.d <= 0 || p.d % 4 || p.d > 256) GB_REFUSE("%s: head_dim %d is not a multiple of 4 up to 256", who, p.d);
-        return launch_f32(p, stream);
+        const int G = p.heads / p.kv_heads;
+        return G <= 1 ? launch_f32<1>(p, stream) : G <= 2 ? launch_f32<2>(p, stream) : G <= 4 ? launch_f32<4>(p, stream) : launch_f32<8>(p, stream);
     }
     if (((uintptr_t)p.q & 15) || (p.q_row_stride & 7)) GB_REFUSE("%s: query rows must be 16-byte aligned", who);
     if (p.max_q_len >= TC5_MIN_ROWS && gb_attention_pages_tc5_accepts(p)) {
