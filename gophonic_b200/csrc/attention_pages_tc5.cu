@@ -165,7 +165,8 @@ __device__ __noinline__ void row_alone(const PagesParams& p, const int* bt, int 
 }
 
 __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                                 const __grid_constant__ CUtensorMap map_v, PagesParams p) {
+                                                                 const __grid_constant__ CUtensorMap map_v,
+                                                                 const __grid_constant__ PagesParams p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* Qs = base;                          // [GROUPS][Q_BYTES]

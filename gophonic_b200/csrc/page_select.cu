@@ -216,7 +216,7 @@ struct Coef64 {
 // `err`.  Warp w has the candidates from w * seg on, 32 at a time; where there are few enough (R > 0: up to 32 R a warp) they stay in
 // registers: every step of the search for the border is a loop over them, and from shared memory it took 670 cycles for 500
 // scores where it takes a tenth.
-template <int W, int BAND>
+template <int W, int BAND, int FEW, int MORE>
 struct Chooser {
     double band_s[BAND];
     int band_i[BAND];        // pages near the border, kept with their 64-bit scores
@@ -381,7 +381,7 @@ struct Chooser {
     // Scores beyond float32, or hundreds that tie: the k-th highest of the 64-bit scores, which are summed anew for every digit.
     // Rare, and right for any input.
     template <typename T>
-    __device__ __noinline__ void slow(const PagesParams& p, const Row<T>& r, uint32_t* key, int warp, int lane) {
+    __device__ __noinline__ void slow(const PagesParams& p, const Row<T> r, uint32_t* key, int warp, int lane) {
         const int nc = r.nc, NT = W * 32, tid = warp * 32 + lane;
         Coef64 c;
         c.load(p, r.q, lane);
@@ -423,14 +423,15 @@ struct Chooser {
     // unsafe: the float32 scores cannot be relied on.
     template <typename T>
     __device__ __forceinline__ void run(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, bool unsafe, int tid) {
-        constexpr int FEW = W == 1 ? 16 : 4;
         const int warp = W == 1 ? 0 : tid >> 5, lane = tid & 31;
         for (int i = tid; i < r.c0; i += W * 32) r.list[i] = i;
         for (int i = tid; i < p.last; i += W * 32) r.list[p.top - p.last + i] = r.n - p.last + i;
         if (r.k > 0) {
             bool done = false;
             if (!unsafe)
-                done = r.nc <= FEW * 32 * W ? fast<T, FEW>(p, r, key, err, warp, lane) : fast<T, 0>(p, r, key, err, warp, lane);
+                done = r.nc <= FEW * 32 * W    ? fast<T, FEW>(p, r, key, err, warp, lane)
+                       : r.nc <= MORE * 32 * W ? fast<T, MORE>(p, r, key, err, warp, lane)
+                                               : fast<T, 0>(p, r, key, err, warp, lane);
             if (!done) slow(p, r, key, warp, lane);
         }
         sync();     // before the group's next row
@@ -446,7 +447,10 @@ constexpr int MAX_PIECES = 8;
 constexpr int ROW_BAND = 512;
 
 struct SelectSmem {
-    Chooser<SELECT_WARPS, ROW_BAND> choose;
+    union {
+        Chooser<SELECT_WARPS, ROW_BAND, 16, 16> all;
+        Chooser<1, ROW_BAND, 16, 32> one;       // up to 1024 candidates: no barriers between the steps of the search
+    } choose;
     float coef[2 * 256];                        // [N | P], in the order of a page's bounds
     float err[MAX_PIECES * SELECT_WARPS];       // of every warp of the cluster; a NaN: unsafe
 };
@@ -472,7 +476,7 @@ __device__ __forceinline__ float sum_many(float (&v)[N], int lane) {
 }
 
 template <typename T, int LP, int CPL>
-__global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams p) {
+__global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(const __grid_constant__ PagesParams p) {
     constexpr int E = Chunk<T>::E, U = 8 / CPL, PER_WARP = 32 / LP;     // pages a group of LP lanes takes at a time
     extern __shared__ __align__(16) unsigned char raw[];
     SelectSmem& s = *reinterpret_cast<SelectSmem*>(raw);
@@ -492,9 +496,29 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams 
         return;
     }
     auto started = cluster.barrier_arrive();    // waited for before the first CTA's memory is written
-    const int d2 = 2 * p.d, G = p.heads / p.kv_heads;
+    const int d2 = 2 * p.d, G = p.heads / p.kv_heads, NC = d2 / E, sub = lane / LP, l = lane % LP;
+    constexpr int BATCH = U * PER_WARP;
+    const int first_batch = (piece * SELECT_WARPS + warp) * BATCH, step = pieces * SELECT_WARPS * BATCH;
+    const T* plane = (const T*)p.bounds;
+    // A lane's page of the batch at i; the numbers are asked for a batch ahead of the bounds, the bounds a batch ahead of their sums.
+    auto page_for = [&](int i) -> int { return lane < BATCH && i + lane < r.nc ? (int)page_of(r.bt, (r.c0 + i + lane) * GB_PAGE, p.bt_stride, p.pages) : 0; };
+    auto ask = [&](int i, int page, uint4 (&x)[U][CPL]) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = min(sub * U + u, r.nc - 1 - i);     // pages beyond the last are the last once more
+            const int64_t pg = __shfl_sync(0xffffffffu, page, at);
+            const uint4* b = reinterpret_cast<const uint4*>(plane + (pg * p.kv_heads + r.kvh) * d2);
+#pragma unroll
+            for (int j = 0; j < CPL; j++) x[u][j] = l + j * LP < NC ? b[l + j * LP] : make_uint4(0, 0, 0, 0);
+        }
+    };
+    uint4 now[U][CPL];
+    int next = page_for(first_batch);
+    if (first_batch < r.nc) ask(first_batch, next, now);
+    next = page_for(first_batch + step);
     for (int c = tid; c < p.d; c += SELECT_THREADS) {
         float up = 0.f, down = 0.f;
+#pragma unroll 4
         for (int h = 0; h < G; h++) {
             const float x = to_f32<T>(r.q[(int64_t)h * p.d + c]);
             up += x <= 0.f ? 0.f : x;      // a NaN is in both
@@ -505,7 +529,6 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams 
     }
     __syncthreads();
     cluster.barrier_wait(std::move(started));
-    const int NC = d2 / E, sub = lane / LP, l = lane % LP;
     float cf[CPL][E], mx[CPL][E];
 #pragma unroll
     for (int j = 0; j < CPL; j++)
@@ -516,34 +539,18 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams 
         }
     uint32_t* keys0 = cluster.map_shared_rank(key, 0);
     bool odd = false;
-    const T* plane = (const T*)p.bounds;
-    constexpr int BATCH = U * PER_WARP;
-    auto page_for = [&](int i) -> int { return lane < BATCH && i + lane < r.nc ? (int)page_of(r.bt, (r.c0 + i + lane) * GB_PAGE, p.bt_stride, p.pages) : 0; };
-    const int first_batch = (piece * SELECT_WARPS + warp) * BATCH, step = pieces * SELECT_WARPS * BATCH;
-    int next = page_for(first_batch);      // a lane a page: asked for a batch ahead of its bounds
     for (int i0 = first_batch; i0 < r.nc; i0 += step) {
-        const int page = next;
-        uint4 x[U][CPL];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            // pages beyond the last are the sequence's last once more
-            const int at = min(sub * U + u, r.nc - 1 - i0);
-            const int64_t pg = __shfl_sync(0xffffffffu, page, at);
-            const uint4* b = reinterpret_cast<const uint4*>(plane + (pg * p.kv_heads + r.kvh) * d2);
-#pragma unroll
-            for (int j = 0; j < CPL; j++)
-                if (l + j * LP < NC) x[u][j] = b[l + j * LP];
-        }
-        next = page_for(i0 + step);
+        uint4 then[U][CPL];
+        if (i0 + step < r.nc) ask(i0 + step, next, then);
+        next = page_for(i0 + 2 * step);
         float acc[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             acc[u] = 0.f;
 #pragma unroll
             for (int j = 0; j < CPL; j++) {
-                if (l + j * LP >= NC) break;
                 float f[E];
-                unpack(x[u][j], f);
+                unpack(now[u][j], f);
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     acc[u] = fmaf(cf[j][e], f[e], acc[u]);
@@ -556,6 +563,10 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams 
         const int i = i0 + sub * U + l / SHARE;
         odd = odd || !(fabsf(sum) <= 3.0e38f);
         if (l % SHARE == 0 && i < r.nc) keys0[i] = order_key(sum);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < CPL; j++) now[u][j] = then[u][j];
     }
     float most = 0.f;      // the sum of the terms' sizes is no more than that of the coefficients times the channels' largest bounds
 #pragma unroll
@@ -575,14 +586,19 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams 
     if (piece != 0) return;
     float err = 0.f;
     bool unsafe = false;
-    for (int w = 0; w < pieces * SELECT_WARPS; w++) {
+    for (int w = lane; w < pieces * SELECT_WARPS; w += 32) {
         err = fmaxf(err, s.err[w]);
         unsafe = unsafe || !(s.err[w] <= 3.0e38f);
     }
+    err = warp_max(err);
+    unsafe = __any_sync(0xffffffffu, unsafe);
     // A float32 sum of at most 16 products a lane and 5 steps between lanes, of coefficients that are sums of G values: 22 + G half steps
     // of 2^-23 relative to the sum of the terms' sizes, itself known to 2^-18; products below the normal range add next to nothing.
     err = err * ((24.f + (float)G) * 5.9604645e-8f) + 1.0e-42f;
-    s.choose.run(p, r, key, err, unsafe, tid);
+    if (r.nc > 1024)
+        s.choose.all.run(p, r, key, err, unsafe, tid);
+    else if (warp == 0)
+        s.choose.one.run(p, r, key, err, unsafe, lane);
 }
 
 // Runs of rows -----------------------------------------------------------------------------------
@@ -593,7 +609,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(PagesParams 
 constexpr int TILE_THREADS = 512, TILE_WARPS = TILE_THREADS / 32, TILE_BAND = 48;
 
 struct alignas(16) TileSmem {
-    Chooser<1, TILE_BAND> choose[TILE_WARPS];
+    Chooser<1, TILE_BAND, 16, 16> choose[TILE_WARPS];
     float size[64];          // per chunk of 8 bounds: their largest size, over all pages
 };
 
@@ -601,7 +617,7 @@ __host__ __device__ inline int tile_coef_stride(int d) { return 2 * d + 32; }   
 __host__ __device__ inline int tile_key_stride(int pages) { return (pages + 31) / 32 * 32 + 8; }
 
 template <int MT, int KB_MAX>
-__global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(PagesParams p) {
+__global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(const __grid_constant__ PagesParams p) {
     constexpr int RT = MT * 16;
     extern __shared__ __align__(16) unsigned char raw[];
     TileSmem& s = *reinterpret_cast<TileSmem*>(raw);
