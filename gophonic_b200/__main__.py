@@ -44,6 +44,9 @@ def main(argv=None) -> int:
     ap.add_argument("-stop", "--stop", default=None,
                     help="comma-separated stop token ids (default: the end-of-sequence ids the model folder names; '' for none)")
     ap.add_argument("-batch", "--batch", type=int, default=8, help="sequences that start together")
+    ap.add_argument("-sparse-pages", "--sparse-pages", type=int, default=0,
+                    help="pages of 64 tokens that a reply's token reads of its context (0: all of it)")
+    ap.add_argument("-sparse-prompts", "--sparse-prompts", action="store_true", help="prompts read no more than that either")
     ap.add_argument("-device", "--device", default="cuda:0")
     ap.add_argument("-prompt-ids", "--prompt-ids", default="", help="a file of prompts, one a line, as token ids")
     ap.add_argument("-prompt", "--prompt", action="append", default=[], help="a question in text (needs the folder's tokenizer.json)")
@@ -77,7 +80,8 @@ def main(argv=None) -> int:
         if not prompts and not args.prompt:
             raise ValueError("no prompt: give token ids, -prompt-ids FILE or -prompt TEXT")
         path = args.model or random_model_path(args.random_config, args.weights_seed, args.layers)
-        model = Open(path, Options(Threads=args.threads, Format=args.format, Device=args.device, Batch=args.batch))
+        model = Open(path, Options(Threads=args.threads, Format=args.format, Device=args.device, Batch=args.batch,
+                                   SparsePages=args.sparse_pages, SparsePrompts=args.sparse_prompts))
         opts = ChatOptions(MaxTokens=args.max_tokens, Temperature=args.temperature, TopK=args.top_k,
                            TopP=args.top_p, Presence=args.presence, Seed=args.seed)
         if prompts:

@@ -54,6 +54,11 @@ class Options:
     # up to 64); Batch bounds how many sequences start together.
     CacheTokens: int = 0
     Batch: int = 8
+    # SparsePages > 0: behind more than that many pages of 64 tokens, a token of a layer that attends to its whole context reads
+    # only so many pages: the first, the two up to its own, and those whose keys could score highest.  Replies behind long
+    # contexts then cost what a context of 64 * SparsePages costs.  Prompts are still read in full, unless SparsePrompts.
+    SparsePages: int = 0
+    SparsePrompts: bool = False
 
 
 @dataclass
@@ -130,6 +135,8 @@ def Open(path: str, opts: Optional[Options] = None) -> OpenedModel:
     opts = opts or Options()
     if opts.Threads < 0:
         raise ValueError(f"gophonic_b200: invalid thread count {opts.Threads}")
+    if opts.SparsePages and not 3 <= opts.SparsePages <= 1024 or opts.SparsePrompts and not opts.SparsePages:
+        raise ValueError(f"gophonic_b200: {opts.SparsePages} pages a token (0: all; else 3 to 1024)")
     if opts.Format not in ("", FormatBF16, FormatF32):
         raise ErrUnsupported(f"gophonic_b200: unknown weight format '{opts.Format}'")
     f = Detect(path)
@@ -225,10 +232,18 @@ def _open_chat(model, opts: Options, path: str):
     return ChatGenerator(engine, sampler, min(context, engine.capacity), template, tokenizer)
 
 
+def _selection(opts: Options):
+    """The page selection the options ask for, or None."""
+    if not opts.SparsePages:
+        return None
+    from .config.spec import PageSelection
+    return PageSelection(opts.SparsePages, prompts=opts.SparsePrompts)
+
+
 def _open_dir(path: str, opts: Options) -> OpenedModel:
     from .engine.model import Model
     mode = "float32" if opts.Format == FormatF32 else "bfloat16"
-    model = Model.from_dir(path, dtype=mode, device=opts.Device)
+    model = Model.from_dir(path, dtype=mode, device=opts.Device, selection=_selection(opts))
     m = OpenedModel(model.spec.architecture, path)
     m.model = model
     Provide(m, TokensGenerator, lambda: TokenGenerator(model, opts, read_stop_ids(path)))
@@ -280,7 +295,7 @@ def _open_random(path: str, opts: Options) -> OpenedModel:
     from .engine.model import Model
     config, seed = _parse_random(path)
     mode = "float32" if opts.Format == FormatF32 else "bfloat16"
-    model = Model.from_random(config, seed=seed, dtype=mode, device=opts.Device)
+    model = Model.from_random(config, seed=seed, dtype=mode, device=opts.Device, selection=_selection(opts))
     m = OpenedModel(model.spec.architecture, path)
     m.model = model
     Provide(m, TokensGenerator, lambda: TokenGenerator(model, opts, ()))

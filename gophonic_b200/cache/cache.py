@@ -8,7 +8,7 @@ block.  A block table [slot][logical page] -> physical page, mirrored on the dev
 by every group: page p of a sequence is physical page table[slot][p] in every plane.
 
 Groups.  Runs of layers are grouped by what they need: (kv_heads, head_dim, window) for
-key/value planes (and the size of a value head where it is not a key head's), (shape, dtype) for fixed-size state.  Each group has storage of its own; a run
+key/value planes (and the size of a value head where it is not a key head's; a run may ask for bounds beside its group's keys), (shape, dtype) for fixed-size state.  Each group has storage of its own; a run
 is given the plane with its ordinal inside its group (the reference indexes KV planes the same
 way, by a layer's place among layers of its kind: internal/qwen3lm/gpu_darwin.go:51-55, 270-277,
 831, and keeps per-sequence state beside K/V: gpu_darwin.go:800-808).  A run that reads another
@@ -106,6 +106,8 @@ class KVView:
     writable: bool
     window: int
     state: Optional[torch.Tensor] = None   # [max_slots, *shape]: fixed-size state beside the keys, if the run asked for it
+    bounds: Optional[torch.Tensor] = None  # [n_pages, kv_heads, 2, head_dim]: the full pages' lowest and highest key values, if a run
+                                           # of the group asked for them
 
 
 @dataclass
@@ -164,6 +166,7 @@ class Cache:
 
         # groups
         self._kv_groups: Dict[Tuple[int, ...], List[int]] = {}
+        self._bounded: set = set()                            # the groups with bounds beside their keys
         self._state_groups: Dict[Tuple[Tuple[int, ...], torch.dtype], List[int]] = {}
         self._plane: Dict[int, Tuple[str, object, int]] = {}
         self._beside: Dict[int, Tuple[object, int]] = {}     # the state plane of a run that asked for keys and state
@@ -197,6 +200,8 @@ class Cache:
                 self._v[key] = self._k[key][..., :dv]      # a view: the first channels of every key
             else:
                 self._v[key] = torch.zeros((len(planes), self.n_pages + 1, vh, PAGE, dv), dtype=dtype, device=self.device)
+        self._bounds = {key: torch.zeros(k.shape[:3] + (2, k.shape[4]), dtype=dtype, device=self.device)
+                        for key, k in self._k.items() if key in self._bounded}
         self._state: Dict[Tuple[Tuple[int, ...], torch.dtype], torch.Tensor] = {}
         for key, planes in self._state_groups.items():
             shape, sdtype = key
@@ -231,6 +236,10 @@ class Cache:
                 key += (req.value_dim or req.head_dim, vheads or req.kv_heads, in_keys)
             elif req.value_dim and req.value_dim != req.head_dim:
                 key += (req.value_dim,)
+            if getattr(req, "bounds", False):
+                if in_keys:
+                    raise CacheError(f"schedule position {pos}: no bounds are kept of keys that hold their values")
+                self._bounded.add(key)
             planes = self._kv_groups.setdefault(key, [])
             self._plane[pos] = ("kv", key, len(planes))
             planes.append(pos)
@@ -291,8 +300,20 @@ class Cache:
             if at in self._beside:
                 skey, sord = self._beside[at]
                 state = self._state[skey][sord]
-            return KVView(self._k[key][ordinal], self._v[key][ordinal], self.block_table, writable, key[2], state)
+            bounds = self._bounds[key][ordinal] if key in self._bounds else None
+            return KVView(self._k[key][ordinal], self._v[key][ordinal], self.block_table, writable, key[2], state, bounds)
         return StateView(self._state[key][ordinal], writable)
+
+    def keep_bounds(self, batch) -> None:
+        """Behind all layers of a step of single tokens: the bounds of the pages it has filled, in every plane that keeps them, by one
+        kernel a group.  (A token always reads its own page, so the step itself has no use for them.  A run of tokens that
+        selects pages needs those it fills itself: its mixer sees to them layer by layer.)  A page that is refilled after a
+        ``truncate`` or ``restore`` gets its bounds anew when its last token is written; until then nothing reads them."""
+        if self._bounds and self._ops is None:
+            raise CacheError("bounds beside the keys need the kernel library (``attach``)")
+        for key, bounds in self._bounds.items():
+            self._ops.page_bounds(self._k[key], bounds, self.block_table, batch.seq_slot, batch.seq_q_len, batch.seq_kv_len, batch.nseq,
+                                  batch.max_q_len)
 
     # ---- slots -------------------------------------------------------------------------
     def alloc_slot(self) -> int:

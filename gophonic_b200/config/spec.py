@@ -13,6 +13,7 @@ shared struct.
 """
 from __future__ import annotations
 
+import dataclasses
 from dataclasses import dataclass, field
 from typing import Optional, Sequence, Tuple
 
@@ -105,6 +106,29 @@ class AttentionSpec:
     qk_norm: Optional[RMSNormSpec] = None
     window: int = 0
     kind: str = "attention"
+
+
+@dataclass(frozen=True)
+class PageSelection:
+    """How much of its context a token reads: ``pages`` pages of 64 tokens in all, among them always the first ``first`` and the
+    last ``last`` (its own included), the others those whose keys could score highest.  ``prompts`` False: only single tokens
+    select, runs of tokens (prompts) attend to everything; True: every token does, so that a token's result does not depend
+    on whether it came in a prompt or alone."""
+    pages: int
+    first: int = 1
+    last: int = 2
+    prompts: bool = False
+
+    def __post_init__(self):
+        if self.first < 0 or self.last < 1 or self.pages < self.first + self.last:
+            raise ValueError(f"page selection: {self.pages} pages, of which the first {self.first} and the last {self.last} (at least one) are always read")
+
+
+@dataclass(frozen=True)
+class SparseAttentionSpec(AttentionSpec):
+    """Grouped-query causal attention of which a token reads a part of the cache (``PageSelection``); no window."""
+    selection: Optional[PageSelection] = None
+    kind: str = "sparse_attention"
 
 
 @dataclass(frozen=True)
@@ -664,3 +688,18 @@ class ModelSpec:
 
 def default_schedule(n_layers: int) -> Tuple[ScheduleEntry, ...]:
     return tuple(ScheduleEntry(layer=i) for i in range(n_layers))
+
+
+def with_page_selection(spec: ModelSpec, selection: PageSelection) -> ModelSpec:
+    """``spec`` with every plain attention over the whole context (``AttentionSpec``, no window) turned into one that reads the
+    selected pages; the weights are the same.  ValueError if the model has no such layer."""
+    layers = []
+    for layer in spec.layers:
+        mixer = getattr(layer, "mixer", None)
+        if type(mixer) is AttentionSpec and mixer.window == 0:
+            values = {f.name: getattr(mixer, f.name) for f in dataclasses.fields(mixer) if f.name != "kind"}
+            layer = dataclasses.replace(layer, mixer=SparseAttentionSpec(**values, selection=selection))
+        layers.append(layer)
+    if tuple(layers) == tuple(spec.layers):
+        raise ValueError(f"{spec.architecture}: no layer attends to its whole context in the plain way; there is nothing to select pages for")
+    return dataclasses.replace(spec, layers=tuple(layers))

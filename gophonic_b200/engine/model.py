@@ -16,6 +16,7 @@ import torch
 
 from .. import registry
 from ..cache import Cache
+from ..config.spec import with_page_selection
 from ..parts.base import RowStats, Runtime, fold_buffers, fold_weight
 from ..weights import InitScales, declare_model, load_tensors, random_tensors_on_device
 from ..weights.declare import final_norm_prefix
@@ -86,21 +87,22 @@ class Model:
 
     # ---- construction --------------------------------------------------------------------
     @classmethod
-    def from_dir(cls, model_dir: str, dtype="bfloat16", device="cuda:0") -> "Model":
+    def from_dir(cls, model_dir: str, dtype="bfloat16", device="cuda:0", selection=None) -> "Model":
+        """``selection``: a ``PageSelection`` for the layers that attend to their whole context (``with_page_selection``)."""
         mode = dtype_mode(dtype)
         config = registry.read_config(model_dir)
-        spec = config.model_spec()
+        spec = config.model_spec() if selection is None else with_page_selection(config.model_spec(), selection)
         rt = make_runtime(mode, device)
         tensors = load_tensors(model_dir, declare_model(spec), mode, rt.device)
         return cls(spec, tensors, rt, config)
 
     @classmethod
     def from_random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0",
-                    scales: InitScales = InitScales()) -> "Model":
+                    scales: InitScales = InitScales(), selection=None) -> "Model":
         """Random weights made on the device (for sizes too large to pass through a file): the tensors
         ``write_random_model`` writes for the same configuration and seed, bit for bit."""
         mode = dtype_mode(dtype)
-        spec = config.model_spec()
+        spec = config.model_spec() if selection is None else with_page_selection(config.model_spec(), selection)
         rt = make_runtime(mode, device)
         tied = bool(getattr(config, "tie_word_embeddings", False))
         tensors = random_tensors_on_device(spec, seed, mode, rt.device, scales, tied=tied, ops=rt.ops)
@@ -151,12 +153,20 @@ class Model:
     def forward(self, batch, cache: Cache, want_rows: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
         """Run the rows of ``batch`` through every scheduled layer; return fp32 logits
         [len(want_rows), vocab] for the wanted packed rows (None if none are wanted)."""
+        if self._takes_streams[0]:
+            logits = self._forward_streams(batch, cache, want_rows)
+        elif self._takes_history[0]:
+            logits = self._forward_history(batch, cache, want_rows)
+        else:
+            logits = self._forward_residual(batch, cache, want_rows)
+        if batch.max_q_len == 1:
+            cache.keep_bounds(batch)
+        return logits
+
+    def _forward_residual(self, batch, cache: Cache, want_rows: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """The pass for blocks that share one residual."""
         ops = self.rt.ops
         rows = batch.rows
-        if self._takes_streams[0]:
-            return self._forward_streams(batch, cache, want_rows)
-        if self._takes_history[0]:
-            return self._forward_history(batch, cache, want_rows)
         h = torch.empty((rows, self.spec.hidden), dtype=torch.float32, device=self.rt.device)
         # What is still owed to the residual travels from block to block: an addend not yet added, the
         # rows' statistics (``RowStats``) where the last kernel left them, or nothing.

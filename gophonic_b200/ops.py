@@ -856,6 +856,14 @@ def _need_rows(who: str, name: str, t: torch.Tensor, dtype, width: int) -> None:
         raise KernelError(f"{who}: {name} {tuple(t.shape)} with strides {tuple(t.stride())} for rows of {width}")
 
 
+def page_attention_accepts(dtype: torch.dtype, head_dim: int) -> bool:
+    """Whether ``page_bounds``, ``select_pages`` and ``attention_pages`` all take heads of this size: bfloat16 in steps of 16 up to 128,
+    and 256; float32 in steps of 4 up to 256."""
+    if dtype == torch.bfloat16:
+        return head_dim > 0 and head_dim % 16 == 0 and (head_dim <= 128 or head_dim == 256)
+    return dtype == torch.float32 and 0 < head_dim <= 256 and head_dim % 4 == 0
+
+
 def page_bounds(k_planes: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_slot: torch.Tensor, seq_q_len: torch.Tensor,
                 seq_kv_len: torch.Tensor, nseq: int, max_q_len: int) -> None:
     """The extremes of every key channel of the pages that a step has filled: for each sequence's pages whose last position is among

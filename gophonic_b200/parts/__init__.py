@@ -21,6 +21,7 @@ from .reinject import AddStart, Reinject
 from .rope import NoPosition, PairRotaryEmbedding, RotaryEmbedding
 from .sandwich import SandwichBlock
 from .sigmoid_attention import SigmoidAttention
+from .sparse_attention import SparseAttention
 from .swiglu import SwiGLU
 
 registry.register_norm("rmsnorm", RMSNorm)
@@ -29,6 +30,7 @@ registry.register_position("rope_pairs", PairRotaryEmbedding)
 registry.register_position("none", NoPosition)
 registry.register_mixer("attention", Attention)
 registry.register_mixer("gated_attention", GatedAttention)
+registry.register_mixer("sparse_attention", SparseAttention)
 registry.register_mixer("gla", DecayState)
 registry.register_mixer("mlstm", MatrixMemory)
 registry.register_mixer("sigmoid_attention", SigmoidAttention)
@@ -50,5 +52,5 @@ registry.register_block("sandwich", SandwichBlock)
 registry.register_junction("reinject", Reinject)
 registry.register_junction("add_start", AddStart)
 
-__all__ = ["AddStart", "BlockStateRequest", "GatedDelta", "Gelu", "Parallel", "PartsRequest", "ForgetState", "SandwichBlock", "ClampedGLU", "DiffAttention", "LatentAttention", "PostNormBlock", "ReluSquared", "Attention", "DecayState", "DeltaRule", "FeedForward", "GatedAttention", "HyperBlock", "KVStateRequest", "MatrixMemory", "MoE", "SigmoidAttention", "PairRotaryEmbedding", "KVRequest", "Mixer", "NoPosition", "Norm", "Part", "PositionEncoding",
+__all__ = ["AddStart", "BlockStateRequest", "GatedDelta", "Gelu", "Parallel", "PartsRequest", "ForgetState", "SandwichBlock", "ClampedGLU", "DiffAttention", "LatentAttention", "PostNormBlock", "ReluSquared", "Attention", "DecayState", "DeltaRule", "FeedForward", "GatedAttention", "HyperBlock", "KVStateRequest", "MatrixMemory", "MoE", "SigmoidAttention", "SparseAttention", "PairRotaryEmbedding", "KVRequest", "Mixer", "NoPosition", "Norm", "Part", "PositionEncoding",
            "PreNormBlock", "Reinject", "RMSNorm", "RotaryEmbedding", "Runtime", "StateRequest", "SwiGLU", "TensorDecl"]

@@ -50,6 +50,7 @@ class KVRequest:
     value_heads: int = 0          # value heads a token has if not ``kv_heads`` (several key heads may read one value head)
     values_in_keys: bool = False  # the values are the first ``value_dim`` channels of the keys: no value plane is kept,
                                   # the run's ``v`` is a view of its key plane
+    bounds: bool = False          # keep the extremes of every key channel of the full pages beside the keys (``view.bounds``)
 
 
 @dataclass(frozen=True)

@@ -22,7 +22,7 @@ def refused(name, dtype, **kw):
 
 BAD = {
     "gb_page_bounds": [dict(d=20), dict(d=264), dict(d=0), dict(kv_heads=0), dict(pages=0), dict(bt_stride=0), dict(max_slots=0), dict(bounds=4098),
-                       dict(k_plane=4104), dict(planes=40000), dict(nseq=70000)],
+                       dict(k_plane=4104), dict(planes=1 << 28), dict(nseq=70000)],
     "gb_select_pages": [dict(d=20), dict(heads=3), dict(heads=0), dict(first=-1), dict(last=0), dict(first=3), dict(top=2), dict(top=0), dict(bt_stride=32769),
                         dict(bounds=4098), dict(nseq=1 << 20, max_q_len=1 << 12)],
     "gb_attention_pages": [dict(d=20), dict(d=144), dict(d=272), dict(heads=3), dict(kv_heads=0), dict(top=0), dict(top=1025), dict(pages=0), dict(k_plane=4104),
