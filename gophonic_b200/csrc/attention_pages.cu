@@ -16,7 +16,7 @@
 #include <math.h>
 
 int gb_attention_pages_tc5_accepts(const PagesParams& p);
-int gb_attention_pages_tc5(const PagesParams& p, int pieces, cudaStream_t stream);
+int gb_attention_pages_tc5(const PagesParams& p, cudaStream_t stream);
 
 namespace {
 
@@ -26,7 +26,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int THREADS = 128;
 constexpr int MAX_TOP = 1024;     // entries of a list
 constexpr int MAX_PIECES = 8;     // CTAs of a cluster: the portable most
-constexpr int TC5_MIN_ROWS = 16;  // rows of a sequence from which on its tiles run on tcgen05 (attention_pages_tc5.cu)
+// Rows times key heads from which on runs of rows go to tcgen05 (attention_pages_tc5.cu), us here / there, 32 pages behind 20000: 8
+// key heads, one sequence of 4 rows 11.7 / 14.0, of 8 rows 16.8 / 15.6, of 16 rows 28 / 18; eight sequences of 2 rows 28 / 20; two
+// key heads, one sequence of 16 rows 13 / 18, of 32 rows 18 / 19, of 48 rows 28 / 21.
+constexpr int TC5_MIN_UNITS = 64;
 
 // The row's listed pages that it can see, in the list's order, packed into `to`; how many there are.  Every thread of the CTA.
 __device__ __forceinline__ int pack_list(const PagesParams& p, const int* list, int own_page, int* to, int* counts) {
@@ -507,13 +510,7 @@ GB_API int gb_attention_pages(const PagesParams* pp, int dtype, cudaStream_t str
         return G <= 1 ? launch_f32<1>(p, stream) : G <= 2 ? launch_f32<2>(p, stream) : G <= 4 ? launch_f32<4>(p, stream) : launch_f32<8>(p, stream);
     }
     if (((uintptr_t)p.q & 15) || (p.q_row_stride & 7)) GB_REFUSE("%s: query rows must be 16-byte aligned", who);
-    if (p.max_q_len >= TC5_MIN_ROWS && gb_attention_pages_tc5_accepts(p)) {
-        int gp = 1, pieces = 1;
-        while (gp < p.heads / p.kv_heads) gp *= 2;
-        const int64_t tiles = (int64_t)p.nseq * ceil_div(p.max_q_len, 256 / gp) * p.kv_heads;
-        while (pieces < MAX_PIECES && tiles * pieces * 2 <= gb_sm_count()) pieces *= 2;
-        return gb_attention_pages_tc5(p, pieces, stream);
-    }
+    if (p.max_q_len > 1 && (int64_t)p.nseq * p.max_q_len * p.kv_heads >= TC5_MIN_UNITS && gb_attention_pages_tc5_accepts(p)) return gb_attention_pages_tc5(p, stream);
     switch (p.d) {
         case 16: return launch_mma<16>(p, stream);
         case 32: return launch_mma<32>(p, stream);

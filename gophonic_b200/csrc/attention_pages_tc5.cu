@@ -1,16 +1,21 @@
 // Attention over listed pages for runs of rows, on the fifth-generation tensor cores (bfloat16, head_dim 128).
 //
 // Every row has a list of pages of its own, but rows that follow one another list nearly the same ones.  A CTA owns a tile of one
-// sequence and kv head, 256 rows of (token, query head of the group) in two groups of 128, and walks the pages that any of its
-// tokens lists, each once: its keys and values are fetched once for the tile.  For each of these pages a word of bits says which
-// tokens list it.  A group's products are issued for the pages its own tokens list; a warp none of whose tokens lists the
-// page writes zero weights without looking at the scores; a row that does not list it takes none of what its warp finds.
-//     S_g = Q_g K^T   (M 128, N 64 keys, K 128)   -> two S buffers of 64 columns per group
-//     O_g += P_g V    (M 128, N 128, K 64 keys)    -> one O buffer of 128 columns per group
-// Roles by warp: warp 0 loads queries and keys by TMA, the one behind the softmax warps the values, four pages deep each; one
-// thread each of warps 1-2 issues the scores products of group A and B, one each of warps 3-4 their values products; warps 5-8
-// and 9-12 are the softmax of group A and B (a thread a row, probabilities back into tensor memory as the second product's A
-// operand, O rescaled only when a row's maximum has grown by more than 2^8 since the scale in use was chosen).
+// sequence and kv head, 128 rows of (token, query head of the group), and walks the pages that any of its tokens lists, each
+// once: its keys and values are fetched once for the tile.  For each of these pages a word of bits says which tokens list it.  A
+// warp none of whose tokens lists the page writes zero weights without looking at the scores; a row that does not list it
+// takes none of what its warp finds.
+//     S = Q K^T   (M 128, N 64 keys, K 128)   -> two S buffers of 64 columns
+//     O += P V    (M 128, N 128, K 64 keys)    -> 128 columns
+// Roles by warp: warp 0 loads queries and keys by TMA, the last one the values, two pages deep each; one thread each of warps 1 and
+// 2 issues the scores and the values products; warps 3-6 are the softmax (a thread a row, probabilities back into tensor memory
+// over the scores as the second product's A operand, O rescaled only when a row's maximum has grown by more than 2^8 since the
+// scale in use was chosen).
+//
+// Two CTAs share an SM (110 KB, half of the tensor memory each).  A page takes a CTA some 2000 cycles, of which the softmax has 900,
+// and the chain probabilities - values product - next scores in the same buffer most of the rest; two CTAs overlap.  2000 rows of
+// 32 heads over 8 behind 30700, 32 pages each (113 in a tile): 237 us; with two groups of 128 rows in one CTA of four stages,
+// whose tiles list 163 pages, 279; with one group in a CTA of three or four stages, which has the SM to itself, 394.
 //
 // The heads of a group are rows of the tile (a group of G heads takes the next power of two: a tensor map of three dimensions
 // brings token after token, head after head), so that they share every page too.
@@ -21,6 +26,7 @@
 //
 // Where there are few tiles, a cluster of CTAs shares one: each takes a stretch of the pages, and they join their rows through
 // distributed shared memory.  All barrier waits are bounded; one that gives up sets a status word and the CTA runs out.
+#include "mma.cuh"
 #include "tc5.cuh"
 #include "api.h"
 
@@ -34,29 +40,27 @@ namespace cg = cooperative_groups;
 __device__ int g_status;
 
 typedef __nv_bfloat16 bf16;
-constexpr int HD = 128, BQ = 128, GROUPS = 2, ROWS = GROUPS * BQ, BKV = 64, STAGES = 4;
-constexpr int FIRST_SOFTMAX_WARP = 1 + 2 * GROUPS;
-constexpr int VALUE_LOADER_WARP = FIRST_SOFTMAX_WARP + 4 * GROUPS, WARPS = VALUE_LOADER_WARP + 1, THREADS = WARPS * 32;
+constexpr int HD = 128, BKV = 64;
 constexpr int QPANEL = 128 * 128;               // 128 rows of 128 bytes (64 channels)
 constexpr int KPANEL = 64 * 128;                // 64 keys of 128 bytes
 constexpr int Q_BYTES = 2 * QPANEL, K_BYTES = 2 * KPANEL, V_BYTES = 2 * KPANEL, STAGE_BYTES = K_BYTES + V_BYTES;
-constexpr int TILE_BYTES = GROUPS * Q_BYTES + STAGES * STAGE_BYTES;
-constexpr int LIST_BYTES = 232448 - 3072 - 1024 - TILE_BYTES;   // for the tile's pages and their bits, beside the static part and the alignment
+constexpr int ROWS = 128, STAGES = 2;
+constexpr int FIRST_SOFTMAX_WARP = 3, VALUE_LOADER_WARP = FIRST_SOFTMAX_WARP + 4, WARPS = VALUE_LOADER_WARP + 1, THREADS = WARPS * 32;
+constexpr int TILE_BYTES = Q_BYTES + STAGES * STAGE_BYTES;
+constexpr int LIST_BYTES = 232448 - 3072 - 1024 - TILE_BYTES;   // most for the tile's pages and their bits, beside the static part and the alignment
+constexpr int TMEM_COLS = 256, O_COL = 128;                     // two buffers of 64 columns for S, then O
+static_assert(ROWS * HD * 4 <= STAGES * STAGE_BYTES, "a tile's sums fit where the pages were");
 constexpr int MAX_TABLE = 32768;                // pages of a sequence: their bitmap is made where the pages will go
-constexpr int TMEM_COLS = 512;                  // S: 2 groups x 2 buffers x 64; O: 2 groups x 128
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_AT = 8.0f;
 constexpr int MAX_PIECES = 8;
-static_assert(ROWS * HD * 4 <= STAGES * STAGE_BYTES, "a tile's sums fit where the pages were");
-
 // The tile: tokens, bits of a page's entry.
 __host__ __device__ inline int padded_group(int G) {
     int gp = 1;
     while (gp < G) gp *= 2;
     return gp;
 }
-__host__ __device__ inline int tile_tokens(int gp) { return ROWS / gp; }
-__host__ __device__ inline int mask_words(int gp) { return tile_tokens(gp) > 32 ? tile_tokens(gp) / 32 : 1; }
+__host__ __device__ inline int mask_words(int tokens) { return tokens > 32 ? tokens / 32 : 1; }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(s32(bar)) : "memory");
@@ -92,6 +96,47 @@ __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
+}
+// Packed pairs of fp32: one instruction works on two values.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2_down(uint64_t a, uint64_t b) {  // rounded towards minus infinity
+    uint64_t d;
+    asm("add.rm.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// 2^x of two values on the FMA pipe, for a quarter of the exponentials (the special-function unit takes eight cycles for a warp's):
+// x = n + f by adding 1.5 * 2^23 rounded down, 2^f by a cubic (relative error 1.9e-4, a twentieth of the bfloat16 step the
+// probabilities are rounded to), n added into the exponent field.
+__device__ __forceinline__ void exp2_poly_x2(uint64_t x, float& y0, float& y1) {
+    float x0, x1;
+    unpack2(x, x0, x1);
+    x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    const uint64_t r = add2_down(x, pack2(12582912.f, 12582912.f));
+    const uint64_t n = add2(r, pack2(-12582912.f, -12582912.f));
+    const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
+    uint64_t q = fma2(f, pack2(0.0790199414f, 0.0790199414f), pack2(0.2241264433f, 0.2241264433f));
+    q = fma2(q, f, pack2(0.6968385577f, 0.6968385577f));
+    q = fma2(q, f, pack2(0.9998119473f, 0.9998119473f));
+    float q0, q1, r0, r1;
+    unpack2(q, q0, q1);
+    unpack2(r, r0, r1);
+    y0 = __int_as_float(__float_as_int(q0) + (__float_as_int(r0) << 23));
+    y1 = __int_as_float(__float_as_int(q1) + (__float_as_int(r1) << 23));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -164,15 +209,15 @@ __device__ __noinline__ void row_alone(const PagesParams& p, const int* bt, int 
     for (int e = 0; e < 4; e++) to[e] = __float2bfloat16_rn(o[e] * inv);
 }
 
-__global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                  const __grid_constant__ CUtensorMap map_v,
                                                                  const __grid_constant__ PagesParams p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    unsigned char* Qs = base;                          // [GROUPS][Q_BYTES]
-    unsigned char* KVs = Qs + GROUPS * Q_BYTES;        // [STAGES][K | V]
+    unsigned char* Qs = base;                 // two panels of 64 channels
+    unsigned char* KVs = Qs + Q_BYTES;        // [STAGES][K | V]
     __shared__ uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES];
-    __shared__ uint64_t s_full[GROUPS][2], p_full[GROUPS][2], o_done[GROUPS][2];
+    __shared__ uint64_t s_full[2], p_full[2], o_done[2];
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s, n_s;
     __shared__ float row_m[ROWS], row_l[ROWS];         // of a tile that several CTAs share
@@ -182,7 +227,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
     pdl_trigger();
     const cg::cluster_group cluster = cg::this_cluster();
     const int pieces = (int)cluster.num_blocks(), piece = (int)cluster.block_rank();
-    const int G = p.heads / p.kv_heads, GP = padded_group(G), TOK = tile_tokens(GP), TOKG = TOK / GROUPS, MW = mask_words(GP);
+    const int G = p.heads / p.kv_heads, GP = padded_group(G), TOK = ROWS / GP, MW = mask_words(TOK);
     const int seq = blockIdx.z, kvh = blockIdx.y;
     const int q_len = p.seq_q_len[seq], kv_len = p.seq_kv_len[seq];
     const int q0 = ((int)blockIdx.x / pieces) * TOK;
@@ -190,7 +235,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
     const int past = kv_len - q_len, q_start = p.seq_q_start[seq];
     const int tokens = min(TOK, q_len - q0);
     const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
-    int* entry = reinterpret_cast<int*>(KVs + STAGES * STAGE_BYTES);    // page | bit 30: group A lists it | bit 31: group B
+    int* entry = reinterpret_cast<int*>(KVs + STAGES * STAGE_BYTES);    // the tile's pages
     const int cap = min(TOK * p.top, p.bt_stride);
     uint32_t* bits = reinterpret_cast<uint32_t*>(entry + cap);          // [entry][MW]: the tokens that list it
 
@@ -199,27 +244,23 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&k_full[s], 1);
             mbar_init(&v_full[s], 1);
-            mbar_init(&k_empty[s], GROUPS);
-            mbar_init(&v_empty[s], GROUPS);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_empty[s], 1);
         }
-        for (int g = 0; g < GROUPS; g++) {
-            for (int b = 0; b < 2; b++) {
-                mbar_init(&s_full[g][b], 1);
-                mbar_init(&p_full[g][b], 4);
-                mbar_init(&o_done[g][b], 1);
-            }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&s_full[b], 1);
+            mbar_init(&p_full[b], 4);
+            mbar_init(&o_done[b], 1);
         }
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        mbar_expect_tx(&q_full, GROUPS * Q_BYTES);
+        mbar_expect_tx(&q_full, Q_BYTES);
 #pragma unroll
-        for (int g = 0; g < GROUPS; g++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) tma_load_3d(Qs + g * Q_BYTES + h * QPANEL, &map_q, h * 64, kvh * G, q_start + q0 + g * TOKG, &q_full);
+        for (int h = 0; h < 2; h++) tma_load_3d(Qs + h * QPANEL, &map_q, h * 64, kvh * G, q_start + q0, &q_full);
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(s32(&tmem_base_s)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(s32(&tmem_base_s)), "n"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     // The tile's pages in ascending order, and who lists them: a bitmap of the sequence's pages, the number of pages ahead of
@@ -229,11 +270,26 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
         int* ahead = reinterpret_cast<int*>(map + MAX_TABLE / 32);
         const int words = (p.bt_stride + 31) / 32;
         const int* lists = p.list + ((int64_t)(q_start + q0) * p.kv_heads + kvh) * p.top;
+        constexpr int KEPT = 8;        // entries of the lists a thread keeps, all asked for at once; longer lists are read twice
+        const bool kept = tokens * p.top <= KEPT * THREADS;
+        auto place = [&](int i) -> int {      // token and page of entry i of the tile's lists, -1 for one that names nothing
+            const int tok = i / p.top;
+            const int lp = lists[(int64_t)tok * p.kv_heads * p.top + (i - tok * p.top)];
+            return lp >= 0 && lp <= (past + q0 + tok) / BKV && lp < p.bt_stride ? tok << 16 | lp : -1;
+        };
+        int mine[KEPT];
+#pragma unroll
+        for (int e = 0; e < KEPT; e++) mine[e] = kept && (int)threadIdx.x + e * THREADS < tokens * p.top ? place(threadIdx.x + e * THREADS) : -1;
         auto each = [&](auto use) {
-            for (int i = threadIdx.x; i < tokens * p.top; i += THREADS) {
-                const int tok = i / p.top;
-                const int lp = lists[(int64_t)tok * p.kv_heads * p.top + (i - tok * p.top)];
-                if (lp >= 0 && lp <= (past + q0 + tok) / BKV && lp < p.bt_stride) use(tok, lp);
+            if (kept) {
+#pragma unroll
+                for (int e = 0; e < KEPT; e++)
+                    if (mine[e] >= 0) use(mine[e] >> 16, mine[e] & 0xffff);
+            } else {
+                for (int i = threadIdx.x; i < tokens * p.top; i += THREADS) {
+                    const int v = place(i);
+                    if (v >= 0) use(v >> 16, v & 0xffff);
+                }
             }
         };
         for (int i = threadIdx.x; i < words; i += THREADS) map[i] = 0;
@@ -268,21 +324,6 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
             const int at = ahead[lp >> 5] + __popc(map[lp >> 5] & ((1u << (lp & 31)) - 1u));
             atomicOr(&bits[at * MW + (tok >> 5)], 1u << (tok & 31));
         });
-        __syncthreads();
-        for (int i = threadIdx.x; i < n_s; i += THREADS) {
-            uint32_t a = 0, b = 0;
-            for (int w = 0; w < MW; w++) {
-                const uint32_t m = bits[i * MW + w];
-                if (MW > 1) {
-                    if (w < MW / 2) a |= m; else b |= m;
-                } else {
-                    const uint32_t low = (1u << TOKG) - 1u;    // a tile of at most 32 tokens: TOKG is at most 16
-                    a |= m & low;
-                    b |= m & ~low;
-                }
-            }
-            entry[i] |= (a ? 1 << 30 : 0) | (b ? (int)0x80000000u : 0);
-        }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -292,7 +333,6 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
     const int lo = (int)((int64_t)n_s * piece / pieces), n = (int)((int64_t)n_s * (piece + 1) / pieces) - lo;
     entry += lo;
     bits += lo * MW;
-    auto lists_it = [&](int j, int g) { return g ? entry[j] < 0 : (entry[j] & (1 << 30)) != 0; };
 
     if (warp == 0 || warp == VALUE_LOADER_WARP) {
         if (lane == 0) {
@@ -308,7 +348,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
                 if (*(volatile int*)&abort_s) break;
                 mbar_expect_tx(&full[s], K_BYTES);
                 unsigned char* to = KVs + (size_t)s * STAGE_BYTES + (keys ? 0 : K_BYTES);
-                const int row = ((int)page_of(bt, (entry[j] & 0x3fffffff) * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * BKV;
+                const int row = ((int)page_of(bt, entry[j] * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * BKV;
 #pragma unroll
                 for (int h = 0; h < 2; h++) tma_load_2d(to + h * KPANEL, keys ? &map_k : &map_v, h * 64, row, &full[s]);
                 issued = j + 1;
@@ -320,53 +360,41 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
         }
     } else if (warp < FIRST_SOFTMAX_WARP) {
         if (lane == 0) {
-            const int g = (warp - 1) % GROUPS;
-            const bool scores_role = warp - 1 < GROUPS;
             bool ok = true;
-            int i = 0;        // pages of the group so far
-            if (scores_role) {
-                const uint32_t idesc = instr_desc(BQ, BKV);
+            if (warp == 1) {
+                const uint32_t idesc = instr_desc(ROWS, BKV);
                 ok = mbar_wait(&q_full, 0);
-                const uint64_t q_desc = smem_desc(s32(Qs + g * Q_BYTES)), k_desc = smem_desc(s32(KVs));
+                const uint64_t q_desc = smem_desc(s32(Qs)), k_desc = smem_desc(s32(KVs));
                 for (int j = 0; j < n && ok; j++) {
-                    ok = mbar_wait_relaxed(&k_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
-                    if (ok && lists_it(j, g)) {
-                        const int b = i & 1;
-                        // the probabilities of the page before last lie in this buffer's columns until their product has read them
-                        if (i >= 2) ok = mbar_wait_relaxed(&o_done[g][b], (uint32_t)((i - 2) >> 1) & 1u);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                        const uint64_t kd = k_desc + (uint64_t)((j % STAGES) * (STAGE_BYTES >> 4));
-                        const uint32_t d_tmem = tmem_base + (uint32_t)(g * 128 + b * 64);
+                    const int b = j & 1;
+                    ok = mbar_wait(&k_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+                    // the probabilities of the page before last lie in this buffer's columns until their product has read them
+                    if (ok && j >= 2) ok = mbar_wait(&o_done[b], (uint32_t)((j - 2) >> 1) & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    const uint64_t kd = k_desc + (uint64_t)((j % STAGES) * (STAGE_BYTES >> 4));
 #pragma unroll
-                        for (int ks = 0; ks < 8; ks++)
-                            umma(d_tmem, q_desc + (uint64_t)((ks >> 2) * (QPANEL >> 4) + (ks & 3) * 2),
-                                 kd + (uint64_t)((ks >> 2) * (KPANEL >> 4) + (ks & 3) * 2), idesc, ks > 0 ? 1u : 0u);
-                        umma_commit(&s_full[g][b]);
-                        i++;
-                    }
-                    if (ok) umma_commit(&k_empty[j % STAGES]);
+                    for (int ks = 0; ks < 8; ks++)
+                        umma(tmem_base + (uint32_t)(b * 64), q_desc + (uint64_t)((ks >> 2) * (QPANEL >> 4) + (ks & 3) * 2),
+                             kd + (uint64_t)((ks >> 2) * (KPANEL >> 4) + (ks & 3) * 2), idesc, ks > 0 ? 1u : 0u);
+                    umma_commit(&s_full[b]);
+                    umma_commit(&k_empty[j % STAGES]);
                 }
             } else {
-                const uint32_t idesc = instr_desc(BQ, HD) | (1u << 16);  // values enter MN-major
+                const uint32_t idesc = instr_desc(ROWS, HD) | (1u << 16);  // values enter MN-major
                 const uint64_t v_desc = smem_desc_mn(s32(KVs + K_BYTES));
                 for (int j = 0; j < n && ok; j++) {
-                    ok = mbar_wait_relaxed(&v_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
-                    if (ok && lists_it(j, g)) {
-                        const int b = i & 1;
-                        ok = mbar_wait(&p_full[g][b], (uint32_t)(i >> 1) & 1u);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                        const uint64_t vd = v_desc + (uint64_t)((j % STAGES) * (STAGE_BYTES >> 4));
-                        const uint32_t d_tmem = tmem_base + (uint32_t)(256 + g * 128);
+                    const int b = j & 1;
+                    ok = mbar_wait(&v_full[j % STAGES], (uint32_t)(j / STAGES) & 1u) && mbar_wait(&p_full[b], (uint32_t)(j >> 1) & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    const uint64_t vd = v_desc + (uint64_t)((j % STAGES) * (STAGE_BYTES >> 4));
 #pragma unroll
-                        for (int kk = 0; kk < BKV / 16; kk++)
-                            umma_ta(d_tmem, tmem_base + (uint32_t)(g * 128 + b * 64 + kk * 8), vd + (uint64_t)(kk * ((16 * 128) >> 4)), idesc,
-                                    (i > 0 || kk > 0) ? 1u : 0u);
-                        umma_commit(&o_done[g][b]);
-                        i++;
-                    }
-                    if (ok) umma_commit(&v_empty[j % STAGES]);
+                    for (int kk = 0; kk < BKV / 16; kk++)
+                        umma_ta(tmem_base + O_COL, tmem_base + (uint32_t)(b * 64 + kk * 8), vd + (uint64_t)(kk * ((16 * 128) >> 4)), idesc,
+                                (j > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit(&o_done[b]);
+                    umma_commit(&v_empty[j % STAGES]);
                 }
             }
             if (!ok) {
@@ -375,31 +403,28 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
             }
         }
     }
-    const int g = warp >= FIRST_SOFTMAX_WARP && warp < VALUE_LOADER_WARP ? (warp - FIRST_SOFTMAX_WARP) >> 2 : -1;   // a softmax warp's group
-    const int quad = warp & 3, r = quad * 32 + lane;          // row within the group
-    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    const uint32_t o_addr = tmem_base + lane_addr + (uint32_t)(256 + (g > 0 ? g : 0) * 128);
-    const int tok = (g > 0 ? g : 0) * TOKG + r / GP, h = r % GP;
-    const bool row_ok = g >= 0 && tok < tokens && h < G;
+    const bool softmax = warp >= FIRST_SOFTMAX_WARP && warp < VALUE_LOADER_WARP;
+    const int r = (warp & 3) * 32 + lane, tok = r / GP, h = r % GP;       // a softmax thread's row: the warp's quarter of tensor memory
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16, o_addr = tmem_base + lane_addr + O_COL;
+    const bool row_ok = softmax && tok < tokens && h < G;
     float m_used = -INFINITY, l = 0.f;
-    int i = 0;             // pages of the group so far
-    if (g >= 0) {
+    if (softmax) {
         const int pos = past + q0 + tok;
         const float sc = p.scale * LOG2E;    // > 0
         float m_run = -INFINITY;
         bool ok = true;
         for (int j = 0; j < n && ok; j++) {
-            if (!lists_it(j, g)) continue;
-            const int b = i & 1, key0 = (entry[j] & 0x3fffffff) * BKV;
+            const int b = j & 1, key0 = entry[j] * BKV;
             const bool mine = (bits[j * MW + (tok >> 5)] >> (tok & 31)) & 1u;
             const bool any = __any_sync(0xffffffffu, mine);
-            if (!mbar_wait(&s_full[g][b], (uint32_t)(i >> 1) & 1u)) {
+            if (!mbar_wait(&s_full[b], (uint32_t)(j >> 1) & 1u)) {
                 ok = false;
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)(g * 128 + b * 64);
+            const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)(b * 64);
             uint32_t pw[32];
+            uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
             if (!any) {
                 // scores of this buffer were issued behind the product of two pages ago: it may be written
 #pragma unroll
@@ -410,7 +435,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
                 tmem_ld32_nowait(s_addr, v0);
                 tmem_ld32_nowait(s_addr + 32u, v1);
                 tmem_wait_ld();
-                if (key0 + BKV - 1 > pos) {
+                if (mine && key0 + BKV - 1 > pos) {      // (0 times -inf, where the row does not list the page, would be NaN)
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         if (key0 + e > pos) v0[e] = 0xff800000u;  // -inf
@@ -425,13 +450,13 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
                 const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
                 if (mine) m_run = fmaxf(m_run, tile_max);
                 const bool grow = m_run > m_used + RESCALE_AT || (m_used == -INFINITY && m_run != -INFINITY);
-                if (__any_sync(0xffffffffu, grow && i > 0)) {
-                    // O_g may only be touched between products: wait for the previous page's
-                    if (!mbar_wait(&o_done[g][(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) {
+                if (__any_sync(0xffffffffu, grow && j > 0)) {
+                    // O may only be touched between products: wait for the previous page's
+                    if (!mbar_wait(&o_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u)) {
                         ok = false;
                         break;
                     }
-                    const float f = (grow && i > 0) ? fast_exp2(m_used - m_run) : 1.f;  // m_used = -inf gives 0: O is all zeros then
+                    const float f = (grow && j > 0) ? fast_exp2(m_used - m_run) : 1.f;  // m_used = -inf gives 0: O is all zeros then
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
                     for (int c0 = 0; c0 < HD; c0 += 32) {
@@ -445,24 +470,36 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
                 }
                 if (grow) m_used = m_run;
                 const float mbase = m_used == -INFINITY ? 0.f : m_used;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                // a row that does not list the page: 2^-inf, which is 0 (2^-126 where the polynomial has it, of which its sum takes
+                // nothing); a NaN score makes its sums NaN, and they are made anew
+                const uint64_t sc2 = mine ? pack2(sc, sc) : pack2(0.f, 0.f), nmb2 = mine ? pack2(-mbase, -mbase) : pack2(-INFINITY, -INFINITY);
 #pragma unroll
                 for (int c = 0; c < 32; c++) {
                     const uint32_t a = c < 16 ? v0[(c & 15) * 2] : v1[(c & 15) * 2], bb = c < 16 ? v0[(c & 15) * 2 + 1] : v1[(c & 15) * 2 + 1];
-                    const float p0 = fast_exp2(fmaf(__uint_as_float(a), sc, -mbase)), p1 = fast_exp2(fmaf(__uint_as_float(bb), sc, -mbase));
-                    sum[c & 3] += p0 + p1;
+                    const uint64_t t = fma2(pack2(__uint_as_float(a), __uint_as_float(bb)), sc2, nmb2);
+                    float p0, p1;
+                    if (c % 4 == 3) {
+                        exp2_poly_x2(t, p0, p1);
+                    } else {
+                        unpack2(t, p0, p1);
+                        p0 = fast_exp2(p0);
+                        p1 = fast_exp2(p1);
+                    }
+                    sum2[c & 1] = add2(sum2[c & 1], pack2(p0, p1));
                     const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
-                    pw[c] = mine ? *reinterpret_cast<const uint32_t*>(&h2) : 0u;
+                    pw[c] = *reinterpret_cast<const uint32_t*>(&h2);
                 }
                 tmem_st32(s_addr, pw);
-                if (mine) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[g][b]);
-            i++;
+            if (lane == 0) mbar_arrive(&p_full[b]);
+            float sum[4];
+            unpack2(sum2[0], sum[0], sum[1]);
+            unpack2(sum2[1], sum[2], sum[3]);
+            if (mine) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
-        if (ok && i > 0 && !mbar_wait(&o_done[g][(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) ok = false;
+        if (ok && n > 0 && !mbar_wait(&o_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u)) ok = false;
         if (!ok) {
             atomicCAS(&g_status, 0, 4);
             abort_s = 1;
@@ -472,14 +509,14 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
     __syncthreads();      // every role is done with the pages
     const bool aborted = *(volatile int*)&abort_s != 0;
     if (pieces == 1) {
-        if (g >= 0 && !aborted) {
+        if (softmax && !aborted) {
             const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;       // nothing seen: zeros; a NaN stays one
             bf16* op = (bf16*)p.out + (int64_t)(q_start + q0 + tok) * p.out_row_stride + (int64_t)(kvh * G + h) * HD;
             uint32_t most = 0;     // of the sums' exponents
 #pragma unroll 1
             for (int c0 = 0; c0 < HD; c0 += 32) {
                 uint32_t o[32];
-                if (i > 0) {
+                if (n > 0) {
                     tmem_ld32(o_addr + (uint32_t)c0, o);
                 } else {
 #pragma unroll
@@ -501,7 +538,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
                 }
             }
             for (unsigned again = __ballot_sync(0xffffffffu, row_ok && most >= 0x7f800000u); again; again &= again - 1) {
-                const int rr = quad * 32 + __ffs(again) - 1, tk = g * TOKG + rr / GP;
+                const int rr = (warp & 3) * 32 + __ffs(again) - 1, tk = rr / GP;
                 row_alone(p, bt, q_start + q0 + tk, past + q0 + tk, kvh * G + rr % GP, kvh, lane);
             }
         }
@@ -509,11 +546,11 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
         // A row's 32 chunks of four channels stand in an order of their own (the chunk's number xor the row's), so that the
         // threads of a warp, a row each, write to different banks.
         float* sums = reinterpret_cast<float*>(KVs);
-        if (g >= 0) {
-            const int at = g * BQ + r;
+        if (softmax) {
+            const int at = r;
             row_m[at] = m_used;
             row_l[at] = l;
-            if (i > 0) {
+            if (n > 0) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD; c0 += 32) {
                     uint32_t o[32];
@@ -526,31 +563,34 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
             }
         }
         cluster.sync();
-        bool gone = false;
-        for (int w = 0; w < pieces; w++) gone |= *cluster.map_shared_rank(&abort_s, w) != 0;
-        for (int at = piece + warp * pieces; at < ROWS && !gone; at += WARPS * pieces) {
-            const int tk = (at / BQ) * TOKG + (at % BQ) / GP, hh = (at % BQ) % GP;
+        // (A CTA that gave up has left a status and whatever its rows held: the results are not valid, but they are written.)
+        for (int at = piece + warp * pieces; at < ROWS; at += WARPS * pieces) {
+            const int tk = at / GP, hh = at % GP;
             if (tk >= tokens || hh >= G) continue;
-            float m[MAX_PIECES], M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < MAX_PIECES; w++) {
-                if (w >= pieces) break;
-                m[w] = *cluster.map_shared_rank(&row_m[at], w);
-                M = fmaxf(M, m[w]);
+            // a lane a piece: its maximum and sum; all pieces' values are asked for before the first is used
+            float m = -INFINITY, l_w = 0.f;
+            if (lane < pieces) {
+                m = *cluster.map_shared_rank(&row_m[at], lane);
+                l_w = *cluster.map_shared_rank(&row_l[at], lane);
             }
-            float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+            float4 x[MAX_PIECES];
+#pragma unroll
+            for (int w = 0; w < MAX_PIECES; w++)
+                if (w < pieces) x[w] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums, w) + (size_t)at * HD + (lane ^ (at & 31)) * 4);
+            const float M = warp_max(m);
+            // this row saw nothing there: neither a maximum nor a sum (a NaN score leaves no maximum but a NaN sum)
+            const bool none = m == -INFINITY && l_w == 0.f;
+            const float f_w = none ? 0.f : m == -INFINITY ? 1.f : fast_exp2(m - M);
+            const float L = warp_sum(none ? 0.f : f_w * l_w);
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < MAX_PIECES; w++) {
-                if (w >= pieces) break;
-                const float lw = *cluster.map_shared_rank(&row_l[at], w);
-                if (m[w] == -INFINITY && lw == 0.f) continue;      // this row saw nothing there (a NaN score leaves a NaN sum)
-                const float f = m[w] == -INFINITY ? 1.f : fast_exp2(m[w] - M);
-                const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums, w) + (size_t)at * HD + (lane ^ (at & 31)) * 4);
-                L += f * lw;
-                o[0] += f * x.x;
-                o[1] += f * x.y;
-                o[2] += f * x.z;
-                o[3] += f * x.w;
+                const float f = __shfl_sync(0xffffffffu, f_w, w);
+                if (w >= pieces || __shfl_sync(0xffffffffu, (int)none, w)) continue;      // its sums may be anything
+                o[0] += f * x[w].x;
+                o[1] += f * x[w].y;
+                o[2] += f * x[w].z;
+                o[3] += f * x[w].w;
             }
             if (__any_sync(0xffffffffu, !(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < INFINITY))) {
                 row_alone(p, bt, q_start + q0 + tk, past + q0 + tk, kvh * G + hh, kvh, lane);
@@ -567,7 +607,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_tc5_kernel(const __grid_co
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
     }
 }
 
@@ -582,10 +622,10 @@ int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dim
 }
 
 int list_bytes(const PagesParams& p) {
-    const int gp = padded_group(p.heads / p.kv_heads);
-    const int64_t most = (int64_t)tile_tokens(gp) * p.top;
+    const int tokens = ROWS / padded_group(p.heads / p.kv_heads);
+    const int64_t most = (int64_t)tokens * p.top;
     const int cap = (int)(most < p.bt_stride ? most : p.bt_stride);
-    return cap * 4 * (1 + mask_words(gp));
+    return cap * 4 * (1 + mask_words(tokens));
 }
 
 }  // namespace
@@ -593,23 +633,24 @@ int list_bytes(const PagesParams& p) {
 // Whether this kernel takes the call: heads of 128 in groups of up to 128, 16-byte aligned rows, a positive scale, and a tile's
 // pages (those its tokens can list together) within the shared memory there is for them.
 int gb_attention_pages_tc5_accepts(const PagesParams& p) {
-    return p.d == HD && p.heads / p.kv_heads <= BQ && p.scale > 0.f && !((uintptr_t)p.q & 15) && !(p.q_row_stride & 7) && !((uintptr_t)p.out & 15) &&
+    return p.d == HD && p.heads / p.kv_heads <= ROWS && p.scale > 0.f && !((uintptr_t)p.q & 15) && !(p.q_row_stride & 7) && !((uintptr_t)p.out & 15) &&
            !(p.out_row_stride & 7) && p.rows > 0 && p.bt_stride <= MAX_TABLE && (int64_t)p.pages * p.kv_heads * BKV <= 0x7fffffff &&
            list_bytes(p) <= LIST_BYTES;
 }
 
-int gb_attention_pages_tc5(const PagesParams& p, int pieces, cudaStream_t stream) {
+int gb_attention_pages_tc5(const PagesParams& p, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_pages_tc5_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_BYTES + 1024 + LIST_BYTES);
-        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", TILE_BYTES + LIST_BYTES, cudaGetErrorString(e));
+        const int most = TILE_BYTES + 1024 + LIST_BYTES;
+        const cudaError_t e = cudaFuncSetAttribute(attn_pages_tc5_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", most, cudaGetErrorString(e));
         configured = true;
     }
-    const int G = p.heads / p.kv_heads, gp = padded_group(G), tok = tile_tokens(gp);
+    const int G = p.heads / p.kv_heads, gp = padded_group(G), tok = ROWS / gp;
     CUtensorMap map_q, map_k, map_v;
     {
         const cuuint64_t dims[3] = {HD, (cuuint64_t)p.heads, (cuuint64_t)p.rows}, strides[2] = {HD * 2, (cuuint64_t)p.q_row_stride * 2};
-        const cuuint32_t box[3] = {64, (cuuint32_t)gp, (cuuint32_t)(tok / GROUPS)};
+        const cuuint32_t box[3] = {64, (cuuint32_t)gp, (cuuint32_t)tok};
         if (int rc = make_map(&map_q, p.q, 3, dims, strides, box)) return rc;
     }
     {
@@ -618,9 +659,14 @@ int gb_attention_pages_tc5(const PagesParams& p, int pieces, cudaStream_t stream
         if (int rc = make_map(&map_k, p.k_plane, 2, dims, strides, box)) return rc;
         if (int rc = make_map(&map_v, p.v_plane, 2, dims, strides, box)) return rc;
     }
+    // As many CTAs to a tile as run at once, two an SM (24 tiles of 90 rows behind 20000, us: 106 in one piece, 64 in two, 37 in four, 35 in
+    // six, 31 in eight).
+    const int64_t tiles = (int64_t)p.nseq * ceil_div(p.max_q_len, tok) * p.kv_heads;
+    int pieces = (int)(2 * gb_sm_count() / tiles);
+    pieces = pieces < 1 ? 1 : pieces > MAX_PIECES ? MAX_PIECES : pieces;
     const dim3 grid(ceil_div(p.max_q_len, tok) * pieces, p.kv_heads, p.nseq);
     if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("attention_pages: grid (%u, %u, %u) exceeds one launch", grid.x, grid.y, grid.z);
-    cudaError_t e = launch_pdl_cluster(attn_pages_tc5_kernel, grid, dim3(THREADS), (size_t)(TILE_BYTES + 1024 + list_bytes(p)), stream, pieces, 1, map_q, map_k, map_v, p);
+    const cudaError_t e = launch_pdl_cluster(attn_pages_tc5_kernel, grid, dim3(THREADS), (size_t)(TILE_BYTES + 1024 + list_bytes(p)), stream, pieces, 1, map_q, map_k, map_v, p);
     if (e != cudaSuccess) GB_REFUSE("attention_pages: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }
