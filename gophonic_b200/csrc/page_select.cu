@@ -218,9 +218,13 @@ struct Coef64 {
 // scores where it takes a tenth.
 template <int W, int BAND, int FEW, int MORE>
 struct Chooser {
-    double band_s[BAND];
-    int band_i[BAND];        // pages near the border, kept with their 64-bit scores
-    int hist[256];
+    union {
+        struct {
+            double band_s[BAND];
+            int band_i[BAND];          // pages near the border, kept with their 64-bit scores
+        };
+        alignas(8) int hist[256];      // of the slow way; and what the fast one packs, before it has a border
+    };
     int warp_a[W], warp_b[W];
     int digit, rest;
 
@@ -274,37 +278,23 @@ struct Chooser {
         }
     }
 
-    // false: too many pages near the border
-    template <typename T, int R>
-    __device__ __forceinline__ bool fast(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, int warp, int lane) {
-        const int nc = r.nc, k = r.k;
-        const int steps = R > 0 ? R : (nc + 32 * W - 1) / (32 * W), from = warp * steps * 32 + lane;
-        uint32_t reg[R > 0 ? R : 1];
-        if constexpr (R > 0) {
-#pragma unroll
-            for (int j = 0; j < R; j++) reg[j] = from + j * 32 < nc ? key[from + j * 32] : 0u;     // no finite score's key is 0
-        }
-        auto at = [&](int j) -> uint32_t {
-            if constexpr (R > 0) return reg[j];
-            return from + j * 32 < nc ? key[from + j * 32] : 0u;
-        };
+    // The choice among scores at(j) of candidates id(j), `steps` a lane (N of them if N > 0: registers), in the candidates' order lane by
+    // lane and step by step; scores of 0 are none.  `lo` and `hi`: as many as k or more keys from lo on, fewer from hi on.  false: too
+    // many pages near the border.
+    template <typename T, int N, class At, class Id>
+    __device__ __forceinline__ bool choose(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, int steps, At at, Id id, uint32_t lo, uint32_t hi,
+                                           int warp, int lane) {
+        const int k = r.k;
         auto each = [&](auto use) {
-            if constexpr (R > 0) {
+            if constexpr (N > 0) {
 #pragma unroll
-                for (int j = 0; j < R; j++) use(j, at(j));
+                for (int j = 0; j < N; j++) use(j, at(j));
             } else {
                 for (int j = 0; j < steps; j++) use(j, at(j));
             }
         };
-        // tau, the k-th highest float32 score: the keys from `lo` on are k or more, those from `hi` on fewer; halved until a border
-        // parts exactly k of them (a dozen steps for some hundred scores), or one value is left
-        uint32_t lo = 0xffffffffu, most = 0u;
-        each([&](int, uint32_t v) {
-            if (v) lo = min(lo, v);
-            most = max(most, v);
-        });
-        lo = least(lo, warp_a, warp, lane);
-        uint32_t hi = ~least(~most, warp_b, warp, lane) + 1u;
+        // tau, the k-th highest float32 score: [lo, hi) is halved until a border parts exactly k keys (some ten steps), or one value is
+        // left
         for (bool odd = false; hi - lo > 1u; odd = !odd) {
             const uint32_t mid = lo + (hi - lo) / 2u;
             int c = 0;
@@ -320,8 +310,7 @@ struct Chooser {
         sync();
         border = least(border, warp_a, warp, lane);
         const float tau = of_key(border);
-        const float upper = tau + 2.f * err + fabsf(tau) * 2.4e-7f, lower = tau - 2.f * err - fabsf(tau) * 2.4e-7f;
-        const uint32_t sure_from = order_key(upper) + 1u, near_from = order_key(lower == 0.f ? -0.f : lower);
+        const uint32_t sure_from = order_key(tau + 2.f * err + fabsf(tau) * 2.4e-7f) + 1u, near_from = lowest_near(border, err);
         int sure = 0, near = 0;
         each([&](int, uint32_t v) {
             sure += v >= sure_from;
@@ -338,7 +327,7 @@ struct Chooser {
             sync();
             if (__any_sync(0xffffffffu, near_mine > 0))
                 each([&](int j, uint32_t v) {
-                    if (v >= near_from && v < sure_from) band_i[atomicAdd(&rest, 1)] = from + j * 32;
+                    if (v >= near_from && v < sure_from) band_i[atomicAdd(&rest, 1)] = id(j);
                 });
             sync();
             Coef64 c;
@@ -356,7 +345,7 @@ struct Chooser {
             sync();
         }
         auto taken = [&](int j, uint32_t v) -> bool {
-            if (settle && v >= near_from && v < sure_from) v = key[from + j * 32];
+            if (settle && v >= near_from && v < sure_from) v = key[id(j)];
             return v >= (settle ? sure_from : near_from);
         };
         int before = 0;
@@ -372,10 +361,83 @@ struct Chooser {
         each([&](int j, uint32_t v) {
             const bool yes = taken(j, v);
             const unsigned who = __ballot_sync(0xffffffffu, yes);
-            if (yes) list[before + __popc(who & ((1u << lane) - 1u))] = r.c0 + from + j * 32;
+            if (yes) list[before + __popc(who & ((1u << lane) - 1u))] = r.c0 + id(j);
             before += __popc(who);
         });
         return true;
+    }
+
+    // The least key that a score can have and still be within 2 err of that of `border`, or above it.
+    static __device__ __forceinline__ uint32_t lowest_near(uint32_t border, float err) {
+        const float v = of_key(border), lower = v - 2.f * err - fabsf(v) * 2.4e-7f;
+        return order_key(lower == 0.f ? -0.f : lower);
+    }
+
+    template <typename T, int R>
+    __device__ __forceinline__ bool fast(const PagesParams& p, const Row<T>& r, uint32_t* key, float err, int warp, int lane) {
+        const int nc = r.nc, k = r.k;
+        const int steps = R > 0 ? R : (nc + 32 * W - 1) / (32 * W), from = warp * steps * 32 + lane;
+        auto id = [&](int j) { return from + j * 32; };
+        if constexpr (R > 0) {
+            uint32_t reg[R];
+#pragma unroll
+            for (int j = 0; j < R; j++) reg[j] = from + j * 32 < nc ? key[from + j * 32] : 0u;     // no finite score's key is 0
+            if (W == 1 && k <= 32) {
+                // One warp, and no more wanted than lanes there are: of the lanes' highest scores the k-th is no higher than tau, and only
+                // some dozens of all are as high or near it.  They are packed and the rest forgotten.  (2000 rows 100 -> 88 us.  With
+                // half lanes for up to 64 wanted too many are left: 50 sequences that want 61 took 31 us instead of 26.)
+                uint32_t a = 0;
+#pragma unroll
+                for (int j = 0; j < R; j++) a = max(a, reg[j]);
+                uint32_t lo = max(1u, __reduce_min_sync(0xffffffffu, a));
+                const uint32_t end = __reduce_max_sync(0xffffffffu, a) + 1u;
+                for (uint32_t hi = end; hi - lo > 1u;) {
+                    const uint32_t mid = lo + (hi - lo) / 2u;
+                    const int c = __popc(__ballot_sync(0xffffffffu, a >= mid));
+                    if (c >= k) lo = mid; else hi = mid;
+                    if (c == k) break;
+                }
+                const uint32_t cut = lowest_near(lo, err);
+                uint2* packed = reinterpret_cast<uint2*>(hist);
+                constexpr int MOST = sizeof(hist) / sizeof(uint2), N = MOST / 32;
+                int m = 0;
+#pragma unroll
+                for (int j = 0; j < R; j++) {
+                    const bool in = reg[j] >= cut && reg[j] != 0u;
+                    const unsigned who = __ballot_sync(0xffffffffu, in);
+                    const int to = m + __popc(who & ((1u << lane) - 1u));
+                    if (in && to < MOST) packed[to] = make_uint2(reg[j], id(j));
+                    m += __popc(who);
+                }
+                __syncwarp();
+                if (m <= MOST) {
+                    uint2 few[N];
+#pragma unroll
+                    for (int j = 0; j < N; j++) few[j] = j * 32 + lane < m ? packed[j * 32 + lane] : make_uint2(0u, 0u);
+                    return choose<T, N>(p, r, key, err, N, [&](int j) { return few[j].x; }, [&](int j) { return (int)few[j].y; }, lo, end, warp, lane);
+                }
+            }
+            uint32_t lo = 0xffffffffu, most = 0u;
+#pragma unroll
+            for (int j = 0; j < R; j++) {
+                if (reg[j]) lo = min(lo, reg[j]);
+                most = max(most, reg[j]);
+            }
+            lo = least(lo, warp_a, warp, lane);
+            const uint32_t hi = ~least(~most, warp_b, warp, lane) + 1u;
+            return choose<T, R>(p, r, key, err, R, [&](int j) { return reg[j]; }, id, lo, hi, warp, lane);
+        } else {
+            auto at = [&](int j) -> uint32_t { return from + j * 32 < nc ? key[from + j * 32] : 0u; };
+            uint32_t lo = 0xffffffffu, most = 0u;
+            for (int j = 0; j < steps; j++) {
+                const uint32_t v = at(j);
+                if (v) lo = min(lo, v);
+                most = max(most, v);
+            }
+            lo = least(lo, warp_a, warp, lane);
+            const uint32_t hi = ~least(~most, warp_b, warp, lane) + 1u;
+            return choose<T, 0>(p, r, key, err, steps, at, id, lo, hi, warp, lane);
+        }
     }
 
     // Scores beyond float32, or hundreds that tie: the k-th highest of the 64-bit scores, which are summed anew for every digit.
@@ -476,7 +538,7 @@ __device__ __forceinline__ float sum_many(float (&v)[N], int lane) {
 }
 
 template <typename T, int LP, int CPL>
-__global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(const __grid_constant__ PagesParams p) {
+__global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __grid_constant__ PagesParams p, int longest_first) {
     constexpr int E = Chunk<T>::E, U = 8 / CPL, PER_WARP = 32 / LP;     // pages a group of LP lanes takes at a time
     extern __shared__ __align__(16) unsigned char raw[];
     SelectSmem& s = *reinterpret_cast<SelectSmem*>(raw);
@@ -486,11 +548,26 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(const __grid
     const int pieces = (int)cluster.num_blocks(), piece = (int)cluster.block_rank();
     pdl_wait();
     pdl_trigger();
-    const int unit = blockIdx.x / pieces, seq = unit / p.max_q_len, qi = unit % p.max_q_len;
+    const int unit = blockIdx.x / pieces / p.kv_heads, head = blockIdx.x / pieces % p.kv_heads, qi = unit % p.max_q_len;
+    int seq = unit / p.max_q_len;
+    if (longest_first) {
+        // more CTAs than run at once: the sequence that is `seq`-th in length, so that none of the long ones begins last
+        int* at = reinterpret_cast<int*>(s.coef);
+        for (int i = tid; i < p.nseq; i += SELECT_THREADS) at[i] = p.seq_kv_len[i];
+        __syncthreads();
+        for (int i = tid; i < p.nseq; i += SELECT_THREADS) {
+            int before = 0;
+            for (int j = 0; j < p.nseq; j++) before += at[j] > at[i] || (at[j] == at[i] && j < i);
+            if (before == seq) s.err[0] = __int_as_float(i);
+        }
+        __syncthreads();
+        seq = __float_as_int(s.err[0]);
+        __syncthreads();
+    }
     const int q_len = p.seq_q_len[seq];
     if (qi >= q_len) return;                    // the whole cluster
     Row<T> r;
-    if (!r.find(p, block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots), p.seq_q_start[seq] + qi, p.seq_kv_len[seq] - q_len + qi, blockIdx.y)) {
+    if (!r.find(p, block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots), p.seq_q_start[seq] + qi, p.seq_kv_len[seq] - q_len + qi, head)) {
         if (piece == 0)
             for (int i = tid; i < p.top; i += SELECT_THREADS) r.list[i] = i < r.n ? i : -1;
         return;
@@ -606,8 +683,9 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_row_kernel(const __grid
 // coefficients, each as the sum of two bfloat16 values (2^-17 relative), against the pages' bounds, which come from the cache
 // straight into the fragments.  The channels of a block of 32 are dealt to the k steps so that a lane's share of a page is 16
 // consecutive bytes; the coefficients are read in the same order.  The scores stand in shared memory, a warp chooses for a row.
-constexpr int TILE_THREADS = 512, TILE_WARPS = TILE_THREADS / 32, TILE_BAND = 48;
+constexpr int TILE_BAND = 48;
 
+template <int TILE_WARPS>
 struct alignas(16) TileSmem {
     Chooser<1, TILE_BAND, 16, 16> choose[TILE_WARPS];
     float size[64];          // per chunk of 8 bounds: their largest size, over all pages
@@ -616,9 +694,10 @@ struct alignas(16) TileSmem {
 __host__ __device__ inline int tile_coef_stride(int d) { return 2 * d + 32; }        // elements: rows 64 bytes of banks apart
 __host__ __device__ inline int tile_key_stride(int pages) { return (pages + 31) / 32 * 32 + 8; }
 
-template <int MT, int KB_MAX>
-__global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(const __grid_constant__ PagesParams p) {
-    constexpr int RT = MT * 16;
+template <int MT, int KB_MAX, int TILE_WARPS>
+__global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_kernel(const __grid_constant__ PagesParams p) {
+    constexpr int RT = MT * 16, TILE_THREADS = TILE_WARPS * 32;
+    using TileSmem = TileSmem<TILE_WARPS>;
     extern __shared__ __align__(16) unsigned char raw[];
     TileSmem& s = *reinterpret_cast<TileSmem*>(raw);
     const int CS = tile_coef_stride(p.d), KS = tile_key_stride(p.bt_stride);
@@ -775,6 +854,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) select_tile_kernel(const __gr
 
 constexpr int MAX_PAGES = 32768;        // of a sequence: their scores stand in shared memory
 constexpr int MAX_TILE_SMEM = 232448;   // what a CTA can have
+constexpr int HALF_TILE_SMEM = 115712;  // what a CTA can have where two share an SM
 constexpr int TILE_MIN_ROWS = 8;        // rows of a sequence from which on they are scored as tiles
 
 int check(const PagesParams& p, int dtype, const char* who) {
@@ -826,29 +906,30 @@ static int launch_rows(const PagesParams& p, cudaStream_t stream) {
     const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads;
     int pieces = 1;
     while (pieces < MAX_PIECES && units * pieces * 2 <= 4 * gb_sm_count() && p.bt_stride > pieces * SELECT_WARPS * 8) pieces *= 2;
-    const int64_t x = (int64_t)p.nseq * p.max_q_len * pieces;
-    if (p.kv_heads > 65535 || x > 0x7fffffff) GB_REFUSE("select_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
-    launch_pdl_cluster(select_row_kernel<T, LP, CPL>, dim3((unsigned)x, p.kv_heads), dim3(SELECT_THREADS), sizeof(SelectSmem) + (size_t)p.bt_stride * sizeof(uint32_t),
-                       stream, pieces, 1, p);
+    if (units * pieces > 0x7fffffff) GB_REFUSE("select_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
+    const int longest_first = pieces == 1 && p.max_q_len == 1 && p.nseq <= 512 && units > gb_sm_count();    // (the lengths stand where the coefficients will)
+    launch_pdl_cluster(select_row_kernel<T, LP, CPL>, dim3((unsigned)(units * pieces)), dim3(SELECT_THREADS), sizeof(SelectSmem) + (size_t)p.bt_stride * sizeof(uint32_t),
+                       stream, pieces, 1, p, longest_first);
     GB_CHECK_LAUNCH("select_pages");
     return 0;
 }
 
+template <int TILE_WARPS>
 static int64_t tile_smem(const PagesParams& p, int rt) {
-    return (int64_t)sizeof(TileSmem) + 2 * rt * tile_coef_stride(p.d) * 2 + (int64_t)rt * tile_key_stride(p.bt_stride) * 4;
+    return (int64_t)sizeof(TileSmem<TILE_WARPS>) + 2 * rt * tile_coef_stride(p.d) * 2 + (int64_t)rt * tile_key_stride(p.bt_stride) * 4;
 }
 
-template <int MT, int KB_MAX>
+template <int MT, int KB_MAX, int TILE_WARPS>
 static int launch_tiles(const PagesParams& p, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(select_tile_kernel<MT, KB_MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_TILE_SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(select_tile_kernel<MT, KB_MAX, TILE_WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_TILE_SMEM);
         if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
         configured = true;
     }
     const dim3 grid(ceil_div(p.max_q_len, MT * 16), p.kv_heads, p.nseq);
     if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("select_pages: %d kv heads, %d sequences exceed one launch", p.kv_heads, p.nseq);
-    launch_pdl(select_tile_kernel<MT, KB_MAX>, grid, dim3(TILE_THREADS), (size_t)tile_smem(p, MT * 16), stream, p);
+    launch_pdl(select_tile_kernel<MT, KB_MAX, TILE_WARPS>, grid, dim3(TILE_WARPS * 32), (size_t)tile_smem<TILE_WARPS>(p, MT * 16), stream, p);
     GB_CHECK_LAUNCH("select_pages");
     return 0;
 }
@@ -861,8 +942,9 @@ GB_API int gb_select_pages(const PagesParams* pp, int dtype, cudaStream_t stream
     if (p.first < 0 || p.last < 1 || p.first + p.last > p.top) GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
     if (p.bt_stride > MAX_PAGES) GB_REFUSE("select_pages: sequences of up to %d pages; this kernel takes %d", p.bt_stride, MAX_PAGES);
     if (dtype == GB_BF16 && p.max_q_len >= TILE_MIN_ROWS && p.d % 16 == 0) {
-        if (p.max_q_len > 16 && tile_smem(p, 32) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<2, 8>(p, stream) : launch_tiles<2, 16>(p, stream);
-        if (tile_smem(p, 16) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<1, 8>(p, stream) : launch_tiles<1, 16>(p, stream);
+        if (p.max_q_len > 16 && p.d <= 128 && tile_smem<8>(p, 32) <= HALF_TILE_SMEM) return launch_tiles<2, 8, 8>(p, stream);
+        if (p.max_q_len > 16 && tile_smem<16>(p, 32) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<2, 8, 16>(p, stream) : launch_tiles<2, 16, 16>(p, stream);
+        if (tile_smem<16>(p, 16) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<1, 8, 16>(p, stream) : launch_tiles<1, 16, 16>(p, stream);
     }
     const int chunks = 2 * p.d / (dtype == GB_F32 ? 4 : 8);
     if (dtype == GB_F32) {

@@ -186,6 +186,19 @@ def test_select_pages_long(ops, dtype, new, pages):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=names)
+@pytest.mark.parametrize("equal", [True, False])
+def test_select_pages_of_many_sequences(ops, dtype, equal):
+    """More single tokens than run at once: the longest begin first, and every one gets its own."""
+    g = torch.Generator().manual_seed(1)
+    seqs = [(640 if equal else int(torch.randint(1, 900, (1,), generator=g)), 1) for _ in range(90)]
+    s = Step(seqs, 4, 2, 16, dtype, seed=5, more_rows=1)
+    bounds = s.bounds_plane()
+    pages = s.select(ops, bounds, 5)
+    check_selection(s, pages, bounds, 5, 1, 2)
+    assert (pages[s.rows:] == -7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=names)
 @pytest.mark.parametrize("kind", ["equal", "few kinds", "zero query", "one ulp", "nan", "inf", "huge", "tiny", "nan query", "inf query", "cancel"])
 @pytest.mark.parametrize("pages,new", [(40, 2), (700, 2), (40, 21), (300, 9)])
 def test_select_pages_near_the_border(ops, dtype, kind, pages, new):
