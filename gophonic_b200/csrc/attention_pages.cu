@@ -7,6 +7,8 @@
 // kernel.  The query heads of the group are the rows of the tiles and share every key and value that is read.
 //   bfloat16: both products on mma.sync, a page of 64 keys at a time, 16 keys a warp, pages asked for three deep by cp.async;
 //   float32:  CUDA cores, half a page a stage, three deep by cp.async.
+// Neither these kernels nor the selection ahead of them let the kernel behind them start early: its CTAs took the SMs that clusters
+// were waiting for (36 layers of one token behind 32768, 64 pages: 5.2 ms a step with early starts, 3.7 without).
 // Scores, the softmax and the sums are float32; with bfloat16 the probabilities are rounded to bfloat16 for the second product, as
 // the values are.
 #include "mma.cuh"
@@ -25,7 +27,7 @@ typedef __nv_bfloat16 bf16;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int THREADS = 128;
 constexpr int MAX_TOP = 1024;     // entries of a list
-constexpr int MAX_PIECES = 8;     // CTAs of a cluster: the portable most
+constexpr int MAX_PIECES = 16;    // CTAs of a cluster (more than eight: where the GPU has room for them all)
 // Rows times key heads from which on runs of rows go to tcgen05 (attention_pages_tc5.cu), us here / there, 32 pages behind 20000: 8
 // key heads, one sequence of 4 rows 11.7 / 14.0, of 8 rows 16.8 / 15.6, of 16 rows 28 / 18; eight sequences of 2 rows 28 / 20; two
 // key heads, one sequence of 16 rows 13 / 18, of 32 rows 18 / 19, of 48 rows 28 / 21.
@@ -127,7 +129,6 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
     __shared__ float ml[16][2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     pdl_wait();
-    pdl_trigger();
     Place at;
     const int G = p.heads / p.kv_heads, GC = G < 16 ? G : 16;
     if (!at.find(p, GC)) return;
@@ -446,12 +447,13 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
 // Into how many pieces a row's list is cut: the CTAs of a cluster.  As many as run at once (one token over eight key heads, 32 pages:
 // 34 us in one piece, 19 in two, 12 in four, 8.4 in eight); where not even two pieces each do, two if their waves end sooner than
 // those of whole rows (50 sequences over eight key heads, 64 pages: 173 us in one piece, 147 in two, 158 in four, 197 in eight).
-int pieces_for(const PagesParams& p, int chunks, int per_sm) {
+int pieces_for(const PagesParams& p, int chunks, int per_sm, int wide) {
     const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads * chunks;
     int pieces = 1;
     const int64_t slots = (int64_t)gb_sm_count() * per_sm;
-    while (pieces < MAX_PIECES && units * pieces * 2 <= slots && p.top >= 4 * pieces) pieces *= 2;
+    while (pieces < 8 && units * pieces * 2 <= slots && p.top >= 4 * pieces) pieces *= 2;
     if (pieces == 1 && p.top >= 8 && units <= 4 * slots && (units * 2 + slots - 1) / slots < 2 * ((units + slots - 1) / slots)) pieces = 2;
+    if (pieces == 8 && units <= wide && p.top >= 32) pieces = 16;
     return pieces;
 }
 
@@ -464,33 +466,50 @@ int launch(K kernel, const PagesParams& p, int chunks, int pieces, int smem, cud
     return 0;
 }
 
+// Shared memory and clusters of 16 for a kernel; how many of those clusters the GPU holds at once (0: none, or not allowed).
+template <typename K>
+int configure(K kernel, int smem, int& wide) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    wide = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(16);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 16;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&wide, kernel, &cfg) != cudaSuccess) wide = 0;
+    }
+    cudaGetLastError();     // what was not possible is no error of the call
+    return 0;
+}
+
 template <int HD>
 int launch_mma(const PagesParams& p, cudaStream_t stream) {
     constexpr int SD = HD + 8;
     constexpr int base = (16 * SD + STAGES * 2 * 64 * SD) * 2;
     static_assert(base >= (128 + 64 * HD) * 4 + 16 * SD * 2, "the warps' results fit where the pages were");
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_pages_mma_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, base + MAX_TOP * 4);
-        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", base + MAX_TOP * 4, cudaGetErrorString(e));
-        configured = true;
-    }
+    static int wide = -1;
+    if (wide < 0)
+        if (int rc = configure(attn_pages_mma_kernel<HD>, base + MAX_TOP * 4, wide)) return rc;
     const int G = p.heads / p.kv_heads, chunks = (G + 15) / 16;
-    return launch(attn_pages_mma_kernel<HD>, p, chunks, pieces_for(p, chunks, HD <= 128 ? 2 : 1), base + p.top * 4, stream);
+    return launch(attn_pages_mma_kernel<HD>, p, chunks, pieces_for(p, chunks, HD <= 128 ? 2 : 1, wide), base + p.top * 4, stream);
 }
 
 template <int NH>
 int launch_f32(const PagesParams& p, cudaStream_t stream) {
-    static bool configured = false;
+    static int wide = -1;
     constexpr int most = f32_floats(256, NH) * 4 + MAX_TOP * 4;
     static_assert(most <= 231000, "the widest heads' stages fit");
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_pages_f32_kernel<NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", most, cudaGetErrorString(e));
-        configured = true;
-    }
+    if (wide < 0)
+        if (int rc = configure(attn_pages_f32_kernel<NH>, most, wide)) return rc;
     const int G = p.heads / p.kv_heads, chunks = (G + NH - 1) / NH;
-    return launch(attn_pages_f32_kernel<NH>, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1), f32_floats(p.d, NH) * 4 + p.top * 4, stream);
+    return launch(attn_pages_f32_kernel<NH>, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1, wide), f32_floats(p.d, NH) * 4 + p.top * 4, stream);
 }
 
 }  // namespace

@@ -547,7 +547,6 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __g
     const cg::cluster_group cluster = cg::this_cluster();
     const int pieces = (int)cluster.num_blocks(), piece = (int)cluster.block_rank();
     pdl_wait();
-    pdl_trigger();
     const int unit = blockIdx.x / pieces / p.kv_heads, head = blockIdx.x / pieces % p.kv_heads, qi = unit % p.max_q_len;
     int seq = unit / p.max_q_len;
     if (longest_first) {
