@@ -188,27 +188,42 @@ struct Coef64 {
                 }
         }
     }
-    // A page's score, the same in every lane; NaN counts as the lowest.  Where no head looks one way there is nothing to add, also
+    // Two pages' scores, the same in every lane; NaN counts as the lowest.  Where no head looks one way there is nothing to add, also
     // where the bound is infinite.
     template <typename T>
-    __device__ __forceinline__ double score(const T* b, int d, int lane) const {
-        T lo[8], hi[8];
+    __device__ __forceinline__ void scores(const T* b0, const T* b1, int d, int lane, double& s0, double& s1) const {
+        T lo[2][8], hi[2][8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int c = lane + 32 * j;
-            lo[j] = c < d ? b[c] : from_f32<T>(0.f);
-            hi[j] = c < d ? b[d + c] : from_f32<T>(0.f);
+            lo[0][j] = c < d ? b0[c] : from_f32<T>(0.f);
+            hi[0][j] = c < d ? b0[d + c] : from_f32<T>(0.f);
+            lo[1][j] = c < d ? b1[c] : from_f32<T>(0.f);
+            hi[1][j] = c < d ? b1[d + c] : from_f32<T>(0.f);
         }
-        double s = 0.0;
+        double s[2] = {0.0, 0.0};
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             if (32 * j >= d) break;
-            if (down[j] != 0.0) s += down[j] * (double)to_f32<T>(lo[j]);
-            if (up[j] != 0.0) s += up[j] * (double)to_f32<T>(hi[j]);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                if (down[j] != 0.0) s[e] += down[j] * (double)to_f32<T>(lo[e][j]);
+                if (up[j] != 0.0) s[e] += up[j] * (double)to_f32<T>(hi[e][j]);
+            }
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        return s == s ? s : -INFINITY;
+        for (int o = 16; o > 0; o >>= 1) {
+            s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+            s[1] += __shfl_xor_sync(0xffffffffu, s[1], o);
+        }
+        s0 = s[0] == s[0] ? s[0] : -INFINITY;
+        s1 = s[1] == s[1] ? s[1] : -INFINITY;
+    }
+    template <typename T>
+    __device__ __forceinline__ double score(const T* b, int d, int lane) const {
+        double s0, s1;
+        scores(b, b, d, lane, s0, s1);
+        return s0;
     }
 };
 
@@ -332,9 +347,13 @@ struct Chooser {
             sync();
             Coef64 c;
             c.load(p, r.q, lane);
-            for (int j = warp; j < m; j += W) {
-                const double v = c.score(r.bounds(p, band_i[j]), p.d, lane);
-                if (lane == 0) band_s[j] = v;
+            for (int j = 2 * warp; j < m; j += 2 * W) {
+                double v0, v1;
+                c.scores(r.bounds(p, band_i[j]), r.bounds(p, band_i[min(j + 1, m - 1)]), p.d, lane, v0, v1);
+                if (lane == 0) {
+                    band_s[j] = v0;
+                    if (j + 1 < m) band_s[j + 1] = v1;
+                }
             }
             sync();
             for (int j = warp * 32 + lane; j < m; j += W * 32) {
@@ -688,6 +707,7 @@ template <int TILE_WARPS>
 struct alignas(16) TileSmem {
     Chooser<1, TILE_BAND, 16, 16> choose[TILE_WARPS];
     float size[64];          // per chunk of 8 bounds: their largest size, over all pages
+    int next;                // the row that the next warp to be done takes: rows whose border is close take twice as long
 };
 
 __host__ __device__ inline int tile_coef_stride(int d) { return 2 * d + 32; }        // elements: rows 64 bytes of banks apart
@@ -756,6 +776,7 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
             }
         }
         for (int i = tid; i < 64; i += TILE_THREADS) s.size[i] = 0.f;
+        if (tid == 0) s.next = TILE_WARPS;
     }
     __syncthreads();
     const int KB = d / 16;             // blocks of 32 bounds
@@ -832,21 +853,27 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
         if (g == 0) atomicMax(reinterpret_cast<int*>(&s.size[kb * 4 + t4]), __float_as_int(v));   // not negative: ordered as integers
     }
     __syncthreads();
-    for (int row = warp; row < rows; row += TILE_WARPS) {
+    for (int row = warp; row < rows; row = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(&s.next, 1) : 0, 0)) {
         Row<bf16> r;
         if (!r.find(p, bt, q_start + q0 + row, past + q0 + row, kvh)) {
             for (int i = lane; i < p.top; i += 32) r.list[i] = i < r.n ? i : -1;
             continue;
         }
-        // The coefficients are good to 2^-18 (3.9e-6) and G half steps of 2^-23, their products' sums on the tensor cores to 6 units of 2^-23
-        // for each of 4 d / 16 steps (16 products and the sum so far, cut off behind 25 bits of the largest of them, and the result).
-        // All relative to the sum of the terms' sizes; what is below the normal range of a coefficient's second part is let in by 1e-35.
-        float most = 0.f;
+        // The coefficients are good to 2^-18 (3.9e-6) and G half steps of 2^-23, relative to the sum of the terms' sizes.  Their products'
+        // sums on the tensor cores: 4 KB steps of 16 products and the sum so far, cut off behind 25 bits of the largest of them, and
+        // the result: 6 units of 2^-23 of what has been summed up to there, so that a block's terms count once for every step
+        // from their own on.  What is below the normal range of a coefficient's second part is let in by 1e-35.
+        float most = 0.f, steps = 0.f;
 #pragma unroll 8
-        for (int c = lane; c < 2 * d; c += 32) most = fmaf(fabsf(__bfloat162float(coef[row * CS + c])) + 1.0e-35f, s.size[c >> 3], most);
+        for (int c = lane; c < 2 * d; c += 32) {
+            const float term = (fabsf(__bfloat162float(coef[row * CS + c])) + 1.0e-35f) * s.size[c >> 3];
+            most += term;
+            steps = fmaf(term, (float)(4 * (KB - (c >> 5))), steps);
+        }
         most = warp_sum(most);
-        const bool unsafe = !(most <= 1.0e38f);
-        const float err = most * (1.02f * (3.9e-6f + (float)d * 1.8e-7f + (float)G * 5.9604645e-8f)) + 1.0e-42f;
+        steps = warp_sum(steps);
+        const bool unsafe = !(most <= 1.0e36f);
+        const float err = 1.02f * (most * (3.9e-6f + (float)G * 5.9604645e-8f) + steps * (6.f * 1.1920929e-7f)) + 1.0e-42f;
         s.choose[warp].run(p, r, keys + row * KS, err, unsafe, lane);
     }
 }
