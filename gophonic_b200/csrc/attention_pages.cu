@@ -27,7 +27,6 @@ typedef __nv_bfloat16 bf16;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int THREADS = 128;
 constexpr int MAX_TOP = 1024;     // entries of a list
-constexpr int MAX_PIECES = 16;    // CTAs of a cluster (more than eight: where the GPU has room for them all)
 // Rows times key heads from which on runs of rows go to tcgen05 (attention_pages_tc5.cu), us here / there, 32 pages behind 20000: 8
 // key heads, one sequence of 4 rows 11.7 / 14.0, of 8 rows 16.8 / 15.6, of 16 rows 28 / 18; eight sequences of 2 rows 28 / 20; two
 // key heads, one sequence of 16 rows 13 / 18, of 32 rows 18 / 19, of 48 rows 28 / 21.
@@ -55,32 +54,38 @@ __device__ __forceinline__ int pack_list(const PagesParams& p, const int* list, 
     return n;
 }
 
-// What the CTAs of a cluster leave for one another: per head of the chunk its maximum, sum and weighted values.
-// Joined by all of them: CTA r of the cluster writes every pieces-th four channels.
-template <typename T>
-__device__ __forceinline__ void join(const PagesParams& p, const float* ml, const float* os, int nh, int hd, T* out) {
+// What the CTAs of a cluster leave for one another: per head of the chunk its maximum, sum and weighted values.  Joined by all of them:
+// CTA r of the cluster writes every PIECES-th four channels.  All pieces' values are asked for before the first is used: one
+// trip through the cluster's shared memory instead of two dozen.
+template <typename T, int PIECES>
+__device__ __forceinline__ void join_pieces(const float* ml, const float* os, int nh, int hd, T* out) {
     cg::cluster_group cluster = cg::this_cluster();
-    const int pieces = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    cluster.sync();
+    const int rank = PIECES == 1 ? 0 : (int)cluster.block_rank();
     const int quads = hd / 4;
-    for (int idx = threadIdx.x * pieces + rank; idx < nh * quads; idx += THREADS * pieces) {
+    for (int idx = threadIdx.x * PIECES + rank; idx < nh * quads; idx += THREADS * PIECES) {
         const int r = idx / quads, c = (idx - r * quads) * 4;
-        float m[MAX_PIECES], M = -INFINITY;
-        for (int w = 0; w < pieces; w++) {
-            m[w] = cluster.map_shared_rank(ml, w)[2 * r];
-            M = fmaxf(M, m[w]);
+        float2 v[PIECES];
+        float4 x[PIECES];
+#pragma unroll
+        for (int w = 0; w < PIECES; w++) {
+            const float* m = PIECES == 1 ? ml : cluster.map_shared_rank(ml, w);
+            const float* o = PIECES == 1 ? os : cluster.map_shared_rank(os, w);
+            v[w] = *reinterpret_cast<const float2*>(m + 2 * r);
+            x[w] = *reinterpret_cast<const float4*>(o + (size_t)r * hd + c);
         }
-        float L = 0.f;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < PIECES; w++) M = fmaxf(M, v[w].x);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         const float base = M == -INFINITY ? 0.f : M;
-        for (int w = 0; w < pieces; w++) {
-            const float e = exp2f(m[w] - base);        // a NaN score leaves no maximum but a NaN sum, which stays one
-            L += e * cluster.map_shared_rank(ml, w)[2 * r + 1];
-            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(os, w) + (size_t)r * hd + c);
-            acc.x += e * x.x;
-            acc.y += e * x.y;
-            acc.z += e * x.z;
-            acc.w += e * x.w;
+#pragma unroll
+        for (int w = 0; w < PIECES; w++) {
+            const float e = exp2f(v[w].x - base);        // a NaN score leaves no maximum but a NaN sum, which stays one
+            L += e * v[w].y;
+            acc.x += e * x[w].x;
+            acc.y += e * x[w].y;
+            acc.z += e * x[w].z;
+            acc.w += e * x[w].w;
         }
         T* op = out + (int64_t)r * hd + c;
         const float inv = L == 0.f ? 0.f : 1.f / L;     // nothing seen: zeros
@@ -88,6 +93,24 @@ __device__ __forceinline__ void join(const PagesParams& p, const float* ml, cons
         op[1] = from_f32<T>(acc.y * inv);
         op[2] = from_f32<T>(acc.z * inv);
         op[3] = from_f32<T>(acc.w * inv);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void join(const float* ml, const float* os, int nh, int hd, T* out) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int pieces = (int)cluster.num_blocks();
+    if (pieces == 1) {
+        __syncthreads();
+        join_pieces<T, 1>(ml, os, nh, hd, out);
+        return;
+    }
+    cluster.sync();
+    switch (pieces) {
+        case 2: join_pieces<T, 2>(ml, os, nh, hd, out); break;
+        case 4: join_pieces<T, 4>(ml, os, nh, hd, out); break;
+        case 8: join_pieces<T, 8>(ml, os, nh, hd, out); break;
+        default: join_pieces<T, 16>(ml, os, nh, hd, out); break;
     }
     cluster.sync();     // a CTA's shared memory outlives its readers
 }
@@ -126,7 +149,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
     bf16* KV = Qs + 16 * SD;                       // [STAGES][2][64][SD]
     int* pages = reinterpret_cast<int*>(KV + STAGES * STAGE);   // [top]
     __shared__ int counts[THREADS / 32];
-    __shared__ float ml[16][2];
+    __shared__ alignas(8) float ml[16][2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     pdl_wait();
     Place at;
@@ -303,7 +326,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
             ml[r][1] = L;
         }
     }
-    join<bf16>(p, &ml[0][0], Os, at.nh, HD, (bf16*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * HD);
+    join<bf16>(&ml[0][0], Os, at.nh, HD, (bf16*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * HD);
 }
 
 // ---- float32 -------------------------------------------------------------------------------------
@@ -326,7 +349,8 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
     float* Ps = Part + 4 * NH * F_KEYS;            // [NH][32]
     int* pages = reinterpret_cast<int*>(Ps + NH * F_KEYS);
     __shared__ int counts[THREADS / 32];
-    __shared__ float ml[NH][2], corr[NH];
+    __shared__ alignas(8) float ml[NH][2];
+    __shared__ float corr[NH];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     Place at;
@@ -441,10 +465,10 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
         for (int c = 0; c < F_CH; c++)
             if (h < at.nh && tid + c * THREADS < d) Os[h * d + tid + c * THREADS] = o[h][c];
     __syncthreads();
-    join<float>(p, &ml[0][0], Os, at.nh, d, (float*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * d);
+    join<float>(&ml[0][0], Os, at.nh, d, (float*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * d);
 }
 
-// Into how many pieces a row's list is cut: the CTAs of a cluster.  As many as run at once (one token over eight key heads, 32 pages:
+// Into how many pieces a row's list is cut: the CTAs of a cluster, a power of two (sixteen where the GPU holds all of the clusters).  As many as run at once (one token over eight key heads, 32 pages:
 // 34 us in one piece, 19 in two, 12 in four, 8.4 in eight); where not even two pieces each do, two if their waves end sooner than
 // those of whole rows (50 sequences over eight key heads, 64 pages: 173 us in one piece, 147 in two, 158 in four, 197 in eight).
 int pieces_for(const PagesParams& p, int chunks, int per_sm, int wide) {
@@ -466,26 +490,34 @@ int launch(K kernel, const PagesParams& p, int chunks, int pieces, int smem, cud
     return 0;
 }
 
-// Shared memory and clusters of 16 for a kernel; how many of those clusters the GPU holds at once (0: none, or not allowed).
+// Shared memory and clusters of 16 for a kernel on the current device; how many of those clusters it holds at once (0: none, or not
+// allowed).  known: one number a device, one more than that.
 template <typename K>
-int configure(K kernel, int smem, int& wide) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    wide = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(16);
-        cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = smem;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 16;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&wide, kernel, &cfg) != cudaSuccess) wide = 0;
+int configure(K kernel, int smem, int (&known)[64], int& wide) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64) GB_REFUSE("attention_pages: no current device");
+    if (!known[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+        int most = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(16);
+            cfg.blockDim = dim3(THREADS);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 16;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess) most = 0;
+        }
+        cudaGetLastError();     // what was not possible is no error of the call
+        known[dev] = 1 + (most > 0 ? most : 0);
     }
-    cudaGetLastError();     // what was not possible is no error of the call
+    wide = known[dev] - 1;
     return 0;
 }
 
@@ -494,20 +526,20 @@ int launch_mma(const PagesParams& p, cudaStream_t stream) {
     constexpr int SD = HD + 8;
     constexpr int base = (16 * SD + STAGES * 2 * 64 * SD) * 2;
     static_assert(base >= (128 + 64 * HD) * 4 + 16 * SD * 2, "the warps' results fit where the pages were");
-    static int wide = -1;
-    if (wide < 0)
-        if (int rc = configure(attn_pages_mma_kernel<HD>, base + MAX_TOP * 4, wide)) return rc;
+    static int known[64];
+    int wide = 0;
+    if (int rc = configure(attn_pages_mma_kernel<HD>, base + MAX_TOP * 4, known, wide)) return rc;
     const int G = p.heads / p.kv_heads, chunks = (G + 15) / 16;
     return launch(attn_pages_mma_kernel<HD>, p, chunks, pieces_for(p, chunks, HD <= 128 ? 2 : 1, wide), base + p.top * 4, stream);
 }
 
 template <int NH>
 int launch_f32(const PagesParams& p, cudaStream_t stream) {
-    static int wide = -1;
+    static int known[64];
+    int wide = 0;
     constexpr int most = f32_floats(256, NH) * 4 + MAX_TOP * 4;
     static_assert(most <= 231000, "the widest heads' stages fit");
-    if (wide < 0)
-        if (int rc = configure(attn_pages_f32_kernel<NH>, most, wide)) return rc;
+    if (int rc = configure(attn_pages_f32_kernel<NH>, most, known, wide)) return rc;
     const int G = p.heads / p.kv_heads, chunks = (G + NH - 1) / NH;
     return launch(attn_pages_f32_kernel<NH>, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1, wide), f32_floats(p.d, NH) * 4 + p.top * 4, stream);
 }

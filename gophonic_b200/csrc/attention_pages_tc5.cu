@@ -639,13 +639,10 @@ int gb_attention_pages_tc5_accepts(const PagesParams& p) {
 }
 
 int gb_attention_pages_tc5(const PagesParams& p, cudaStream_t stream) {
-    static bool configured = false;
-    if (!configured) {
-        const int most = TILE_BYTES + 1024 + LIST_BYTES;
-        const cudaError_t e = cudaFuncSetAttribute(attn_pages_tc5_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (e != cudaSuccess) GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", most, cudaGetErrorString(e));
-        configured = true;
-    }
+    static bool done[64];
+    constexpr int most = TILE_BYTES + 1024 + LIST_BYTES;
+    if (const cudaError_t e = gb_allow_smem(attn_pages_tc5_kernel, most, done))
+        GB_REFUSE("attention_pages: cannot reserve %d bytes of shared memory: %s", most, cudaGetErrorString(e));
     const int G = p.heads / p.kv_heads, gp = padded_group(G), tok = ROWS / gp;
     CUtensorMap map_q, map_k, map_v;
     {

@@ -119,6 +119,18 @@ __device__ __forceinline__ const int* block_table_row(const int* __restrict__ ta
     return table + (int64_t)slot * bt_stride;
 }
 
+// Lets `kernel` have `smem` bytes of dynamic shared memory on the current device.  `done`: one flag a device, kept by the caller's static;
+// the attribute belongs to the device that is current when it is set.
+template <typename K>
+static inline cudaError_t gb_allow_smem(K kernel, int smem, bool (&done)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+}
+
 static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Programmatic dependent launch.  A kernel launched with the programmatic-serialization attribute

@@ -57,11 +57,10 @@ __device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
 
 // ---- bounds ------------------------------------------------------------------------------------
 // A warp takes one page of one key head of one plane: the page whose last position is among the step's new rows.  A key is CH chunks
-// of 16 bytes; LPR lanes (a power of two) have one key's chunks, so the warp reads 32 / LPR keys with one load, and asks for up to 16
-// loads before it looks at any.  Bound by the read of the keys: 36 planes of 16 single tokens of which four fill a
-// page 5.0 us, eight prompts of up to 2048 4.8, 16384 rows of one sequence 5.3 (34 MB from L2).  A CTA of 256 threads for a page and
-// head, its threads' extremes joined in shared memory: 13.0, 9.7, 15.4.
-constexpr int BOUND_WARPS = 4;
+// of 16 bytes; LPR lanes (a power of two) have one key's chunks, so the warp reads 32 / LPR keys with one copy, and asks for 32
+// copies (16 KB, a whole page of 128 bfloat16 channels) before it looks at any: by cp.async, each lane into places of its own
+// that only it reads.  Bound by the read of the keys.
+constexpr int BOUND_WARPS = 4, BOUND_LOADS = 32;
 
 __device__ __forceinline__ uint32_t low2(uint32_t a, uint32_t b, bf16) {
     const __nv_bfloat162 v = __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
@@ -76,7 +75,9 @@ __device__ __forceinline__ uint32_t high2(uint32_t a, uint32_t b, float) { retur
 
 template <typename T, int LPR, int CPL>
 __global__ void __launch_bounds__(BOUND_WARPS * 32) page_bounds_kernel(PagesParams p) {
-    constexpr int KEYS = 32 / LPR, LOADS = GB_PAGE / KEYS < 16 / CPL ? GB_PAGE / KEYS : 16 / CPL;   // keys a load; loads in flight
+    constexpr int KEYS = 32 / LPR, TIMES = GB_PAGE / KEYS, STEP = BOUND_LOADS / CPL < TIMES ? BOUND_LOADS / CPL : TIMES;   // keys a copy; of each chunk at once
+    extern __shared__ __align__(16) unsigned char raw[];
+    uint4* mine = reinterpret_cast<uint4*>(raw) + (threadIdx.x >> 5) * BOUND_LOADS * 32 + (threadIdx.x & 31);
     pdl_wait();                     // the keys, and the step's metadata
     pdl_trigger();
     const int seq = blockIdx.z, lane = threadIdx.x & 31;
@@ -90,22 +91,24 @@ __global__ void __launch_bounds__(BOUND_WARPS * 32) page_bounds_kernel(PagesPara
     const uint4* k = reinterpret_cast<const uint4*>((const T*)p.k_plane + at * GB_PAGE * p.d) + sub * CH;
     uint4* to = reinterpret_cast<uint4*>((T*)p.bounds + at * 2 * p.d);
     uint32_t lo[CPL][4], hi[CPL][4];
+    for (int r0 = 0; r0 < TIMES; r0 += STEP) {
 #pragma unroll
-    for (int r0 = 0; r0 < GB_PAGE / KEYS; r0 += LOADS) {
-        uint4 x[LOADS][CPL];
+        for (int r = 0; r < STEP; r++)
 #pragma unroll
-        for (int r = 0; r < LOADS; r++)
+            for (int c = 0; c < CPL; c++) cp_async16(mine + (r * CPL + c) * 32, l + c * LPR < CH ? k + (r0 + r) * KEYS * CH + l + c * LPR : k, l + c * LPR < CH ? 16 : 0);
+        cp_async_commit();
+        cp_async_wait<0>();
 #pragma unroll
-            for (int c = 0; c < CPL; c++) x[r][c] = l + c * LPR < CH ? k[(r0 + r) * KEYS * CH + l + c * LPR] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < LOADS; r++)
+        for (int r = 0; r < STEP; r++)
 #pragma unroll
             for (int c = 0; c < CPL; c++) {
-                const uint32_t w[4] = {x[r][c].x, x[r][c].y, x[r][c].z, x[r][c].w};
+                const uint4 x = mine[(r * CPL + c) * 32];
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    lo[c][e] = r0 + r == 0 ? w[e] : low2(lo[c][e], w[e], T());
-                    hi[c][e] = r0 + r == 0 ? w[e] : high2(hi[c][e], w[e], T());
+                    const bool first = r0 == 0 && r == 0;
+                    lo[c][e] = first ? w[e] : low2(lo[c][e], w[e], T());
+                    hi[c][e] = first ? w[e] : high2(hi[c][e], w[e], T());
                 }
             }
     }
@@ -899,12 +902,19 @@ GB_API int gb_page_bounds(const PagesParams* pp, int dtype, cudaStream_t stream)
     if (p.nseq <= 0 || p.max_q_len <= 0 || p.planes <= 0) return 0;
     if (int rc = check(p, dtype, "page_bounds")) return rc;
     if ((uintptr_t)p.k_plane & 15) GB_REFUSE("page_bounds: the key plane must be 16-byte aligned");
+    constexpr int smem = BOUND_WARPS * BOUND_LOADS * 512;
     const int pages = ceil_div(p.max_q_len, GB_PAGE);
     if ((int64_t)p.kv_heads * p.planes > (1 << 28) || pages > 65535 || p.nseq > 65535)
         GB_REFUSE("page_bounds: %d kv heads x %d planes, %d sequences of up to %d rows exceed one launch", p.kv_heads, p.planes, p.nseq, p.max_q_len);
     const dim3 grid(ceil_div(p.kv_heads * p.planes, BOUND_WARPS), pages, p.nseq);
     const int chunks = p.d * (dtype == GB_F32 ? 4 : 2) / 16;
-#define GB_BOUNDS(T, LPR, CPL) launch_pdl(page_bounds_kernel<T, LPR, CPL>, grid, dim3(BOUND_WARPS * 32), 0, stream, p)
+#define GB_BOUNDS(T, LPR, CPL)                                                                                                          \
+    do {                                                                                                                                \
+        static bool done[64];                                                                                                           \
+        const cudaError_t e = gb_allow_smem(page_bounds_kernel<T, LPR, CPL>, smem, done);                                               \
+        if (e != cudaSuccess) GB_REFUSE("page_bounds: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));       \
+        launch_pdl(page_bounds_kernel<T, LPR, CPL>, grid, dim3(BOUND_WARPS * 32), (size_t)smem, stream, p);                             \
+    } while (0)
     if (dtype == GB_F32) {
         if (chunks <= 16) GB_BOUNDS(float, 16, 1);
         else if (chunks <= 32) GB_BOUNDS(float, 32, 1);
@@ -921,13 +931,9 @@ GB_API int gb_page_bounds(const PagesParams* pp, int dtype, cudaStream_t stream)
 
 template <typename T, int LP, int CPL>
 static int launch_rows(const PagesParams& p, cudaStream_t stream) {
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(select_row_kernel<T, LP, CPL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)(sizeof(SelectSmem) + MAX_PAGES * sizeof(uint32_t)));
-        if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
-        configured = true;
-    }
+    static bool done[64];
+    const cudaError_t e = gb_allow_smem(select_row_kernel<T, LP, CPL>, (int)(sizeof(SelectSmem) + MAX_PAGES * sizeof(uint32_t)), done);
+    if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
     // pieces of no fewer pages than the CTA's warps take at a time, while they all run at once
     const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads;
     int pieces = 1;
@@ -947,12 +953,9 @@ static int64_t tile_smem(const PagesParams& p, int rt) {
 
 template <int MT, int KB_MAX, int TILE_WARPS>
 static int launch_tiles(const PagesParams& p, cudaStream_t stream) {
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(select_tile_kernel<MT, KB_MAX, TILE_WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_TILE_SMEM);
-        if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
-        configured = true;
-    }
+    static bool done[64];
+    const cudaError_t e = gb_allow_smem(select_tile_kernel<MT, KB_MAX, TILE_WARPS>, MAX_TILE_SMEM, done);
+    if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
     const dim3 grid(ceil_div(p.max_q_len, MT * 16), p.kv_heads, p.nseq);
     if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("select_pages: %d kv heads, %d sequences exceed one launch", p.kv_heads, p.nseq);
     launch_pdl(select_tile_kernel<MT, KB_MAX, TILE_WARPS>, grid, dim3(TILE_WARPS * 32), (size_t)tile_smem<TILE_WARPS>(p, MT * 16), stream, p);
