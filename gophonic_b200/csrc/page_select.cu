@@ -709,20 +709,22 @@ constexpr int TILE_BAND = 48;
 template <int TILE_WARPS>
 struct alignas(16) TileSmem {
     Chooser<1, TILE_BAND, 16, 16> choose[TILE_WARPS];
-    float size[64];          // per chunk of 8 bounds: their largest size, over all pages
+    float size[32];          // per chunk of 8 channels: their bounds' largest size, over all pages
     int next;                // the row that the next warp to be done takes: rows whose border is close take twice as long
 };
 
 __host__ __device__ inline int tile_coef_stride(int d) { return 2 * d + 32; }        // elements: rows 64 bytes of banks apart
 __host__ __device__ inline int tile_key_stride(int pages) { return (pages + 31) / 32 * 32 + 8; }
 
-template <int MT, int KB_MAX, int TILE_WARPS>
+// KB_MAX: blocks of 32 bounds a page has at most, or, with EXACT (KB_MAX even), has: the offsets are then known (2000 rows 74 -> 70 us).
+template <int MT, int KB_MAX, bool EXACT, int TILE_WARPS>
 __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_kernel(const __grid_constant__ PagesParams p) {
     constexpr int RT = MT * 16, TILE_THREADS = TILE_WARPS * 32;
     using TileSmem = TileSmem<TILE_WARPS>;
     extern __shared__ __align__(16) unsigned char raw[];
     TileSmem& s = *reinterpret_cast<TileSmem*>(raw);
-    const int CS = tile_coef_stride(p.d), KS = tile_key_stride(p.bt_stride);
+    const int d = EXACT ? KB_MAX * 16 : p.d, KB = d / 16;
+    const int CS = tile_coef_stride(d), KS = tile_key_stride(p.bt_stride);
     bf16* coef = reinterpret_cast<bf16*>(raw + sizeof(TileSmem));                    // [2][RT][CS]
     uint32_t* keys = reinterpret_cast<uint32_t*>(coef + 2 * RT * CS);                // [RT][KS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
     const int seq = blockIdx.z, kvh = blockIdx.y, q0 = blockIdx.x * RT;
     const int q_len = p.seq_q_len[seq];
     if (q0 >= q_len) return;
-    const int rows = min(RT, q_len - q0), d = p.d, G = p.heads / p.kv_heads;
+    const int rows = min(RT, q_len - q0), G = p.heads / p.kv_heads;
     const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
     // candidates of the last row, which has the most
     const int past = p.seq_kv_len[seq] - q_len, q_start = p.seq_q_start[seq];
@@ -778,15 +780,16 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
                 *reinterpret_cast<uint4*>(to + RT * CS + side * d) = make_uint4(second[0], second[1], second[2], second[3]);
             }
         }
-        for (int i = tid; i < 64; i += TILE_THREADS) s.size[i] = 0.f;
+        for (int i = tid; i < 32; i += TILE_THREADS) s.size[i] = 0.f;
         if (tid == 0) s.next = TILE_WARPS;
     }
     __syncthreads();
-    const int KB = d / 16;             // blocks of 32 bounds
     const bf16* plane = (const bf16*)p.bounds;
-    __nv_bfloat162 size[KB_MAX];       // of each block: the largest this lane has met in its chunk of 8
+    // Of each block of bounds, in the lane's chunk of 8: the least of the lowest values, the most of the highest.  As lo <= hi, a channel's
+    // bounds are no larger than the larger of the two.
+    __nv_bfloat162 reach[KB_MAX];
 #pragma unroll
-    for (int kb = 0; kb < KB_MAX; kb++) size[kb] = __floats2bfloat162_rn(0.f, 0.f);
+    for (int kb = 0; kb < KB_MAX; kb++) reach[kb] = __floats2bfloat162_rn(0.f, 0.f);
     for (int i0 = warp * 16; i0 < nc; i0 += TILE_WARPS * 16) {
         const bf16* b[2];
 #pragma unroll
@@ -819,8 +822,8 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
                     const uint32_t w[4] = {x[j][t].x, x[j][t].y, x[j][t].z, x[j][t].w};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const uint32_t a = w[e] & 0x7fff7fffu;
-                        size[kb] = __hmax2_nan(size[kb], *reinterpret_cast<const __nv_bfloat162*>(&a));
+                        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&w[e]);
+                        reach[kb] = (EXACT ? kb * 2 < KB : kb * 4 + t4 < KB * 2) ? __hmin2_nan(reach[kb], v) : __hmax2_nan(reach[kb], v);
                     }
                 }
 #pragma unroll
@@ -849,11 +852,15 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
 #pragma unroll
     for (int kb = 0; kb < KB_MAX; kb++) {
         if (kb >= KB) break;
-        const float lo = __low2float(size[kb]), hi = __high2float(size[kb]);
-        float v = lo != lo || hi != hi ? INFINITY : fmaxf(lo, hi);
+        const float a = fabsf(__low2float(reach[kb])), b = fabsf(__high2float(reach[kb]));
+        float v = a != a || b != b ? INFINITY : fmaxf(a, b);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-        if (g == 0) atomicMax(reinterpret_cast<int*>(&s.size[kb * 4 + t4]), __float_as_int(v));   // not negative: ordered as integers
+        // (not negative: ordered as integers); a chunk of the lowest values and the same channels' highest share a place
+        if (g == 0) {
+            const int at = kb * 4 + t4;
+            atomicMax(reinterpret_cast<int*>(&s.size[at < KB * 2 ? at : at - KB * 2]), __float_as_int(v));
+        }
     }
     __syncthreads();
     for (int row = warp; row < rows; row = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(&s.next, 1) : 0, 0)) {
@@ -869,7 +876,7 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
         float most = 0.f, steps = 0.f;
 #pragma unroll 8
         for (int c = lane; c < 2 * d; c += 32) {
-            const float term = (fabsf(__bfloat162float(coef[row * CS + c])) + 1.0e-35f) * s.size[c >> 3];
+            const float term = (fabsf(__bfloat162float(coef[row * CS + c])) + 1.0e-35f) * s.size[(c < d ? c : c - d) >> 3];
             most += term;
             steps = fmaf(term, (float)(4 * (KB - (c >> 5))), steps);
         }
@@ -951,16 +958,23 @@ static int64_t tile_smem(const PagesParams& p, int rt) {
     return (int64_t)sizeof(TileSmem<TILE_WARPS>) + 2 * rt * tile_coef_stride(p.d) * 2 + (int64_t)rt * tile_key_stride(p.bt_stride) * 4;
 }
 
-template <int MT, int KB_MAX, int TILE_WARPS>
-static int launch_tiles(const PagesParams& p, cudaStream_t stream) {
+template <int MT, int KB_MAX, bool EXACT, int TILE_WARPS>
+static int launch_tiles_of(const PagesParams& p, cudaStream_t stream) {
     static bool done[64];
-    const cudaError_t e = gb_allow_smem(select_tile_kernel<MT, KB_MAX, TILE_WARPS>, MAX_TILE_SMEM, done);
+    const cudaError_t e = gb_allow_smem(select_tile_kernel<MT, KB_MAX, EXACT, TILE_WARPS>, MAX_TILE_SMEM, done);
     if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
     const dim3 grid(ceil_div(p.max_q_len, MT * 16), p.kv_heads, p.nseq);
     if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("select_pages: %d kv heads, %d sequences exceed one launch", p.kv_heads, p.nseq);
-    launch_pdl(select_tile_kernel<MT, KB_MAX, TILE_WARPS>, grid, dim3(TILE_WARPS * 32), (size_t)tile_smem<TILE_WARPS>(p, MT * 16), stream, p);
+    launch_pdl(select_tile_kernel<MT, KB_MAX, EXACT, TILE_WARPS>, grid, dim3(TILE_WARPS * 32), (size_t)tile_smem<TILE_WARPS>(p, MT * 16), stream, p);
     GB_CHECK_LAUNCH("select_pages");
     return 0;
+}
+
+template <int MT, int TILE_WARPS>
+static int launch_tiles(const PagesParams& p, cudaStream_t stream) {
+    if (p.d == 128) return launch_tiles_of<MT, 8, true, TILE_WARPS>(p, stream);
+    if (p.d == 64) return launch_tiles_of<MT, 4, true, TILE_WARPS>(p, stream);
+    return launch_tiles_of<MT, 16, false, TILE_WARPS>(p, stream);
 }
 
 GB_API int gb_select_pages(const PagesParams* pp, int dtype, cudaStream_t stream) {
@@ -971,9 +985,9 @@ GB_API int gb_select_pages(const PagesParams* pp, int dtype, cudaStream_t stream
     if (p.first < 0 || p.last < 1 || p.first + p.last > p.top) GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
     if (p.bt_stride > MAX_PAGES) GB_REFUSE("select_pages: sequences of up to %d pages; this kernel takes %d", p.bt_stride, MAX_PAGES);
     if (dtype == GB_BF16 && p.max_q_len >= TILE_MIN_ROWS && p.d % 16 == 0) {
-        if (p.max_q_len > 16 && p.d <= 128 && tile_smem<8>(p, 32) <= HALF_TILE_SMEM) return launch_tiles<2, 8, 8>(p, stream);
-        if (p.max_q_len > 16 && tile_smem<16>(p, 32) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<2, 8, 16>(p, stream) : launch_tiles<2, 16, 16>(p, stream);
-        if (tile_smem<16>(p, 16) <= MAX_TILE_SMEM) return p.d <= 128 ? launch_tiles<1, 8, 16>(p, stream) : launch_tiles<1, 16, 16>(p, stream);
+        if (p.max_q_len > 16 && tile_smem<8>(p, 32) <= HALF_TILE_SMEM) return launch_tiles<2, 8>(p, stream);
+        if (p.max_q_len > 16 && tile_smem<16>(p, 32) <= MAX_TILE_SMEM) return launch_tiles<2, 16>(p, stream);
+        if (tile_smem<16>(p, 16) <= MAX_TILE_SMEM) return launch_tiles<1, 16>(p, stream);
     }
     const int chunks = 2 * p.d / (dtype == GB_F32 ? 4 : 8);
     if (dtype == GB_F32) {

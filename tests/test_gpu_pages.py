@@ -200,10 +200,10 @@ def test_select_pages_of_many_sequences(ops, dtype, equal):
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=names)
 @pytest.mark.parametrize("kind", ["equal", "few kinds", "zero query", "one ulp", "nan", "inf", "huge", "tiny", "nan query", "inf query", "cancel"])
-@pytest.mark.parametrize("pages,new", [(40, 2), (700, 2), (40, 21), (300, 9)])
-def test_select_pages_near_the_border(ops, dtype, kind, pages, new):
+@pytest.mark.parametrize("pages,new,d", [(40, 2, 128), (700, 2, 128), (40, 21, 128), (300, 9, 128), (300, 21, 48), (300, 9, 16), (100, 30, 64), (100, 9, 256), (300, 2, 48)])
+def test_select_pages_near_the_border(ops, dtype, kind, pages, new, d):
     """Scores that tie, that differ in the last place of one channel, that float32 cannot hold: the choice is the 64-bit one."""
-    s = wide_step(dtype, pages, new=new)
+    s = wide_step(dtype, pages, new=new, d=d)
     g = torch.Generator().manual_seed(pages)
     bounds = s.bounds_plane()
     n = s.table.shape[1]
