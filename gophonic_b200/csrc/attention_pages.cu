@@ -39,7 +39,7 @@ __device__ __forceinline__ int pack_list(const PagesParams& p, const int* list, 
     for (int base = 0; base < p.top; base += THREADS) {
         const int i = base + tid;
         const int lp = i < p.top ? list[i] : -1;
-        const bool ok = lp >= 0 && lp <= own_page;
+        const bool ok = lp >= 0 && lp <= own_page && lp < p.bt_stride;
         const unsigned who = __ballot_sync(0xffffffffu, ok);
         if (lane == 0) counts[warp] = __popc(who);
         __syncthreads();

@@ -176,7 +176,7 @@ __device__ __noinline__ void row_alone(const PagesParams& p, const int* bt, int 
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < p.top; i++) {
         const int lp = list[i];
-        if (lp < 0 || lp > pos / BKV) continue;
+        if (lp < 0 || lp > pos / BKV || lp >= p.bt_stride) continue;
         const int64_t off = (page_of(bt, lp * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * (int64_t)(BKV * HD);
         const bf16 *k = (const bf16*)p.k_plane + off, *v = (const bf16*)p.v_plane + off;
         const int n = min(BKV, pos + 1 - lp * BKV);

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(BOUND_WARPS * 32) page_bounds_kernel(PagesPara
     const int unit = (int)blockIdx.x * BOUND_WARPS + (int)(threadIdx.x >> 5), kvh = unit % p.kv_heads, plane = unit / p.kv_heads;
     const int kv_len = p.seq_kv_len[seq], past = kv_len - p.seq_q_len[seq];
     const int lp = past / GB_PAGE + (int)blockIdx.y;
-    if (lp >= kv_len / GB_PAGE || plane >= p.planes) return;
+    if (lp >= kv_len / GB_PAGE || lp >= p.bt_stride || plane >= p.planes) return;
     const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
     const int64_t at = ((int64_t)plane * p.pages + page_of(bt, lp * GB_PAGE, p.bt_stride, p.pages)) * p.kv_heads + kvh;
     const int CH = p.d * (int)sizeof(T) / 16, sub = lane / LPR, l = lane % LPR;
@@ -158,7 +158,7 @@ struct Row {
         list = p.list + ((int64_t)row * p.kv_heads + kvh) * p.top;
         q = (const T*)p.q + (int64_t)row * p.q_row_stride + (int64_t)kvh * (p.heads / p.kv_heads) * p.d;
         bt = table_row;
-        n = pos / GB_PAGE + 1;
+        n = min(pos / GB_PAGE + 1, p.bt_stride);      // (a sequence is no longer than its row of the table)
         c0 = p.first;
         nc = n - p.first - p.last;
         k = p.top - p.first - p.last;
@@ -737,7 +737,7 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
     const int* bt = block_table_row(p.block_table, p.bt_stride, p.seq_slot[seq], p.max_slots);
     // candidates of the last row, which has the most
     const int past = p.seq_kv_len[seq] - q_len, q_start = p.seq_q_start[seq];
-    const int nc = (past + q0 + rows - 1) / GB_PAGE + 1 - p.first - p.last;
+    const int nc = min((past + q0 + rows - 1) / GB_PAGE + 1, p.bt_stride) - p.first - p.last;
     {
         const bf16* q = (const bf16*)p.q + (int64_t)(q_start + q0) * p.q_row_stride + (int64_t)kvh * G * d;
         const bool whole = !(((uintptr_t)p.q & 15) | (p.q_row_stride & 7));     // rows of 16-byte chunks

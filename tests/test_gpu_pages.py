@@ -514,3 +514,8 @@ def test_refusals(ops):
     bad(lambda: ops.page_bounds(odd, torch.zeros((4, 1, 2, 20), dtype=BF, device=DEV), table, slot, q_len, kv_len, 1, 1))
     shifted = torch.zeros(257, dtype=BF, device=DEV)[1:].view(1, 256)
     bad(lambda: attend(q=shifted))
+
+
+def test_zz_no_kernel_met_a_bad_index_or_gave_up(ops):
+    """Behind all of the above: no wait ran out and (in the checked build) no index left its bounds."""
+    assert ops.tc5_status() == 0 and ops.checked_status() is None
