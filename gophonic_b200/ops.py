@@ -826,20 +826,26 @@ for _f in (_lib.gb_page_bounds, _lib.gb_select_pages, _lib.gb_attention_pages):
     _f.argtypes = (c_void_p, c_int, c_void_p)
 
 
-def _is_index(t: torch.Tensor, n: int, dev: int) -> bool:
-    return t.dtype is torch.int32 and t.get_device() == dev and t.numel() >= n and t.is_contiguous()
+_I32, _BF16T, _F32T = torch.int32, torch.bfloat16, torch.float32
 
 
-def _is_plane(t: torch.Tensor, dtype, dev: int) -> bool:
-    return t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
+def _all_flat(dev: int, n: int, lists) -> bool:
+    """Whether all of ``lists`` are contiguous int32 tensors of at least ``n`` entries on device ``dev``."""
+    for t in lists:
+        if t.dtype is not _I32 or t.get_device() != dev or t.numel() < n or not t.is_contiguous():
+            return False
+    return True
 
 
-def _pages_stream(who: str, dev: int) -> c_void_p:
-    """The stream of a call whose tensors are all on device ``dev``, which has to be the library's."""
-    stream = _stream()
+def _pages_call(who: str, fn, packed: bytes, dtype, dev: int) -> None:
+    """``fn`` on the library's stream, for tensors that are all on device ``dev``, which has to be the library's."""
+    global launches
+    stream = _raw_stream(_device_index[0]) if _device_index and _raw_stream is not None else _stream()
     if _device_index and _device_index[0] != dev:
         raise KernelError(f"{who}: tensors on cuda:{dev}, the library serves cuda:{_device_index[0]}")
-    return stream
+    if fn(packed, 1 if dtype is _BF16T else _code(dtype), stream) != 0:
+        raise KernelError(_lib.gb_last_error().decode("utf-8", "replace"))
+    launches += 1
 
 
 def _need_sequences(who: str, block_table: torch.Tensor, nseq: int, **lists: torch.Tensor) -> None:
@@ -872,20 +878,26 @@ def page_bounds(k_planes: torch.Tensor, bounds: torch.Tensor, block_table: torch
     head_dim] of the same dtype, or several such planes in one leading dimension.  Nothing else of ``bounds`` changes.  To be called
     behind what writes the step's keys; ``select_pages`` scores the pages of earlier tokens by it."""
     shape, dtype, dev = k_planes.shape, k_planes.dtype, k_planes.get_device()
-    if len(shape) not in (4, 5):
+    if len(shape) == 5:
+        planes, pages, kv_heads, tokens, d = shape
+        want = (planes, pages, kv_heads, 2, d)
+    elif len(shape) == 4:
+        planes = 1
+        pages, kv_heads, tokens, d = shape
+        want = (pages, kv_heads, 2, d)
+    else:
         raise KernelError(f"page_bounds: key planes {tuple(shape)}")
-    planes, (pages, kv_heads, tokens, d) = (shape[0], shape[1:]) if len(shape) == 5 else (1, shape)
     table = block_table.shape
-    if not (dev >= 0 and k_planes.is_contiguous() and _is_plane(bounds, dtype, dev) and tokens == PAGE and tuple(bounds.shape) == (*shape[:-2], 2, d)
-            and len(table) == 2 and _is_index(block_table, 0, dev) and _is_index(seq_slot, nseq, dev) and _is_index(seq_q_len, nseq, dev)
-            and _is_index(seq_kv_len, nseq, dev)):
+    if not (dev >= 0 and tokens == PAGE and k_planes.is_contiguous() and bounds.dtype is dtype and bounds.get_device() == dev
+            and bounds.is_contiguous() and bounds.shape == want and len(table) == 2 and _all_flat(dev, nseq, (seq_slot, seq_q_len, seq_kv_len))
+            and _all_flat(dev, 0, (block_table,))):
         _need(k_planes, "key planes")
         _need(bounds, "page bounds", dtype)
         _need_sequences("page_bounds", block_table, nseq, seq_slot=seq_slot, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
         raise KernelError(f"page_bounds: key planes {tuple(shape)}, bounds {tuple(bounds.shape)}, or tensors on different devices")
-    p = _PAGES_LAYOUT.pack(0, 0, 0, 0, k_planes.data_ptr(), 0, bounds.data_ptr(), block_table.data_ptr(), table[1], seq_slot.data_ptr(), 0,
-                           seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, 0, kv_heads, d, max_q_len, 0.0, 0, 0, 0, 0, planes, pages, table[0], 0)
-    _check(_lib.gb_page_bounds(p, _code(dtype), _pages_stream("page_bounds", dev)))
+    _pages_call("page_bounds", _lib.gb_page_bounds, _PAGES_LAYOUT.pack(
+        0, 0, 0, 0, k_planes.data_ptr(), 0, bounds.data_ptr(), block_table.data_ptr(), table[1], seq_slot.data_ptr(), 0, seq_q_len.data_ptr(),
+        seq_kv_len.data_ptr(), nseq, 0, kv_heads, d, max_q_len, 0.0, 0, 0, 0, 0, planes, pages, table[0], 0), dtype, dev)
 
 
 def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_slot: torch.Tensor, seq_q_start: torch.Tensor,
@@ -905,10 +917,10 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
     if ok:
         rows, width = shape
         row_stride, unit = q.stride()
-        ok = (unit == 1 and width >= wide and (rows <= 1 or row_stride >= wide) and _is_plane(bounds, dtype, dev)
-              and tuple(plane) == (plane[0], kv_heads, 2, head_dim) and _is_plane(pages, torch.int32, dev) and listed[0] == rows
-              and listed[1] == kv_heads and _is_index(block_table, 0, dev) and _is_index(seq_slot, nseq, dev)
-              and _is_index(seq_q_start, nseq, dev) and _is_index(seq_q_len, nseq, dev) and _is_index(seq_kv_len, nseq, dev))
+        ok = (unit == 1 and width >= wide and (rows <= 1 or row_stride >= wide) and bounds.dtype is dtype and bounds.get_device() == dev
+              and bounds.is_contiguous() and len(plane) == 4 and plane == (plane[0], kv_heads, 2, head_dim) and listed[0] == rows
+              and listed[1] == kv_heads and _all_flat(dev, nseq, (seq_slot, seq_q_start, seq_q_len, seq_kv_len))
+              and _all_flat(dev, 0, (block_table, pages)))
     if not ok:
         _need_rows("select_pages", "q", q, None, wide)
         _need(bounds, "page bounds", dtype, 4)
@@ -916,10 +928,10 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
         _need_sequences("select_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
         raise KernelError(f"select_pages: bounds {tuple(plane)}, lists {tuple(listed)} for q {tuple(shape)} of {heads} over {kv_heads} heads of "
                           f"{head_dim}, or tensors on different devices")
-    p = _PAGES_LAYOUT.pack(q.data_ptr(), row_stride, 0, 0, 0, 0, bounds.data_ptr(), block_table.data_ptr(), table[1], seq_slot.data_ptr(),
-                           seq_q_start.data_ptr(), seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, heads, kv_heads, head_dim, max_q_len, 0.0,
-                           pages.data_ptr(), listed[2], first, last, 0, plane[0], table[0], rows)
-    _check(_lib.gb_select_pages(p, _code(dtype), _pages_stream("select_pages", dev)))
+    _pages_call("select_pages", _lib.gb_select_pages, _PAGES_LAYOUT.pack(
+        q.data_ptr(), row_stride, 0, 0, 0, 0, bounds.data_ptr(), block_table.data_ptr(), table[1], seq_slot.data_ptr(), seq_q_start.data_ptr(),
+        seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, heads, kv_heads, head_dim, max_q_len, 0.0, pages.data_ptr(), listed[2], first, last, 0,
+        plane[0], table[0], rows), dtype, dev)
 
 
 def attention_pages(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, block_table: torch.Tensor,
@@ -939,10 +951,10 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v
         out_stride, out_unit = out.stride()
         ok = (unit == 1 and out_unit == 1 and width >= wide and to[1] >= wide and to[0] == rows
               and (rows <= 1 or (row_stride >= wide and out_stride >= wide)) and out.dtype is dtype and out.get_device() == dev
-              and _is_plane(k_plane, dtype, dev) and _is_plane(v_plane, dtype, dev) and tuple(plane) == (plane[0], kv_heads, PAGE, head_dim)
-              and v_plane.shape == plane and _is_plane(pages, torch.int32, dev) and listed[0] == rows and listed[1] == kv_heads
-              and _is_index(block_table, 0, dev) and _is_index(seq_slot, nseq, dev) and _is_index(seq_q_start, nseq, dev)
-              and _is_index(seq_q_len, nseq, dev) and _is_index(seq_kv_len, nseq, dev))
+              and k_plane.dtype is dtype and k_plane.get_device() == dev and k_plane.is_contiguous() and v_plane.dtype is dtype
+              and v_plane.get_device() == dev and v_plane.is_contiguous() and len(plane) == 4 and plane == (plane[0], kv_heads, PAGE, head_dim)
+              and v_plane.shape == plane and listed[0] == rows and listed[1] == kv_heads
+              and _all_flat(dev, nseq, (seq_slot, seq_q_start, seq_q_len, seq_kv_len)) and _all_flat(dev, 0, (block_table, pages)))
     if not ok:
         _need_rows("attention_pages", "q", q, None, wide)
         _need_rows("attention_pages", "out", out, dtype, wide)
@@ -952,10 +964,10 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v
         _need_sequences("attention_pages", block_table, nseq, seq_slot=seq_slot, seq_q_start=seq_q_start, seq_q_len=seq_q_len, seq_kv_len=seq_kv_len)
         raise KernelError(f"attention_pages: q {tuple(shape)}, out {tuple(to)}, lists {tuple(listed)}, planes {tuple(plane)} and "
                           f"{tuple(v_plane.shape)} for {heads} over {kv_heads} heads of {head_dim}, or tensors on different devices")
-    p = _PAGES_LAYOUT.pack(q.data_ptr(), row_stride, out.data_ptr(), out_stride, k_plane.data_ptr(), v_plane.data_ptr(), 0, block_table.data_ptr(),
-                           table[1], seq_slot.data_ptr(), seq_q_start.data_ptr(), seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, heads, kv_heads,
-                           head_dim, max_q_len, scale, pages.data_ptr(), listed[2], 0, 0, 0, plane[0], table[0], rows)
-    _check(_lib.gb_attention_pages(p, _code(dtype), _pages_stream("attention_pages", dev)))
+    _pages_call("attention_pages", _lib.gb_attention_pages, _PAGES_LAYOUT.pack(
+        q.data_ptr(), row_stride, out.data_ptr(), out_stride, k_plane.data_ptr(), v_plane.data_ptr(), 0, block_table.data_ptr(), table[1],
+        seq_slot.data_ptr(), seq_q_start.data_ptr(), seq_q_len.data_ptr(), seq_kv_len.data_ptr(), nseq, heads, kv_heads, head_dim, max_q_len, scale,
+        pages.data_ptr(), listed[2], 0, 0, 0, plane[0], table[0], rows), dtype, dev)
 
 
 # ---- mixers with a matrix state ------------------------------------------------------------
