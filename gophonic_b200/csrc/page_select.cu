@@ -525,10 +525,11 @@ struct Chooser {
 // Single rows ----------------------------------------------------------------------------------
 // A cluster of CTAs scores one (row, kv head): each takes a stretch of the pages and leaves their scores in the first one's shared
 // memory, which then chooses.  A page's 2 d bounds are 16-byte chunks, LP lanes share them, CPL chunks a lane, and hold their
-// coefficients in registers; a warp asks for eight chunks a lane before it adds anything up.
+// coefficients in registers.
 constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int MAX_PIECES = 8;
 constexpr int ROW_BAND = 512;
+constexpr int RING_CHUNKS = 8;      // 16-byte chunks a lane asks for with one batch: 4 KB a warp
 
 struct SelectSmem {
     union {
@@ -560,7 +561,7 @@ __device__ __forceinline__ float sum_many(float (&v)[N], int lane) {
 }
 
 template <typename T, int LP, int CPL>
-__global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __grid_constant__ PagesParams p, int longest_first) {
+__global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __grid_constant__ PagesParams p, int longest_first, int depth) {
     constexpr int E = Chunk<T>::E, U = 8 / CPL, PER_WARP = 32 / LP;     // pages a group of LP lanes takes at a time
     extern __shared__ __align__(16) unsigned char raw[];
     SelectSmem& s = *reinterpret_cast<SelectSmem*>(raw);
@@ -598,22 +599,29 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __g
     constexpr int BATCH = U * PER_WARP;
     const int first_batch = (piece * SELECT_WARPS + warp) * BATCH, step = pieces * SELECT_WARPS * BATCH;
     const T* plane = (const T*)p.bounds;
-    // A lane's page of the batch at i; the numbers are asked for a batch ahead of the bounds, the bounds a batch ahead of their sums.
+    // A lane's page of the batch at i: the numbers are asked for a batch ahead of the bounds.  The bounds of `depth` (two or three)
+    // batches are on their way by cp.async, each lane's chunks into places of its own that only it reads.
     auto page_for = [&](int i) -> int { return lane < BATCH && i + lane < r.nc ? (int)page_of(r.bt, (r.c0 + i + lane) * GB_PAGE, p.bt_stride, p.pages) : 0; };
-    auto ask = [&](int i, int page, uint4 (&x)[U][CPL]) {
+    uint4* ring = reinterpret_cast<uint4*>(raw + ((sizeof(SelectSmem) + (size_t)p.bt_stride * sizeof(uint32_t) + 15) & ~(size_t)15)) + warp * depth * RING_CHUNKS * 32 + lane;
+    auto ask = [&](int i, int page, int slot) {
+        if (i < r.nc)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int at = min(sub * U + u, r.nc - 1 - i);     // pages beyond the last are the last once more
-            const int64_t pg = __shfl_sync(0xffffffffu, page, at);
-            const uint4* b = reinterpret_cast<const uint4*>(plane + (pg * p.kv_heads + r.kvh) * d2);
+            for (int u = 0; u < U; u++) {
+                const int at = min(sub * U + u, r.nc - 1 - i);     // pages beyond the last are the last once more
+                const int64_t pg = __shfl_sync(0xffffffffu, page, at);
+                const T* b = plane + (pg * p.kv_heads + r.kvh) * d2;
 #pragma unroll
-            for (int j = 0; j < CPL; j++) x[u][j] = l + j * LP < NC ? b[l + j * LP] : make_uint4(0, 0, 0, 0);
-        }
+                for (int j = 0; j < CPL; j++)
+                    if (l + j * LP < NC) cp_async16(ring + (slot * RING_CHUNKS + u * CPL + j) * 32, b + (l + j * LP) * E, 16);
+            }
+        cp_async_commit();
     };
-    uint4 now[U][CPL];
     int next = page_for(first_batch);
-    if (first_batch < r.nc) ask(first_batch, next, now);
-    next = page_for(first_batch + step);
+    for (int s0 = 0; s0 < depth; s0++) {
+        const int page = next;
+        next = page_for(first_batch + (s0 + 1) * step);
+        ask(first_batch + s0 * step, page, s0);
+    }
     for (int c = tid; c < p.d; c += SELECT_THREADS) {
         float up = 0.f, down = 0.f;
 #pragma unroll 4
@@ -637,18 +645,18 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __g
         }
     uint32_t* keys0 = cluster.map_shared_rank(key, 0);
     bool odd = false;
+    int slot = 0;
     for (int i0 = first_batch; i0 < r.nc; i0 += step) {
-        uint4 then[U][CPL];
-        if (i0 + step < r.nc) ask(i0 + step, next, then);
-        next = page_for(i0 + 2 * step);
+        if (depth == 3) cp_async_wait<2>(); else cp_async_wait<1>();      // this batch has landed
         float acc[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             acc[u] = 0.f;
 #pragma unroll
             for (int j = 0; j < CPL; j++) {
+                if (l + j * LP >= NC) break;
                 float f[E];
-                unpack(now[u][j], f);
+                unpack(ring[(slot * RING_CHUNKS + u * CPL + j) * 32], f);
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     acc[u] = fmaf(cf[j][e], f[e], acc[u]);
@@ -656,16 +664,17 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __g
                 }
             }
         }
+        const int page = next;
+        next = page_for(i0 + (depth + 1) * step);
+        ask(i0 + depth * step, page, slot);
+        slot = slot + 1 == depth ? 0 : slot + 1;
         const float sum = sum_many<U, LP>(acc, lane);
         constexpr int SHARE = LP / U;                     // lanes that end with the same page
         const int i = i0 + sub * U + l / SHARE;
         odd = odd || !(fabsf(sum) <= 3.0e38f);
         if (l % SHARE == 0 && i < r.nc) keys0[i] = order_key(sum);
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < CPL; j++) now[u][j] = then[u][j];
     }
+    cp_async_wait<0>();
     float most = 0.f;      // the sum of the terms' sizes is no more than that of the coefficients times the channels' largest bounds
 #pragma unroll
     for (int j = 0; j < CPL; j++)
@@ -939,7 +948,7 @@ GB_API int gb_page_bounds(const PagesParams* pp, int dtype, cudaStream_t stream)
 template <typename T, int LP, int CPL>
 static int launch_rows(const PagesParams& p, cudaStream_t stream) {
     static bool done[64];
-    const cudaError_t e = gb_allow_smem(select_row_kernel<T, LP, CPL>, (int)(sizeof(SelectSmem) + MAX_PAGES * sizeof(uint32_t)), done);
+    const cudaError_t e = gb_allow_smem(select_row_kernel<T, LP, CPL>, MAX_TILE_SMEM, done);
     if (e != cudaSuccess) GB_REFUSE("select_pages: cannot reserve shared memory: %s", cudaGetErrorString(e));
     // pieces of no fewer pages than the CTA's warps take at a time, while they all run at once
     const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads;
@@ -947,8 +956,11 @@ static int launch_rows(const PagesParams& p, cudaStream_t stream) {
     while (pieces < MAX_PIECES && units * pieces * 2 <= 4 * gb_sm_count() && p.bt_stride > pieces * SELECT_WARPS * 8) pieces *= 2;
     if (units * pieces > 0x7fffffff) GB_REFUSE("select_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
     const int longest_first = pieces == 1 && p.max_q_len == 1 && p.nseq <= 512 && units > gb_sm_count();    // (the lengths stand where the coefficients will)
-    launch_pdl_cluster(select_row_kernel<T, LP, CPL>, dim3((unsigned)(units * pieces)), dim3(SELECT_THREADS), sizeof(SelectSmem) + (size_t)p.bt_stride * sizeof(uint32_t),
-                       stream, pieces, 1, p, longest_first);
+    // batches in flight: three, or two beside the scores of more than some 31000 pages
+    const size_t scores = (sizeof(SelectSmem) + (size_t)p.bt_stride * sizeof(uint32_t) + 15) & ~(size_t)15, batch = SELECT_WARPS * RING_CHUNKS * 512;
+    const int depth = scores + 3 * batch <= (size_t)MAX_TILE_SMEM ? 3 : 2;
+    launch_pdl_cluster(select_row_kernel<T, LP, CPL>, dim3((unsigned)(units * pieces)), dim3(SELECT_THREADS), scores + depth * batch, stream, pieces, 1, p, longest_first,
+                       depth);
     GB_CHECK_LAUNCH("select_pages");
     return 0;
 }
