@@ -32,14 +32,17 @@ constexpr int MAX_TOP = 1024;     // entries of a list
 // key heads, one sequence of 16 rows 13 / 18, of 32 rows 18 / 19, of 48 rows 28 / 21.
 constexpr int TC5_MIN_UNITS = 64;
 
-// The row's listed pages that it can see, in the list's order, packed into `to`; how many there are.  Every thread of the CTA.
-__device__ __forceinline__ int pack_list(const PagesParams& p, const int* list, int own_page, int* to, int* counts) {
+// The row's listed pages that it can see, in the list's order, packed into `to`, and behind them (from to[p.top] on) where they are in
+// the planes; how many there are.  Every thread of the CTA.  (Looked up page by page, the block table's latency stood ahead of
+// every page's copies: some 600 cycles of 2000.)
+__device__ __forceinline__ int pack_list(const PagesParams& p, const int* bt, const int* list, int own_page, int* to, int* counts) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int n = 0;
     for (int base = 0; base < p.top; base += THREADS) {
         const int i = base + tid;
         const int lp = i < p.top ? list[i] : -1;
         const bool ok = lp >= 0 && lp <= own_page && lp < p.bt_stride;
+        const int place = ok ? (int)page_of(bt, lp * GB_PAGE, p.bt_stride, p.pages) : 0;
         const unsigned who = __ballot_sync(0xffffffffu, ok);
         if (lane == 0) counts[warp] = __popc(who);
         __syncthreads();
@@ -48,7 +51,10 @@ __device__ __forceinline__ int pack_list(const PagesParams& p, const int* list, 
             if (w < warp) at += counts[w];
             n += counts[w];
         }
-        if (ok) to[at] = lp;
+        if (ok) {
+            to[at] = lp;
+            to[p.top + at] = place;
+        }
         __syncthreads();
     }
     return n;
@@ -147,7 +153,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
     extern __shared__ __align__(16) unsigned char raw[];
     bf16* Qs = reinterpret_cast<bf16*>(raw);       // [16][SD]
     bf16* KV = Qs + 16 * SD;                       // [STAGES][2][64][SD]
-    int* pages = reinterpret_cast<int*>(KV + STAGES * STAGE);   // [top]
+    int* pages = reinterpret_cast<int*>(KV + STAGES * STAGE);   // [2][top]: their numbers, their places
     __shared__ int counts[THREADS / 32];
     __shared__ alignas(8) float ml[16][2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -165,13 +171,13 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
         }
         cp_async_commit();
     }
-    const int n_all = pack_list(p, p.list + ((int64_t)at.row * p.kv_heads + at.kvh) * p.top, at.pos / GB_PAGE, pages, counts);
+    const int n_all = pack_list(p, at.bt, p.list + ((int64_t)at.row * p.kv_heads + at.kvh) * p.top, at.pos / GB_PAGE, pages, counts);
     const int lo = (int)((int64_t)n_all * piece / pieces), n = (int)((int64_t)n_all * (piece + 1) / pieces) - lo;
 
     const bf16* kbase = (const bf16*)p.k_plane;
     const bf16* vbase = (const bf16*)p.v_plane;
     auto load_tile = [&](int i) {
-        const int64_t off = (page_of(at.bt, pages[lo + i] * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + at.kvh) * (int64_t)(GB_PAGE * HD);
+        const int64_t off = ((int64_t)pages[p.top + lo + i] * p.kv_heads + at.kvh) * (GB_PAGE * HD);
         bf16* st = KV + (i % STAGES) * STAGE;
         for (int idx = tid; idx < 64 * CH; idx += THREADS) {
             const int r = idx / CH, c = idx - r * CH;
@@ -364,18 +370,18 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
         ml[tid][0] = -INFINITY;
         ml[tid][1] = 0.f;
     }
-    const int n_all = pack_list(p, p.list + ((int64_t)at.row * p.kv_heads + at.kvh) * p.top, at.pos / GB_PAGE, pages, counts);
+    const int n_all = pack_list(p, at.bt, p.list + ((int64_t)at.row * p.kv_heads + at.kvh) * p.top, at.pos / GB_PAGE, pages, counts);
     const int lo = (int)((int64_t)n_all * piece / pieces), n = 2 * ((int)((int64_t)n_all * (piece + 1) / pieces) - lo);   // half pages
     const int CH = d / 4;
     auto load_tile = [&](int i) {
-        const int64_t off = ((page_of(at.bt, pages[lo + i / 2] * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + at.kvh) * GB_PAGE + (i & 1) * F_KEYS) * (int64_t)d;
+        const int64_t off = (((int64_t)pages[p.top + lo + i / 2] * p.kv_heads + at.kvh) * GB_PAGE + (i & 1) * F_KEYS) * d;
         const float *k = (const float*)p.k_plane + off, *v = (const float*)p.v_plane + off;
         float* st = KV + (i % F_STAGES) * f32_stage(d);
-        for (int idx = tid; idx < F_KEYS * CH; idx += THREADS) {
-            const int r = idx / CH, c = (idx - r * CH) * 4;
-            cp_async16(st + r * sd + c, k + (int64_t)r * d + c, 16);
-            cp_async16(st + F_KEYS * sd + r * d + c, v + (int64_t)r * d + c, 16);
-        }
+        for (int r = warp; r < F_KEYS; r += THREADS / 32)      // a warp a key
+            for (int c = lane * 4; c < d; c += 128) {
+                cp_async16(st + r * sd + c, k + r * d + c, 16);
+                cp_async16(st + F_KEYS * sd + r * d + c, v + r * d + c, 16);
+            }
     };
 #pragma unroll
     for (int s = 0; s < F_STAGES - 1; s++) {
@@ -528,20 +534,20 @@ int launch_mma(const PagesParams& p, cudaStream_t stream) {
     static_assert(base >= (128 + 64 * HD) * 4 + 16 * SD * 2, "the warps' results fit where the pages were");
     static int known[64];
     int wide = 0;
-    if (int rc = configure(attn_pages_mma_kernel<HD>, base + MAX_TOP * 4, known, wide)) return rc;
+    if (int rc = configure(attn_pages_mma_kernel<HD>, base + MAX_TOP * 8, known, wide)) return rc;
     const int G = p.heads / p.kv_heads, chunks = (G + 15) / 16;
-    return launch(attn_pages_mma_kernel<HD>, p, chunks, pieces_for(p, chunks, HD <= 128 ? 2 : 1, wide), base + p.top * 4, stream);
+    return launch(attn_pages_mma_kernel<HD>, p, chunks, pieces_for(p, chunks, HD <= 128 ? 2 : 1, wide), base + p.top * 8, stream);
 }
 
 template <int NH>
 int launch_f32(const PagesParams& p, cudaStream_t stream) {
     static int known[64];
     int wide = 0;
-    constexpr int most = f32_floats(256, NH) * 4 + MAX_TOP * 4;
+    constexpr int most = f32_floats(256, NH) * 4 + MAX_TOP * 8;
     static_assert(most <= 231000, "the widest heads' stages fit");
     if (int rc = configure(attn_pages_f32_kernel<NH>, most, known, wide)) return rc;
     const int G = p.heads / p.kv_heads, chunks = (G + NH - 1) / NH;
-    return launch(attn_pages_f32_kernel<NH>, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1, wide), f32_floats(p.d, NH) * 4 + p.top * 4, stream);
+    return launch(attn_pages_f32_kernel<NH>, p, chunks, pieces_for(p, chunks, p.d <= 128 ? 2 : 1, wide), f32_floats(p.d, NH) * 4 + p.top * 8, stream);
 }
 
 }  // namespace

@@ -339,8 +339,11 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
             const bool keys = warp == 0;
             uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
             int issued = 0;
+            auto row_of = [&](int j) { return j < n ? ((int)page_of(bt, entry[j] * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * BKV : 0; };
+            int next = row_of(0);      // looked up a page ahead
             for (int j = 0; j < n; j++) {
-                const int s = j % STAGES;
+                const int s = j % STAGES, row = next;
+                next = row_of(j + 1);
                 if (!mbar_wait_relaxed(&empty[s], ((uint32_t)(j / STAGES) & 1u) ^ 1u)) {
                     atomicCAS(&g_status, 0, 1);
                     abort_s = 1;
@@ -348,7 +351,6 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
                 if (*(volatile int*)&abort_s) break;
                 mbar_expect_tx(&full[s], K_BYTES);
                 unsigned char* to = KVs + (size_t)s * STAGE_BYTES + (keys ? 0 : K_BYTES);
-                const int row = ((int)page_of(bt, entry[j] * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * BKV;
 #pragma unroll
                 for (int h = 0; h < 2; h++) tma_load_2d(to + h * KPANEL, keys ? &map_k : &map_v, h * 64, row, &full[s]);
                 issued = j + 1;

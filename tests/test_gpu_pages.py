@@ -415,6 +415,27 @@ def test_attention_pages_runs_beside_values_that_are_not_finite(ops, heads, kvh,
     assert got[~sees].isfinite().all() and ops.tc5_status() == 0
 
 
+@pytest.mark.parametrize("width", [4000, 31500, 32768])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=names)
+def test_wide_block_tables(ops, dtype, width):
+    """Sequences that could be millions of tokens long: what stands in shared memory goes by the table's width."""
+    for seqs in ([(1500, 1), (90, 1)], [(1500, 40), (90, 1)]):
+        held = max(-(-(a + b) // PAGE) for a, b in seqs)
+        s = Step(seqs, 8, 4, 128, dtype, seed=9, room=width - held)
+        bounds = s.bounds_plane()
+        pages = s.select(ops, bounds, 9)
+        check_selection(s, pages, bounds, 9, 1, 2)
+        check_attention(s, s.attend(ops, pages), pages, rows={0, 1, 20, s.rows - 1})
+
+
+def test_attention_pages_behind_tables_too_wide_to_select_from(ops):
+    s = Step([(900, 30)], 4, 4, 128, BF, seed=9, room=40000)
+    pages = like_lists(s, 8, 5, 12, 9)
+    check_attention(s, s.attend(ops, pages.to(DEV)), pages, rows={0, 7, 29})
+    with pytest.raises(ops.KernelError):
+        s.select(ops, s.bounds_plane(), 8)
+
+
 # ---- the three together ------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,heads,kvh,d", [(BF, 8, 2, 128), (BF, 6, 3, 32), (F32, 8, 2, 64)], ids=names)
 def test_a_sequence_in_steps(ops, dtype, heads, kvh, d):

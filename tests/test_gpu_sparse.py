@@ -59,21 +59,21 @@ def close(got, ref):
 
 
 @pytest.mark.parametrize("name", ["A", "B", "D", "F"])
-@pytest.mark.parametrize("prompts", [False, True])
-def test_against_the_plain_model(engine, plain_models, monkeypatch, name, prompts):
-    """A prompt, then tokens one by one past several page borders; in float32, where no selection is near enough a tie to flip."""
+@pytest.mark.parametrize("prompts,n", [(False, 250), (True, 250), (False, 100)])
+def test_against_the_plain_model(engine, plain_models, monkeypatch, name, prompts, n):
+    """A prompt, then tokens one by one past several page borders, also past the one from which on they select; in float32, where no
+    selection is near enough a tie to flip."""
     eng = engine(name, "float32", 3, prompts=prompts)
     sel = eng.model.spec.layers[0].mixer.selection
     toks = ids(name, 319, 5)
-    n = 250
     cfg, w = plain_models[name]
     monkeypatch.setattr(P, "causal_attention", plain_attention(sel, 0 if prompts else n))
     ref = P.forward_logits(toks, cfg, w)
     slot = eng.new_sequence()
-    got = [eng.step([(slot, toks[:n])], [[0, 200, n - 1]])]
+    got = [eng.step([(slot, toks[:n])], [[0, n // 2, n - 1]])]
     got += [eng.step([(slot, [t])]) for t in toks[n:]]
     eng.end_sequence(slot)
-    assert close(torch.cat(got), np.concatenate((ref[[0, 200, n - 1]], ref[n:])))
+    assert close(torch.cat(got), np.concatenate((ref[[0, n // 2, n - 1]], ref[n:])))
     monkeypatch.setattr(P, "causal_attention", FULL)
     assert not close(torch.cat(got[1:]), P.forward_logits(toks, cfg, w)[n:])       # the selection shows
 
