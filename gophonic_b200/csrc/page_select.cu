@@ -533,8 +533,8 @@ constexpr int RING_CHUNKS = 8;      // 16-byte chunks a lane asks for with one b
 
 struct SelectSmem {
     union {
-        Chooser<SELECT_WARPS, ROW_BAND, 16, 16> all;
-        Chooser<1, ROW_BAND, 16, 32> one;       // up to 1024 candidates: no barriers between the steps of the search
+        Chooser<SELECT_WARPS, ROW_BAND, 4, 16> all;
+        Chooser<1, ROW_BAND, 16, 16> one;       // up to 32 wanted of 512: no barriers between the steps of the search
     } choose;
     float coef[2 * 256];                        // [N | P], in the order of a page's bounds
     float err[MAX_PIECES * SELECT_WARPS];       // of every warp of the cluster; a NaN: unsafe
@@ -616,12 +616,13 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __g
             }
         cp_async_commit();
     };
-    int next = page_for(first_batch);
-    for (int s0 = 0; s0 < depth; s0++) {
-        const int page = next;
-        next = page_for(first_batch + (s0 + 1) * step);
-        ask(first_batch + s0 * step, page, s0);
-    }
+    int early[3];
+#pragma unroll
+    for (int s0 = 0; s0 < 3; s0++) early[s0] = page_for(first_batch + s0 * step);
+    int next = depth == 3 ? page_for(first_batch + 3 * step) : early[2];
+#pragma unroll
+    for (int s0 = 0; s0 < 3; s0++)
+        if (s0 < depth) ask(first_batch + s0 * step, early[s0], s0);
     for (int c = tid; c < p.d; c += SELECT_THREADS) {
         float up = 0.f, down = 0.f;
 #pragma unroll 4
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_row_kernel(const __g
     // A float32 sum of at most 16 products a lane and 5 steps between lanes, of coefficients that are sums of G values: 22 + G half steps
     // of 2^-23 relative to the sum of the terms' sizes, itself known to 2^-18; products below the normal range add next to nothing.
     err = err * ((24.f + (float)G) * 5.9604645e-8f) + 1.0e-42f;
-    if (r.nc > 1024)
+    if (r.nc > 512 || r.k > 32)
         s.choose.all.run(p, r, key, err, unsafe, tid);
     else if (warp == 0)
         s.choose.one.run(p, r, key, err, unsafe, lane);

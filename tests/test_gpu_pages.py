@@ -185,6 +185,16 @@ def test_select_pages_long(ops, dtype, new, pages):
     check_selection(s, s.select(ops, bounds, 33), bounds, 33, 1, 2)
 
 
+@pytest.mark.parametrize("dtype,pages,top", [(BF, 4600, 33), (F32, 4600, 90), (BF, 600, 90), (F32, 1000, 70), (BF, 4600, 4500)], ids=names)
+def test_select_pages_by_all_warps(ops, dtype, pages, top):
+    """Candidates in a few registers a thread, in many, and from shared memory; more wanted than a warp has lanes."""
+    s = wide_step(dtype, pages, d=16)
+    bounds = s.bounds_plane()
+    check_selection(s, s.select(ops, bounds, top), bounds, top, 1, 2)
+    bounds[s.table[s.slots[0]].long()] = bounds[s.table[s.slots[0], 3].long()].clone()
+    check_selection(s, s.select(ops, bounds, top), bounds, top, 1, 2)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32], ids=names)
 @pytest.mark.parametrize("equal", [True, False])
 def test_select_pages_of_many_sequences(ops, dtype, equal):
