@@ -475,8 +475,9 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
 }
 
 // Into how many pieces a row's list is cut: the CTAs of a cluster, a power of two (sixteen where the GPU holds all of the clusters).  As many as run at once (one token over eight key heads, 32 pages:
-// 34 us in one piece, 19 in two, 12 in four, 8.4 in eight); where not even two pieces each do, two if their waves end sooner than
-// those of whole rows (50 sequences over eight key heads, 64 pages: 173 us in one piece, 147 in two, 158 in four, 197 in eight).
+// 34 us in one piece, 19 in two, 12 in four, 8.4 in eight, 8.1 in sixteen); where not even two pieces each do, two if their waves end sooner than
+// those of whole rows (50 sequences over eight key heads, 64 pages: 173 us in one piece, 147 in two, 158 in four, 197 in eight;
+// 139 in two since a list's places are looked up at once).
 int pieces_for(const PagesParams& p, int chunks, int per_sm, int wide) {
     const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads * chunks;
     int pieces = 1;

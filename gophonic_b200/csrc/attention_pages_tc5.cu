@@ -47,7 +47,7 @@ constexpr int Q_BYTES = 2 * QPANEL, K_BYTES = 2 * KPANEL, V_BYTES = 2 * KPANEL, 
 constexpr int ROWS = 128, STAGES = 2;
 constexpr int FIRST_SOFTMAX_WARP = 3, VALUE_LOADER_WARP = FIRST_SOFTMAX_WARP + 4, WARPS = VALUE_LOADER_WARP + 1, THREADS = WARPS * 32;
 constexpr int TILE_BYTES = Q_BYTES + STAGES * STAGE_BYTES;
-constexpr int LIST_BYTES = 232448 - 3072 - 1024 - TILE_BYTES;   // most for the tile's pages and their bits, beside the static part and the alignment
+constexpr int LIST_BYTES = 232448 - 4 * 1024 - TILE_BYTES;   // most for the tile's pages and their bits, beside the static part and the alignment
 constexpr int TMEM_COLS = 256, O_COL = 128;                     // two buffers of 64 columns for S, then O
 static_assert(ROWS * HD * 4 <= STAGES * STAGE_BYTES, "a tile's sums fit where the pages were");
 constexpr int MAX_TABLE = 32768;                // pages of a sequence: their bitmap is made where the pages will go
