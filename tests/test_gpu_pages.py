@@ -502,6 +502,42 @@ def test_captured_on_another_stream_and_repeated(ops, dtype):
             assert torch.equal(pages, got[0]) and torch.equal(out, got[1])
 
 
+def test_two_streams_at_once(ops):
+    """Calls that overlap share nothing: runs, single tokens and float32 beside one another give what they give alone."""
+    steps = [Step([(2000, 300)], 8, 2, 128, BF, seed=1), Step([(3000, 1), (500, 1)], 8, 2, 128, BF, seed=2), Step([(1500, 20)], 4, 2, 64, F32, seed=3)]
+    alone = []
+    for s in steps:
+        pages = s.select(ops, s.bounds_plane(), 8)
+        alone.append((pages, s.attend(ops, pages)))
+    bounds = [s.bounds_plane().to(DEV) for s in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s, b, stream in zip(steps, bounds, streams):
+            with torch.cuda.stream(stream):
+                pages = s.select(ops, b, 8)
+                got.append((pages, s.attend(ops, pages)))
+        torch.cuda.synchronize()
+        for (p0, o0), (p1, o1) in zip(alone, got):
+            assert torch.equal(p0, p1) and torch.equal(o0, o1)
+
+
+def test_sequences_that_bring_nothing(ops):
+    """A padded batch: sequences of no rows between others."""
+    s = Step([(700, 3), (300, 0), (0, 0), (500, 40)], 4, 2, 128, BF, seed=4, more_rows=2)
+    bounds = s.bounds_plane()
+    out_bounds = torch.full((s.n_pages, 2, 2, 128), 5.0, dtype=BF, device=DEV)
+    slot, _, q_len, kv_len = s.seq
+    ops.page_bounds(s.dev["k_plane"], out_bounds, s.dev["table"], slot, q_len, kv_len, 4, 40)
+    done = int(s.table[s.slots[3], 7])
+    assert torch.equal(out_bounds[done].cpu(), bounds[done]) and int((out_bounds != 5.0).flatten(1).any(1).sum()) == 1
+    pages = s.select(ops, bounds, 5)
+    check_selection(s, pages, bounds, 5, 1, 2)
+    check_attention(s, s.attend(ops, pages), pages)
+    assert (pages[s.rows:] == -7).all()
+
+
 # ---- refusals ----------------------------------------------------------------------------------
 def test_refusals(ops):
     s = Step([(100, 1)], 4, 2, 64, BF)
