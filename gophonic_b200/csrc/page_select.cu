@@ -5,8 +5,8 @@
 // For a query q no key of the page can score more than sum_c max(q_c lo_c, q_c hi_c).  select_pages takes that bound, summed over
 // the G query heads that share a key head, as the page's score:
 //     s = sum_h sum_c max(q_hc lo_c, q_hc hi_c) = sum_c (P_c hi_c + N_c lo_c),   P = sum_h max(q_h, 0), N = sum_h min(q_h, 0),
-// (a head takes hi where q > 0 and lo where q < 0), one product of 2 d channels a page whatever G is, and chooses for every (row, key head) the first `first` pages, the last
-// `last` up to the row's own, and of the others those that score highest, `top` in all.
+// (a head takes hi where q > 0 and lo where q < 0), one product of 2 d channels a page whatever G is, and chooses for every (row,
+// key head) the first `first` pages, the last `last` up to the row's own, and of the others those that score highest, `top` in all.
 //
 // The choice is the one of 64-bit arithmetic.  Scores are float32 sums with a bound e on their error; with tau the k-th highest
 // of them, a page above tau + 2 e is among the k best and one below tau - 2 e is not, whatever the errors were, and only the
