@@ -54,116 +54,6 @@ constexpr int TMEM_COLS = 512;                  // S: 2 groups x 2 buffers x 64;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_AT = 8.0f;              // rescale O when the row maximum outgrew the scale by 2^8
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(s32(bar)) : "memory");
-}
-
-// MN-major operand (values: rows are keys, 128-byte rows of 64 head elements, the second half of
-// the head one panel further): leading byte offset = panel, stride byte offset = 8 rows.
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
-    d |= (uint64_t)(KPANEL >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-
-// D (+)= A B with A in tensor memory (128 lanes, two bfloat16 a column) and B from shared memory
-__device__ __forceinline__ void umma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-        "}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Packed pairs of fp32 (one instruction works on two values) and the three-input maximum: the
-// softmax warps set the pace of the kernel, so their instruction count matters.
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2_down(uint64_t a, uint64_t b) {  // rounded towards minus infinity
-    uint64_t d;
-    asm("add.rm.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
-// 2^x of two values on the FMA pipe alone, for the share of the exponentials that the
-// special-function unit (16 a clock and SM) has no time for: x = n + f with n = floor(x) taken by
-// adding 1.5 * 2^23 rounded down, 2^f by a cubic (relative error 1.9e-4, a twentieth of the
-// bfloat16 step the probabilities are rounded to), and n added into the exponent field.
-__device__ __forceinline__ void exp2_poly_x2(float x0, float x1, float& y0, float& y1) {
-    x0 = fmaxf(x0, -126.f);
-    x1 = fmaxf(x1, -126.f);
-    const uint64_t x = pack2(x0, x1);
-    const uint64_t r = add2_down(x, pack2(12582912.f, 12582912.f));
-    const uint64_t n = add2(r, pack2(-12582912.f, -12582912.f));
-    const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
-    uint64_t q = fma2(f, pack2(0.0790199414f, 0.0790199414f), pack2(0.2241264433f, 0.2241264433f));
-    q = fma2(q, f, pack2(0.6968385577f, 0.6968385577f));
-    q = fma2(q, f, pack2(0.9998119473f, 0.9998119473f));
-    float q0, q1, r0, r1;
-    unpack2(q, q0, q1);
-    unpack2(r, r0, r1);
-    y0 = __int_as_float(__float_as_int(q0) + (__float_as_int(r0) << 23));
-    y1 = __int_as_float(__float_as_int(q1) + (__float_as_int(r1) << 23));
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-        "r"(r[31])
-        : "memory");
-    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-}
-
-// 32 columns of this thread's lane without waiting for them (pair with tmem_wait_ld)
-__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
 // What the form over expanded latents takes besides.
 struct LatentRows {
@@ -392,7 +282,7 @@ __device__ __forceinline__ void prefill_tc5(const CUtensorMap& map_q, const CUte
                 const uint32_t idesc_pv = instr_desc(BQ, HD) | (1u << 16);  // values enter MN-major
                 uint64_t v_desc[STAGES];
 #pragma unroll
-                for (int s = 0; s < STAGES; s++) v_desc[s] = smem_desc_mn(s32(KVs + (size_t)s * STAGE_BYTES + K_BYTES));
+                for (int s = 0; s < STAGES; s++) v_desc[s] = smem_desc_mn(s32(KVs + (size_t)s * STAGE_BYTES + K_BYTES), KPANEL);
                 for (int j = 0; j < n && ok; j++) {
                     ok = need_page(j);
                     if (ok && j < my_n) {
@@ -513,14 +403,15 @@ __device__ __forceinline__ void prefill_tc5(const CUtensorMap& map_q, const CUte
                     const int i = (c & 3) * 8 + e * 2;
                     const uint32_t a = c < 4 ? v0[i] : v1[i], bb = c < 4 ? v0[i + 1] : v1[i + 1];
                     float t0, t1, p0, p1;
-                    unpack2(fma2(pack2(__uint_as_float(a), __uint_as_float(bb)), sc2, nmb2), t0, t1);
+                    const uint64_t t = fma2(pack2(__uint_as_float(a), __uint_as_float(bb)), sc2, nmb2);
+                    unpack2(t, t0, t1);
                     if (sig) {      // a masked key (-inf) weighs nothing
                         asm("tanh.approx.f32 %0, %1;" : "=f"(p0) : "f"(t0));
                         asm("tanh.approx.f32 %0, %1;" : "=f"(p1) : "f"(t1));
                         p0 = a == 0xff800000u ? 0.f : fmaf(p0, 0.5f, 0.5f);
                         p1 = bb == 0xff800000u ? 0.f : fmaf(p1, 0.5f, 0.5f);
                     } else if (e < F::POLY_PAIRS) {
-                        exp2_poly_x2(t0, t1, p0, p1);
+                        exp2_poly_x2(t, p0, p1);
                     } else {
                         p0 = fast_exp2(t0);
                         p1 = fast_exp2(t1);

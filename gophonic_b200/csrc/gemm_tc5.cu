@@ -31,11 +31,6 @@ constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTE
 constexpr int TMEM_COLS = 512;  // two accumulators of 256 columns
 constexpr int THREADS = 192;
 
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(s32(bar)) : "memory");
-}
-
 // Stores 32 accumulator columns (n0c .. n0c + 31 of the product) of row `row`: plain, or through the
 // SwiGLU epilogue, where columns alternate in blocks of eight between gate and up outputs.
 template <typename TC>
