@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
                 }
                 if (grow) m_used = m_run;
                 const float mbase = m_used == -INFINITY ? 0.f : m_used;
-                // a row that does not list the page: 2^-inf, which is 0 (2^-126 where the polynomial has it, of which its sum takes
-                // nothing); a NaN score makes its sums NaN, and they are made anew
+                // a row that does not list the page: 2^-inf, which is 0; a score of it that is not finite makes the row's sums NaN, and
+                // they are made anew
                 const uint64_t sc2 = mine ? pack2(sc, sc) : pack2(0.f, 0.f), nmb2 = mine ? pack2(-mbase, -mbase) : pack2(-INFINITY, -INFINITY);
 #pragma unroll
                 for (int c = 0; c < 32; c++) {
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
                     const uint64_t t = fma2(pack2(__uint_as_float(a), __uint_as_float(bb)), sc2, nmb2);
                     float p0, p1;
                     if (c % 4 == 3) {
-                        exp2_poly_x2(t, p0, p1);
+                        unpack2(exp2_poly_x2(t), p0, p1);
                     } else {
                         unpack2(t, p0, p1);
                         p0 = fast_exp2(p0);

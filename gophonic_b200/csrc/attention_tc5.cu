@@ -411,7 +411,7 @@ __device__ __forceinline__ void prefill_tc5(const CUtensorMap& map_q, const CUte
                         p0 = a == 0xff800000u ? 0.f : fmaf(p0, 0.5f, 0.5f);
                         p1 = bb == 0xff800000u ? 0.f : fmaf(p1, 0.5f, 0.5f);
                     } else if (e < F::POLY_PAIRS) {
-                        exp2_poly_x2(t, p0, p1);
+                        unpack2(exp2_poly_x2(t), p0, p1);
                     } else {
                         p0 = fast_exp2(t0);
                         p1 = fast_exp2(t1);

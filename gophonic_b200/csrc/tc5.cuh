@@ -203,15 +203,23 @@ __device__ __forceinline__ uint64_t add2_down(uint64_t a, uint64_t b) {  // roun
     asm("add.rm.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ uint64_t mul2_ftz(uint64_t a, uint64_t b) {  // what lies below 2^-126 is 0
+    uint64_t d;
+    asm("mul.rn.ftz.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 // 2^x of two values on the FMA pipe, for a quarter of the exponentials (the special-function unit takes eight cycles for a warp's):
 // x = n + f by adding 1.5 * 2^23 rounded down, 2^f by a cubic (relative error 1.9e-4, a twentieth of the bfloat16 step the
-// probabilities are rounded to), n added into the exponent field.
-__device__ __forceinline__ void exp2_poly_x2(uint64_t x, float& y0, float& y1) {
+// probabilities are rounded to), n added into the exponent field.  The field is kept 64 higher and brought back by a product that
+// flushes: like ex2.approx.ftz this gives 0 for all that lies below 2^-126, so that a weight of 2^-inf is none (2^-126, where the
+// clamp alone would leave it, times a value of 3e38 is 3.5).  x up to 60; a NaN gives 0.
+__device__ __forceinline__ uint64_t exp2_poly_x2(uint64_t x) {
+    constexpr float HIGHER = 12582912.f + 64.f;
     float x0, x1;
     unpack2(x, x0, x1);
-    x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-    const uint64_t r = add2_down(x, pack2(12582912.f, 12582912.f));
-    const uint64_t n = add2(r, pack2(-12582912.f, -12582912.f));
+    x = pack2(fmaxf(x0, -190.f), fmaxf(x1, -190.f));
+    const uint64_t r = add2_down(x, pack2(HIGHER, HIGHER));
+    const uint64_t n = add2(r, pack2(-HIGHER, -HIGHER));
     const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
     uint64_t q = fma2(f, pack2(0.0790199414f, 0.0790199414f), pack2(0.2241264433f, 0.2241264433f));
     q = fma2(q, f, pack2(0.6968385577f, 0.6968385577f));
@@ -219,8 +227,8 @@ __device__ __forceinline__ void exp2_poly_x2(uint64_t x, float& y0, float& y1) {
     float q0, q1, r0, r1;
     unpack2(q, q0, q1);
     unpack2(r, r0, r1);
-    y0 = __int_as_float(__float_as_int(q0) + (__float_as_int(r0) << 23));
-    y1 = __int_as_float(__float_as_int(q1) + (__float_as_int(r1) << 23));
+    const float y0 = __int_as_float(__float_as_int(q0) + (__float_as_int(r0) << 23)), y1 = __int_as_float(__float_as_int(q1) + (__float_as_int(r1) << 23));
+    return mul2_ftz(pack2(y0, y1), pack2(5.421010862427522e-20f, 5.421010862427522e-20f));      // 2^-64
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
