@@ -394,6 +394,8 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
             unpack2(sum2[1], sum[2], sum[3]);
             if (mine) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
+        // A score of +inf: the others' weights are all 0, and its own, inf - inf, is 0 too where the polynomial has it.
+        if (m_run == INFINITY) l = NAN;
         if (ok && n > 0 && !mbar_wait(&o_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u)) ok = false;
         if (!ok) {
             atomicCAS(&g_status, 0, 4);

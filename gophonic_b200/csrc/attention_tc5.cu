@@ -443,6 +443,8 @@ __device__ __forceinline__ void prefill_tc5(const CUtensorMap& map_q, const CUte
             // a sink adds one unit to the denominator: a key of score 0, in the scale the sums are kept in
             // (a sum so scaled that the unit overflows gives 1 / inf = 0, which is the limit)
             if (!sig && p.sink && m_used != -INFINITY) l += exp2f((p.sinks ? p.sinks[head] * LOG2E : 0.f) - m_used);
+            // a score of +inf: the others' weights are all 0, and its own, inf - inf, is 0 too where the polynomial has it
+            if (!sig && m_run == INFINITY) l = NAN;
             float inv = 1.f / l;
             if (sig) {
                 inv = 1.f;

@@ -1,5 +1,7 @@
 """Attention for runs of rows (over listed pages, and over the whole cache) beside values and scores at the edge of what the types hold:
 what a row does not see weighs nothing at all, and a score that is not finite shows."""
+import math
+
 import pytest
 import torch
 
@@ -28,7 +30,8 @@ def by_head(s, out):
     return out.cpu().float().reshape(out.shape[0], s.kvh, -1)
 
 
-FORMS = pytest.mark.parametrize("heads,kvh,new", [(4, 1, 150), (16, 8, 700)], ids=["shared tiles", "whole tiles"])
+# by how many CTAs share a tile: eight, three, none
+FORMS = pytest.mark.parametrize("heads,kvh,new", [(4, 1, 150), (16, 8, 700), (32, 8, 700)], ids=["eight", "three", "one"])
 
 
 # ---- what a row does not see -------------------------------------------------------------------
@@ -76,3 +79,70 @@ def test_unseen_values_near_the_largest_weigh_nothing_in_a_prompt(ops, window, s
     assert len(rows) >= 30
     got = attend_all(ops, s, window)
     assert torch.equal(got[rows], clean[rows]) and ops.tc5_status() == 0
+
+
+# ---- scores that are not finite ----------------------------------------------------------------
+def poisoned(s, keys, page, place, score):
+    """A copy of the key plane ``keys`` in which one key of a page scores ``score`` (+inf, -inf or NaN) for every row: their queries' first
+    channel is positive (``looks_up``)."""
+    k = keys.clone()
+    k[s.table[s.slots[0], page], :, place, 0] = score
+    return k
+
+
+def looks_up(s):
+    q = s.wide[:, :s.heads * s.d].view(-1, s.heads, s.d)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.25
+    s.q = s.wide[:, :s.heads * s.d].cpu()
+
+
+def check_places(ops, s, call, sees, clean, scores):
+    """``call(key plane)`` with one key poisoned at each place of page 3: rows that see it hold no finite number, the others are as they were up
+    to the rounding of their weights (a row that shares its tile may be made anew over its own keys)."""
+    keys = s.dev["k_plane"]
+    for place in range(PAGE):
+        for score in scores:
+            got = by_head(s, call(poisoned(s, keys, 3, place, score)))
+            see = sees(place)
+            assert see.any()
+            assert got[see].isnan().all(), (place, score)
+            assert got[~see].isfinite().all(), (place, score)
+            assert see.all() or float((got[~see] - clean[~see]).abs().max()) <= 4 * 2.0 ** -8 * float(s.v_plane.float().abs().max()), (place, score)
+    assert ops.tc5_status() == 0
+
+
+def check_listed(ops, heads, kvh, new, scores):
+    s = Step([(150, new)], heads, kvh, 128, BF, seed=2)
+    looks_up(s)
+    pages = like_lists(s, 5, 5, 12, 5)
+    pos = 150 + torch.arange(new).unsqueeze(1)
+    listed = (pages == 3).any(-1)
+    assert listed.any() and not listed.all()
+    clean = by_head(s, s.attend(ops, pages.to(DEV)))
+
+    def call(k):
+        s.dev["k_plane"] = k
+        return s.attend(ops, pages.to(DEV))
+    check_places(ops, s, call, lambda place: listed & (pos >= 3 * PAGE + place), clean, scores)
+
+
+def check_prompt(ops, scores):
+    s = Step([(150, 200)], 4, 2, 128, BF, seed=3)
+    looks_up(s)
+    clean = by_head(s, attend_all(ops, s))
+    pos = (150 + torch.arange(200)).unsqueeze(1).expand(200, 2)
+
+    def call(k):
+        s.dev["k_plane"] = k
+        return attend_all(ops, s)
+    check_places(ops, s, call, lambda place: pos >= 3 * PAGE + place, clean, scores)
+
+
+@FORMS
+def test_a_score_beyond_all_others_shows(ops, heads, kvh, new):
+    """A score of +inf makes the row's softmax inf / inf, at whichever place of its page the key stands."""
+    check_listed(ops, heads, kvh, new, [math.inf])
+
+
+def test_a_score_beyond_all_others_shows_in_a_prompt(ops):
+    check_prompt(ops, [math.inf])
