@@ -341,9 +341,9 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
 #pragma unroll
                 for (int e = 0; e < 32; e += 4)
 #pragma unroll
-                    for (int f = 0; f < 4; f++) mx[f] = max3(mx[f], __uint_as_float(v0[e + f]), __uint_as_float(v1[e + f]));
-                const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-                if (mine) m_run = fmaxf(m_run, tile_max);
+                    for (int f = 0; f < 4; f++) mx[f] = max3_nan(mx[f], __uint_as_float(v0[e + f]), __uint_as_float(v1[e + f]));
+                const float tile_max = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]) * sc;
+                if (mine) m_run = max_nan(m_run, tile_max);
                 const bool grow = m_run > m_used + RESCALE_AT || (m_used == -INFINITY && m_run != -INFINITY);
                 if (__any_sync(0xffffffffu, grow && j > 0)) {
                     // O may only be touched between products: wait for the previous page's
@@ -394,8 +394,9 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
             unpack2(sum2[1], sum[2], sum[3]);
             if (mine) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
-        // A score of +inf: the others' weights are all 0, and its own, inf - inf, is 0 too where the polynomial has it.
-        if (m_run == INFINITY) l = NAN;
+        // A NaN score's weight is 0 where the polynomial has it; and of a score of +inf, beside which the others weigh nothing, so is its
+        // own, inf - inf.
+        if (!(m_run < INFINITY)) l = NAN;
         if (ok && n > 0 && !mbar_wait(&o_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u)) ok = false;
         if (!ok) {
             atomicCAS(&g_status, 0, 4);

@@ -358,10 +358,10 @@ __device__ __forceinline__ void prefill_tc5(const CUtensorMap& map_q, const CUte
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(v0[i + e]), __uint_as_float(v1[i + e]));
+                    for (int e = 0; e < 4; e++) mx[e] = max3_nan(mx[e], __uint_as_float(v0[i + e]), __uint_as_float(v1[i + e]));
                 }
-                const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;  // sc > 0
-                m_run = fmaxf(m_run, tile_max);
+                const float tile_max = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]) * sc;  // sc > 0
+                m_run = max_nan(m_run, tile_max);
                 // rescale only when the maximum has outgrown the scale in use (or there is none yet)
                 grow = m_run > m_used + RESCALE_AT || (m_used == -INFINITY && m_run != -INFINITY);
             }
@@ -443,8 +443,9 @@ __device__ __forceinline__ void prefill_tc5(const CUtensorMap& map_q, const CUte
             // a sink adds one unit to the denominator: a key of score 0, in the scale the sums are kept in
             // (a sum so scaled that the unit overflows gives 1 / inf = 0, which is the limit)
             if (!sig && p.sink && m_used != -INFINITY) l += exp2f((p.sinks ? p.sinks[head] * LOG2E : 0.f) - m_used);
-            // a score of +inf: the others' weights are all 0, and its own, inf - inf, is 0 too where the polynomial has it
-            if (!sig && m_run == INFINITY) l = NAN;
+            // a NaN score's weight is 0 where the polynomial has it; and of a score of +inf, beside which the others weigh nothing, so
+            // is its own, inf - inf
+            if (!sig && !(m_run < INFINITY)) l = NAN;
             float inv = 1.f / l;
             if (sig) {
                 inv = 1.f;

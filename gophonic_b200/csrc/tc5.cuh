@@ -230,9 +230,15 @@ __device__ __forceinline__ uint64_t exp2_poly_x2(uint64_t x) {
     const float y0 = __int_as_float(__float_as_int(q0) + (__float_as_int(r0) << 23)), y1 = __int_as_float(__float_as_int(q1) + (__float_as_int(r1) << 23));
     return mul2_ftz(pack2(y0, y1), pack2(5.421010862427522e-20f, 5.421010862427522e-20f));      // 2^-64
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// Maxima that are NaN where a value is: a row's maximum is how a NaN score is met, whose weight the polynomial loses.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
 

@@ -146,3 +146,12 @@ def test_a_score_beyond_all_others_shows(ops, heads, kvh, new):
 
 def test_a_score_beyond_all_others_shows_in_a_prompt(ops):
     check_prompt(ops, [math.inf])
+
+
+@FORMS
+def test_a_score_that_is_no_number_shows(ops, heads, kvh, new):
+    check_listed(ops, heads, kvh, new, [math.nan])
+
+
+def test_a_score_that_is_no_number_shows_in_a_prompt(ops):
+    check_prompt(ops, [math.nan])
