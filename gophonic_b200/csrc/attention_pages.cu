@@ -62,9 +62,9 @@ __device__ __forceinline__ int pack_list(const PagesParams& p, const int* bt, co
 
 // What the CTAs of a cluster leave for one another: per head of the chunk its maximum, sum and weighted values.  Joined by all of them:
 // CTA r of the cluster writes every PIECES-th four channels.  All pieces' values are asked for before the first is used: one
-// trip through the cluster's shared memory instead of two dozen.
+// trip through the cluster's shared memory instead of two dozen.  saw: the row's list names a page it can see.
 template <typename T, int PIECES>
-__device__ __forceinline__ void join_pieces(const float* ml, const float* os, int nh, int hd, T* out) {
+__device__ __forceinline__ void join_pieces(const float* ml, const float* os, int nh, int hd, T* out, bool saw) {
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = PIECES == 1 ? 0 : (int)cluster.block_rank();
     const int quads = hd / 4;
@@ -94,7 +94,7 @@ __device__ __forceinline__ void join_pieces(const float* ml, const float* os, in
             acc.w += e * x[w].w;
         }
         T* op = out + (int64_t)r * hd + c;
-        const float inv = L == 0.f ? 0.f : 1.f / L;     // nothing seen: zeros
+        const float inv = L != 0.f ? 1.f / L : saw ? NAN : 0.f;     // nothing seen: zeros; scores that are all -inf: 0 / 0
         op[0] = from_f32<T>(acc.x * inv);
         op[1] = from_f32<T>(acc.y * inv);
         op[2] = from_f32<T>(acc.z * inv);
@@ -103,20 +103,20 @@ __device__ __forceinline__ void join_pieces(const float* ml, const float* os, in
 }
 
 template <typename T>
-__device__ __forceinline__ void join(const float* ml, const float* os, int nh, int hd, T* out) {
+__device__ __forceinline__ void join(const float* ml, const float* os, int nh, int hd, T* out, bool saw) {
     cg::cluster_group cluster = cg::this_cluster();
     const int pieces = (int)cluster.num_blocks();
     if (pieces == 1) {
         __syncthreads();
-        join_pieces<T, 1>(ml, os, nh, hd, out);
+        join_pieces<T, 1>(ml, os, nh, hd, out, saw);
         return;
     }
     cluster.sync();
     switch (pieces) {
-        case 2: join_pieces<T, 2>(ml, os, nh, hd, out); break;
-        case 4: join_pieces<T, 4>(ml, os, nh, hd, out); break;
-        case 8: join_pieces<T, 8>(ml, os, nh, hd, out); break;
-        default: join_pieces<T, 16>(ml, os, nh, hd, out); break;
+        case 2: join_pieces<T, 2>(ml, os, nh, hd, out, saw); break;
+        case 4: join_pieces<T, 4>(ml, os, nh, hd, out, saw); break;
+        case 8: join_pieces<T, 8>(ml, os, nh, hd, out, saw); break;
+        default: join_pieces<T, 16>(ml, os, nh, hd, out, saw); break;
     }
     cluster.sync();     // a CTA's shared memory outlives its readers
 }
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_mma_kernel(PagesParams p) 
             ml[r][1] = L;
         }
     }
-    join<bf16>(&ml[0][0], Os, at.nh, HD, (bf16*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * HD);
+    join<bf16>(&ml[0][0], Os, at.nh, HD, (bf16*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * HD, n_all > 0);
 }
 
 // ---- float32 -------------------------------------------------------------------------------------
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
         for (int c = 0; c < F_CH; c++)
             if (h < at.nh && tid + c * THREADS < d) Os[h * d + tid + c * THREADS] = o[h][c];
     __syncthreads();
-    join<float>(&ml[0][0], Os, at.nh, d, (float*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * d);
+    join<float>(&ml[0][0], Os, at.nh, d, (float*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * d, n_all > 0);
 }
 
 // Into how many pieces a row's list is cut: the CTAs of a cluster, a power of two (sixteen where the GPU holds all of the clusters).  As many as run at once (one token over eight key heads, 32 pages:

@@ -67,9 +67,11 @@ __device__ __noinline__ void row_alone(const PagesParams& p, const int* bt, int 
     const int* list = p.list + ((int64_t)row * p.kv_heads + kvh) * p.top;
     const bf16* q = (const bf16*)p.q + (int64_t)row * p.q_row_stride + (int64_t)head * HD;
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    bool saw = false;
     for (int i = 0; i < p.top; i++) {
         const int lp = list[i];
         if (lp < 0 || lp > pos / BKV || lp >= p.bt_stride) continue;
+        saw = true;
         const int64_t off = (page_of(bt, lp * BKV, p.bt_stride, p.pages) * p.kv_heads + kvh) * (int64_t)(BKV * HD);
         const bf16 *k = (const bf16*)p.k_plane + off, *v = (const bf16*)p.v_plane + off;
         const int n = min(BKV, pos + 1 - lp * BKV);
@@ -98,7 +100,7 @@ __device__ __noinline__ void row_alone(const PagesParams& p, const int* bt, int 
         }
     }
     bf16* to = (bf16*)p.out + (int64_t)row * p.out_row_stride + (int64_t)head * HD + lane * 4;
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    const float inv = m != -INFINITY ? 1.f / l : saw ? NAN : 0.f;
     for (int e = 0; e < 4; e++) to[e] = __float2bfloat16_rn(o[e] * inv);
 }
 
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
         const int pos = past + q0 + tok;
         const float sc = p.scale * LOG2E;    // > 0
         float m_run = -INFINITY;
-        bool ok = true;
+        bool ok = true, saw = false;
         for (int j = 0; j < n && ok; j++) {
             const int b = j & 1, key0 = entry[j] * BKV;
             const bool mine = (bits[j * MW + (tok >> 5)] >> (tok & 31)) & 1u;
@@ -344,6 +346,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
                     for (int f = 0; f < 4; f++) mx[f] = max3_nan(mx[f], __uint_as_float(v0[e + f]), __uint_as_float(v1[e + f]));
                 const float tile_max = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]) * sc;
                 if (mine) m_run = max_nan(m_run, tile_max);
+                saw = saw || mine;
                 const bool grow = m_run > m_used + RESCALE_AT || (m_used == -INFINITY && m_run != -INFINITY);
                 if (__any_sync(0xffffffffu, grow && j > 0)) {
                     // O may only be touched between products: wait for the previous page's
@@ -397,6 +400,8 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
         // A NaN score's weight is 0 where the polynomial has it; and of a score of +inf, beside which the others weigh nothing, so is its
         // own, inf - inf.
         if (!(m_run < INFINITY)) l = NAN;
+        // Scores that are all -inf: 0 / 0, but other CTAs of the tile may have found better ones for the row.
+        if (saw && l == 0.f) l = pieces == 1 ? NAN : -1.f;
         if (ok && n > 0 && !mbar_wait(&o_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u)) ok = false;
         if (!ok) {
             atomicCAS(&g_status, 0, 4);
@@ -476,8 +481,8 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
             for (int w = 0; w < MAX_PIECES; w++)
                 if (w < pieces) x[w] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums, w) + (size_t)at * HD + (lane ^ (at & 31)) * 4);
             const float M = warp_max(m);
-            // this row saw nothing there: neither a maximum nor a sum (a NaN score leaves no maximum but a NaN sum)
-            const bool none = m == -INFINITY && l_w == 0.f;
+            // this row saw nothing there, or scores of -inf alone: no maximum, and a sum of 0 or -1 (a NaN score has a NaN sum)
+            const bool none = m == -INFINITY && l_w <= 0.f, lost = __any_sync(0xffffffffu, l_w < 0.f);
             const float f_w = none ? 0.f : m == -INFINITY ? 1.f : fast_exp2(m - M);
             const float L = warp_sum(none ? 0.f : f_w * l_w);
             float o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -494,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_pages_tc5_kernel(const __grid
                 row_alone(p, bt, q_start + q0 + tk, past + q0 + tk, kvh * G + hh, kvh, lane);
                 continue;
             }
-            const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+            const float inv = L > 0.f ? 1.f / L : L == 0.f && !lost ? 0.f : NAN;
             const __nv_bfloat162 a = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), b = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
             bf16* op = (bf16*)p.out + (int64_t)(q_start + q0 + tk) * p.out_row_stride + (int64_t)(kvh * G + hh) * HD + lane * 4;
             *reinterpret_cast<uint2*>(op) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));

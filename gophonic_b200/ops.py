@@ -940,7 +940,7 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v
     """Causal GQA over a part of the paged cache: row r's heads of kv head g attend to the keys, at positions up to the row's own, of
     the logical pages that ``pages[r, g]`` lists (int32 [rows, kv_heads, top], top up to ``MAX_LISTED_PAGES``; each page once, as
     ``select_pages`` leaves them; negative entries and pages behind the row's own name nothing).  A row that sees no key
-    gives zeros; rows of no sequence keep what they had.  q and out are [rows, >= heads * head_dim] views (row strides free) that do not
+    gives zeros, one that sees a score of NaN or +inf, or scores of -inf alone, NaN; rows of no sequence keep what they had.  q and out are [rows, >= heads * head_dim] views (row strides free) that do not
     overlap.  What a row does not see may hold Inf or NaN."""
     dtype, dev, wide = q.dtype, q.get_device(), heads * head_dim
     table, listed, plane, shape, to = block_table.shape, pages.shape, k_plane.shape, q.shape, out.shape

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_pages import BF, DEV, PAGE, Step, like_lists
+from tests.test_gpu_pages import BF, DEV, F32, PAGE, Step, like_lists, names
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,57 @@ def test_a_score_that_is_no_number_shows(ops, heads, kvh, new):
 
 def test_a_score_that_is_no_number_shows_in_a_prompt(ops):
     check_prompt(ops, [math.nan])
+
+
+@FORMS
+def test_scores_that_are_all_the_lowest_show(ops, heads, kvh, new):
+    """All scores -inf: 0 / 0.  Some of them: keys of no weight."""
+    s = Step([(150, new)], heads, kvh, 128, BF, seed=2)
+    looks_up(s)
+    pages = like_lists(s, 5, 5, 12, 5)
+    pages[pages == 0] = -1       # so that some rows list page 3 alone
+    pages[60:90] = -1
+    pages[60:90, :, 2] = 3
+    own = (150 + torch.arange(new)).view(new, 1, 1) // PAGE
+    pages[(pages == 3) & (own < 3)] = -1
+    alone = (pages == 3).any(-1) & ((pages == 3) | (pages < 0)).all(-1)
+    without = pages.clone()
+    without[without == 3] = -1
+    empty = (pages < 0).all(-1)
+    want = by_head(s, s.attend(ops, without.to(DEV)))
+    s.dev["k_plane"][s.table[s.slots[0], 3], :, :, 0] = -math.inf
+    got = by_head(s, s.attend(ops, pages.to(DEV)))
+    assert alone.any() and (~alone & (pages == 3).any(-1)).any()
+    assert got[alone].isnan().all() and (got[empty] == 0).all()
+    assert got[~alone].isfinite().all()
+    assert float((got[~alone] - want[~alone]).abs().max()) <= 4 * 2.0 ** -8 * float(s.v_plane.float().abs().max())
+    s.dev["k_plane"][:, :, :, 0] = -math.inf
+    got = by_head(s, s.attend(ops, pages.to(DEV)))
+    assert got[~empty].isnan().all() and (got[empty] == 0).all() and ops.tc5_status() == 0
+
+
+@pytest.mark.parametrize("dtype,heads,kvh,d", [(BF, 4, 2, 128), (BF, 20, 1, 64), (F32, 4, 2, 64), (F32, 20, 1, 128)], ids=names)
+def test_scores_of_single_rows_that_are_not_finite(ops, dtype, heads, kvh, d):
+    """Rows one by one, their lists in one piece and in several: NaN for a score of NaN or +inf and for -inf alone, zeros for no key."""
+    for top in (4, 32):
+        s = Step([(2100, 1)] * 7, heads, kvh, d, dtype, seed=4)
+        looks_up(s)
+        pages = torch.full((7, kvh, top), -1, dtype=torch.int32)
+        pages[0:3, :, 1] = 3
+        pages[3:6] = torch.arange(top, dtype=torch.int32) if top == 32 else torch.tensor([0, 2, 3, 9], dtype=torch.int32)
+        keys = s.dev["k_plane"]
+        for i, score in [(0, math.nan), (1, math.inf), (3, math.nan), (4, math.inf)]:
+            keys[s.table[s.slots[i], 3], :, 41, 0] = score
+        for i in (2, 5):
+            keys[s.table[s.slots[i], 3], :, :, 0] = -math.inf
+        want = s.attend(ops, torch.where(pages == 3, -1, pages).to(DEV))
+        got = s.attend(ops, pages.to(DEV))
+        assert got[:5].isnan().all() and (got[6] == 0).all() and got[5].isfinite().all()
+        assert float((got[5].float() - want[5].float()).abs().max()) <= 4 * (2.0 ** -8 if dtype == BF else 2.0 ** -17) * float(s.v_plane.float().abs().max())
+
+
+def test_scores_that_are_all_the_lowest_show_in_a_prompt(ops):
+    s = Step([(0, 150)], 4, 2, 128, BF, seed=3)
+    looks_up(s)
+    s.dev["k_plane"][:, :, :, 0] = -math.inf
+    assert attend_all(ops, s).isnan().all() and ops.tc5_status() == 0
