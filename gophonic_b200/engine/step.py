@@ -46,6 +46,9 @@ class StepBatch:
     sm_count: int = 148
     # (tokens before, rows in this batch) of every sequence, where the host knows them (a replayed step's change)
     extents: Optional[Sequence[Tuple[int, int]]] = None
+    # whether each sequence brings a single token to the step (a pass may hold a single row of a longer run); None: all of them, if
+    # ``max_q_len`` is 1
+    singles: Optional[Sequence[bool]] = None
     # launch plans of the step's mixers, by the mixer's identity (``Mixer.plan``); a mixer that is
     # not listed is asked when it first runs
     plans: Dict[int, object] = field(default_factory=dict)
@@ -120,8 +123,9 @@ class TokenFetch:
 
 def build_batch(pieces: Sequence[Tuple[int, Sequence[int], int]], device, sm_count: int = 148,
                 want_rows: Optional[Sequence[int]] = None,
-                stager: Optional[HostStager] = None) -> Tuple[StepBatch, Optional[torch.Tensor]]:
-    """``pieces[i] = (slot, tokens, first_position)``: one device upload for all row metadata."""
+                stager: Optional[HostStager] = None, singles: Optional[Sequence[bool]] = None) -> Tuple[StepBatch, Optional[torch.Tensor]]:
+    """``pieces[i] = (slot, tokens, first_position)``: one device upload for all row metadata.  ``singles``: see ``StepBatch``; by
+    default a piece of one token is one."""
     nseq = len(pieces)
     rows = sum(len(t) for _, t, _ in pieces)
     nw = 0 if want_rows is None else len(want_rows)
@@ -143,7 +147,8 @@ def build_batch(pieces: Sequence[Tuple[int, Sequence[int], int]], device, sm_cou
                       row_pos=dev[rows:2 * rows], row_seq=dev[2 * rows:3 * rows],
                       seq_slot=dev[o:o + nseq], seq_q_start=dev[o + nseq:o + 2 * nseq],
                       seq_q_len=dev[o + 2 * nseq:o + 3 * nseq], seq_kv_len=dev[o + 3 * nseq:o2],
-                      device=torch.device(device), sm_count=sm_count, extents=[(first, len(toks)) for _, toks, first in pieces])
+                      device=torch.device(device), sm_count=sm_count, extents=[(first, len(toks)) for _, toks, first in pieces],
+                      singles=[len(toks) == 1 for _, toks, _ in pieces] if singles is None else singles)
     return batch, (dev[o2:] if nw else None)
 
 
@@ -359,9 +364,10 @@ class Engine:
         ev.record()
         return TokenFetch(host, ev)
 
-    def _pass(self, pieces, want_rows: Sequence[int], source: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    def _pass(self, pieces, want_rows: Sequence[int], source: Optional[torch.Tensor] = None,
+              singles: Optional[Sequence[bool]] = None) -> Optional[torch.Tensor]:
         batch, want_dev = build_batch(pieces, self.device, self.sm_count, want_rows if want_rows else None,
-                                      self.stager)
+                                      self.stager, singles)
         if source is not None:
             self.model.rt.ops.gather_tokens(batch.ids, source)
         self.passes += 1
@@ -431,13 +437,14 @@ class Engine:
         total = starts[-1] + len(entries[-1][1])
         while lo < total:
             hi = min(total, lo + self.max_rows_per_pass)
-            pieces = []
+            pieces, singles = [], []
             for i, (slot, toks) in enumerate(entries):
                 a, b = max(lo, starts[i]), min(hi, starts[i] + len(toks))
                 if a < b:
                     pieces.append((slot, list(toks[a - starts[i]:b - starts[i]]), self.cache.length(slot) + a - starts[i]))
+                    singles.append(len(toks) == 1)
             local = sorted({row for row in want_rows if lo <= row < hi})
-            logits = self._pass(pieces, [row - lo for row in local])
+            logits = self._pass(pieces, [row - lo for row in local], singles=singles)
             ks = [k for row in local for k in order[row]]
             if ks:
                 js = [j for j, row in enumerate(local) for _ in order[row]]

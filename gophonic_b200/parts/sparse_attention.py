@@ -45,13 +45,33 @@ class SparseAttention(Attention):
             return "selected pages"
         return super().plan(nseq, max_q_len, max_kv_len, sm_count)
 
+    def key_splits(self, batch):
+        if batch.plan_for(self) == "selected pages":     # rows of runs, a row a pass, which read everything
+            return 1, None
+        return super().key_splits(batch)
+
+    def who_selects(self, batch):
+        """Which sequences' rows select: True for all, False for none, else (their rows, the other sequences' rows) as numbers of rows a
+        sequence: unless ``prompts``, a run's rows do not select, also where a pass holds one of them."""
+        limit, runs = 64 * self.spec.selection.pages, not self.spec.selection.prompts
+        if batch.plan_for(self) == "selected pages" and not (runs and batch.singles is not None and not all(batch.singles)):
+            return True
+        if not runs or batch.singles is None or batch.max_q_len > 1 or batch.max_kv_len <= limit:
+            return False
+        key = ("single tokens that select", limit)      # every layer has the same answer
+        if key not in batch.shared:
+            some = [int(single and past + rows > limit) for single, (past, rows) in zip(batch.singles, batch.extents)]
+            mine = torch.tensor(some, dtype=torch.int32, device=batch.seq_q_len.device) if any(some) else None
+            batch.shared[key] = False if mine is None else (mine, batch.seq_q_len - mine)
+        return batch.shared[key]
+
     def _attend(self, batch, qkv: torch.Tensor, cache) -> torch.Tensor:
         ops, s = self.rt.ops, self.spec
-        listed = batch.plan_for(self) == "selected pages"
+        who = self.who_selects(batch)
         # The pages that a run of tokens fills: its own later tokens may select them, and those of later steps will.  Single tokens
         # leave them to the end of the step (``Cache.keep_bounds``).
         fills = batch.max_q_len > 1 and cache is not None and cache.writable
-        if not listed:
+        if who is False:
             ctx = super()._attend(batch, qkv, cache)
             if fills:
                 self._bounds(batch, cache)
@@ -70,9 +90,17 @@ class SparseAttention(Attention):
         pages = batch.workspace(("selected pages", s.kv_heads, sel.pages), rows * s.kv_heads * sel.pages, torch.int32)
         pages = pages[:rows * s.kv_heads * sel.pages].view(rows, s.kv_heads, sel.pages)
         ctx = torch.empty((rows, self.q_dim), dtype=qkv.dtype, device=qkv.device)
-        seqs = (batch.seq_slot, batch.seq_q_start, batch.seq_q_len, batch.seq_kv_len, batch.nseq, batch.max_q_len, s.heads, s.kv_heads, s.head_dim)
-        ops.select_pages(q, cache.bounds, cache.block_table, *seqs, pages, sel.first, sel.last)
-        ops.attention_pages(q, ctx, cache.k, cache.v, cache.block_table, *seqs, float(s.scale), pages)
+        heads = (s.heads, s.kv_heads, s.head_dim)
+        q_len, max_q_len = batch.seq_q_len, batch.max_q_len
+        if who is not True:
+            q_len, others = who
+            # (rows of single tokens are left as they are, or, where all rows of a pass are single ones, written by both, these first)
+            ops.attention(q, ctx, cache.k, cache.v, cache.block_table, batch.seq_slot, batch.seq_q_start, others, batch.seq_kv_len, batch.nseq,
+                          max_q_len, *heads, float(s.scale))
+            max_q_len = 1
+        seqs = (batch.seq_slot, batch.seq_q_start, q_len, batch.seq_kv_len, batch.nseq, max_q_len)
+        ops.select_pages(q, cache.bounds, cache.block_table, *seqs, *heads, pages, sel.first, sel.last)
+        ops.attention_pages(q, ctx, cache.k, cache.v, cache.block_table, *seqs, *heads, float(s.scale), pages)
         return ctx
 
     def _bounds(self, batch, cache) -> None:

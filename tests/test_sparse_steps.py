@@ -1,0 +1,57 @@
+"""Which rows of a step select pages: each sequence by what it brings itself.  What needs no GPU."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from gophonic_b200.config import PageSelection
+from gophonic_b200.engine.step import Engine, build_batch
+from gophonic_b200.parts.sparse_attention import SparseAttention
+
+
+def mixer(pages=3, prompts=False):
+    m = SparseAttention.__new__(SparseAttention)
+    m.spec = SimpleNamespace(selection=PageSelection(pages, prompts=prompts), heads=4, kv_heads=2, head_dim=64, window=0)
+    m.rt = SimpleNamespace(is_fp32=False)
+    return m
+
+
+def who(extents, singles=None, **kw):
+    batch, _ = build_batch([(i, [5] * rows, past) for i, (past, rows) in enumerate(extents)], torch.device("cpu"), singles=singles)
+    got = mixer(**kw).who_selects(batch)
+    return got if isinstance(got, bool) else tuple(t.tolist() for t in got)
+
+
+def test_single_tokens_alone():
+    assert who([(500, 1), (20, 1)]) is True
+    assert who([(191, 1), (20, 1)]) is False
+    assert who([(500, 1), (20, 1)], prompts=True) is True
+
+
+def test_runs_alone():
+    assert who([(500, 40), (20, 2)]) is False
+    assert who([(500, 40), (20, 2)], prompts=True) is True
+
+
+def test_a_row_that_a_pass_holds_of_a_run_is_no_single_token():
+    assert who([(500, 1)], [False]) is False
+    assert who([(500, 1), (600, 1)], [False, True]) == ([0, 1], [1, 0])
+    assert who([(500, 1), (600, 40)], [False, False]) is False
+    assert who([(500, 1)], [False], prompts=True) is True
+
+
+def test_a_row_of_a_run_is_read_in_one_piece():
+    batch, _ = build_batch([(0, [5], 5000)], torch.device("cpu"), singles=[False])
+    assert mixer().key_splits(batch) == (1, None)
+
+
+@pytest.mark.parametrize("most,lens", [(100, [301]), (100, [99, 302]), (100, [301, 1]), (4, [9, 1, 3]), (1, [3, 1])])
+def test_passes_know_which_rows_are_single_tokens(monkeypatch, most, lens):
+    """A long step is cut into passes; what one pass holds of a run stays part of a run."""
+    seen = []
+    eng = SimpleNamespace(max_rows_per_pass=most, vocab=7, device="cpu", cache=SimpleNamespace(length=lambda slot: 0))
+    eng._pass = lambda pieces, want, source=None, singles=None: seen.extend((slot, first, single) for (slot, _, first), single in zip(pieces, singles))
+    starts = [sum(lens[:i]) for i in range(len(lens))]
+    Engine._chunked(eng, [(i, [0] * n) for i, n in enumerate(lens)], starts, [])
+    assert len(seen) > len(lens)
+    assert all(single == (lens[slot] == 1) for slot, _, single in seen)
