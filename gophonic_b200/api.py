@@ -56,7 +56,8 @@ class Options:
     Batch: int = 8
     # SparsePages > 0: behind more than that many pages of 64 tokens, a token of a layer that attends to its whole context reads
     # only so many pages: the first, the two up to its own, and those whose keys could score highest.  Replies behind long
-    # contexts then cost what a context of 64 * SparsePages costs.  Prompts are still read in full, unless SparsePrompts.
+    # contexts then cost what a context of 64 * SparsePages costs.  Prompts are still read in full, unless SparsePrompts
+    # (a prompt that adds a single token to its conversation is a token like a reply's).
     SparsePages: int = 0
     SparsePrompts: bool = False
 

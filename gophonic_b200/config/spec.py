@@ -111,9 +111,9 @@ class AttentionSpec:
 @dataclass(frozen=True)
 class PageSelection:
     """How much of its context a token reads: ``pages`` pages of 64 tokens in all, among them always the first ``first`` and the
-    last ``last`` (its own included), the others those whose keys could score highest.  ``prompts`` False: only single tokens
-    select, runs of tokens (prompts) attend to everything; True: every token does, so that a token's result does not depend
-    on whether it came in a prompt or alone."""
+    last ``last`` (its own included), the others those whose keys could score highest.  ``prompts`` False: only tokens that
+    a sequence brings to a step alone select, runs of tokens (prompts) attend to everything, whatever the step's other sequences
+    bring; True: every token selects, so that a token's result does not depend on whether it came in a prompt or alone."""
     pages: int
     first: int = 1
     last: int = 2

@@ -52,11 +52,12 @@ class SparseAttention(Attention):
 
     def who_selects(self, batch):
         """Which sequences' rows select: True for all, False for none, else (their rows, the other sequences' rows) as numbers of rows a
-        sequence: unless ``prompts``, a run's rows do not select, also where a pass holds one of them."""
+        sequence.  A sequence's answer does not follow from the others': unless ``prompts``, those that bring a single token select,
+        also beside the runs of others, and a run's rows do not, also where a pass holds one of them."""
         limit, runs = 64 * self.spec.selection.pages, not self.spec.selection.prompts
         if batch.plan_for(self) == "selected pages" and not (runs and batch.singles is not None and not all(batch.singles)):
             return True
-        if not runs or batch.singles is None or batch.max_q_len > 1 or batch.max_kv_len <= limit:
+        if not runs or batch.singles is None or batch.max_kv_len <= limit:
             return False
         key = ("single tokens that select", limit)      # every layer has the same answer
         if key not in batch.shared:

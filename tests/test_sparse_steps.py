@@ -33,6 +33,12 @@ def test_runs_alone():
     assert who([(500, 40), (20, 2)], prompts=True) is True
 
 
+def test_single_tokens_beside_runs():
+    assert who([(500, 1), (0, 300), (20, 1), (192, 1)]) == ([1, 0, 0, 1], [0, 300, 1, 0])
+    assert who([(100, 1), (0, 300)]) is False
+    assert who([(500, 1), (0, 300)], prompts=True) is True
+
+
 def test_a_row_that_a_pass_holds_of_a_run_is_no_single_token():
     assert who([(500, 1)], [False]) is False
     assert who([(500, 1), (600, 1)], [False, True]) == ([0, 1], [1, 0])
