@@ -191,6 +191,9 @@ class Cache:
         for pos, cache_of in self._cache_of.items():
             if cache_of is not None and cache_of not in self._plane:
                 raise CacheError(f"schedule position {pos} reads the cache of position {cache_of}, which has none")
+            # bounds are kept by the run that writes the keys: beside the keys of one that does not, they would be of no token's or of another's
+            if cache_of is not None and self._asks_for_bounds(requests[pos][0]) and not self._asks_for_bounds(requests[cache_of][0]):
+                raise CacheError(f"schedule position {pos} needs bounds beside the keys of position {cache_of}, which keeps none")
         self._k: Dict[Tuple[int, ...], torch.Tensor] = {}
         self._v: Dict[Tuple[int, ...], torch.Tensor] = {}
         for key, planes in self._kv_groups.items():
@@ -250,6 +253,14 @@ class Cache:
             planes.append(pos)
         else:
             raise CacheError(f"schedule position {pos}: unknown cache request {req!r}")
+
+    @staticmethod
+    def _asks_for_bounds(req) -> bool:
+        if isinstance(req, BlockStateRequest):
+            req = req.mixer
+        if isinstance(req, KVStateRequest):
+            req = req.kv
+        return bool(getattr(req, "bounds", False))
 
     @staticmethod
     def _geometry(key) -> Tuple[int, int, int, int, int, bool]:

@@ -4,8 +4,10 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from gophonic_b200.cache import Cache, CacheError
 from gophonic_b200.config import PageSelection
 from gophonic_b200.engine.step import Engine, build_batch
+from gophonic_b200.parts.base import BlockStateRequest, KVRequest, KVStateRequest, StateRequest
 from gophonic_b200.parts.sparse_attention import SparseAttention
 
 
@@ -61,3 +63,14 @@ def test_passes_know_which_rows_are_single_tokens(monkeypatch, most, lens):
     Engine._chunked(eng, [(i, [0] * n) for i, n in enumerate(lens)], starts, [])
     assert len(seen) > len(lens)
     assert all(single == (lens[slot] == 1) for slot, _, single in seen)
+
+
+def test_a_run_that_selects_reads_no_cache_without_bounds():
+    """Nor one that has them only because another run of its group asked: who writes the keys keeps them."""
+    plain, bounded = KVRequest(2, 16), KVRequest(2, 16, bounds=True)
+    for owner in (plain, KVStateRequest(plain, StateRequest((4,), torch.float32)), BlockStateRequest(plain, StateRequest((4,), torch.float32))):
+        for more in ([], [(bounded, None)]):
+            with pytest.raises(CacheError, match="bounds"):
+                Cache([(owner, None), (bounded, 0)] + more, 256, "cpu", torch.float32)
+    c = Cache([(bounded, None), (bounded, 0), (plain, 0)], 256, "cpu", torch.float32)
+    assert c.view(1).bounds.data_ptr() == c.view(0).bounds.data_ptr()
