@@ -119,3 +119,42 @@ def test_a_mixed_step_in_bfloat16(models, name, runs):
     singles = torch.stack((mixed[0], mixed[-1]))
     assert float((singles.float() - longest.float()).abs().max()) <= 4 * 2.0 ** -8 * float(view.v.float().abs().max())
     eng.check_kernels()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["A", "D"])
+def test_bounds_follow_the_keys_through_cuts(models, name, dtype):
+    """Cut back and grown with other tokens, in runs, one by one and beside other sequences, also behind a restored mark: the bounds of every full
+    page are the extremes of the keys that stand there, bit for bit."""
+    eng = engine_of(models(name, dtype))
+    toks, other = [ids(name, 460, 60 + i) for i in range(5)], fresh(eng, ids(name, 100, 70))
+
+    def check(slot):
+        n = eng.length(slot) // 64
+        at = eng.cache.block_table[slot, :n].long()
+        for pos in range(len(eng.model.blocks)):
+            view = eng.cache.view(pos)
+            k = view.k[at]
+            assert torch.equal(view.bounds[at], torch.stack((k.amin(2), k.amax(2)), 2)), (pos, n)
+    slot = fresh(eng, toks[0][:400])
+    check(slot)
+    mark = eng.checkpoint(slot)
+    for t in toks[0][400:]:
+        eng.step([(slot, [t])])
+    check(slot)
+    eng.truncate(slot, 100)
+    eng.step([(slot, toks[1][100:250]), (other, [1])])
+    check(slot)
+    for t in toks[1][250:460]:
+        eng.step([(slot, [t])])
+    check(slot)
+    eng.restore(slot, mark)
+    for t in toks[2][400:]:
+        eng.step([(slot, [t])])
+    check(slot)
+    eng.truncate(slot, 130)
+    for i, t in enumerate(toks[3][130:260]):
+        eng.step([(slot, [t]), (other, toks[4][2 * i:2 * i + 2])])
+    check(slot)
+    check(other)
+    eng.cache.check()
