@@ -807,13 +807,13 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
             const int i = min(i0 + t * 8 + g, nc - 1);         // pages beyond the last are the last once more
             b[t] = plane + (page_of(bt, (p.first + i) * GB_PAGE, p.bt_stride, p.pages) * p.kv_heads + kvh) * (2 * d) + t4 * 8;
         }
-        float acc[MT][2][4];
+        float acc[2][MT][2][4];      // of the coefficients' first parts and of their second ones, so that the sums of the larger are short
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[m][t][e] = 0.f;
+                for (int e = 0; e < 4; e++) acc[0][m][t][e] = acc[1][m][t][e] = 0.f;
 #pragma unroll
         for (int half = 0; half < KB_MAX / 4; half++) {        // blocks in fours: what a lane asks for at once
             if (half * 4 >= KB) break;
@@ -844,8 +844,8 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
                         const uint4 a0 = *reinterpret_cast<const uint4*>(a), a1 = *reinterpret_cast<const uint4*>(a + 8 * CS);
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
-                            mma_bf16_16816(acc[m][t], a0.x, a1.x, a0.y, a1.y, x[j][t].x, x[j][t].y);
-                            mma_bf16_16816(acc[m][t], a0.z, a1.z, a0.w, a1.w, x[j][t].z, x[j][t].w);
+                            mma_bf16_16816(acc[term][m][t], a0.x, a1.x, a0.y, a1.y, x[j][t].x, x[j][t].y);
+                            mma_bf16_16816(acc[term][m][t], a0.z, a1.z, a0.w, a1.w, x[j][t].z, x[j][t].w);
                         }
                     }
             }
@@ -855,8 +855,11 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 const int i = i0 + t * 8 + t4 * 2;             // KS has room for whole blocks of 16
-                *reinterpret_cast<uint2*>(keys + (m * 16 + g) * KS + i) = make_uint2(order_key(acc[m][t][0]), order_key(acc[m][t][1]));
-                *reinterpret_cast<uint2*>(keys + (m * 16 + g + 8) * KS + i) = make_uint2(order_key(acc[m][t][2]), order_key(acc[m][t][3]));
+                float sum[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum[e] = acc[0][m][t][e] + acc[1][m][t][e];
+                *reinterpret_cast<uint2*>(keys + (m * 16 + g) * KS + i) = make_uint2(order_key(sum[0]), order_key(sum[1]));
+                *reinterpret_cast<uint2*>(keys + (m * 16 + g + 8) * KS + i) = make_uint2(order_key(sum[2]), order_key(sum[3]));
             }
     }
 #pragma unroll
@@ -879,21 +882,24 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
             for (int i = lane; i < p.top; i += 32) r.list[i] = i < r.n ? i : -1;
             continue;
         }
-        // The coefficients are good to 2^-18 (3.9e-6) and G half steps of 2^-23, relative to the sum of the terms' sizes.  Their products'
-        // sums on the tensor cores: 4 KB steps of 16 products and the sum so far, cut off behind 25 bits of the largest of them, and
-        // the result: 6 units of 2^-23 of what has been summed up to there, so that a block's terms count once for every step
-        // from their own on.  What is below the normal range of a coefficient's second part is let in by 1e-35.
+        // The coefficients are good to 2^-18 (3.9e-6) and G half steps of 2^-23, relative to the sum of the terms' sizes.  The products
+        // of their first parts are summed up by 2 KB products of the tensor cores, of which the PTX manual says that they accumulate with at
+        // least single precision, in any order and rounding: 17 numbers each, the sum so far among them, so no more than 17 units of
+        // 2^-23 of what has been summed up to there, and a block's terms count once for every step from their own on.  (The second parts'
+        // products are 2^-8 of that, the two sums' sum half a unit: 18.)  What is below the normal range may count as nothing: a
+        // coefficient's second part (let in by 1e-35), a coefficient or a bound (1.2e-38 of the other), a sum.
         float most = 0.f, steps = 0.f;
 #pragma unroll 8
         for (int c = lane; c < 2 * d; c += 32) {
-            const float term = (fabsf(__bfloat162float(coef[row * CS + c])) + 1.0e-35f) * s.size[(c < d ? c : c - d) >> 3];
+            const float size = s.size[(c < d ? c : c - d) >> 3], of = fabsf(__bfloat162float(coef[row * CS + c])), term = (of + 1.0e-35f) * size;
             most += term;
-            steps = fmaf(term, (float)(4 * (KB - (c >> 5))), steps);
+            steps = fmaf(term, (float)(2 * (KB - (c >> 5))), steps);
+            steps = fmaf(of + size, 6.0e-33f, steps);      // 1.2e-38 / (18 * 2^-23)
         }
         most = warp_sum(most);
         steps = warp_sum(steps);
         const bool unsafe = !(most <= 1.0e36f);
-        const float err = 1.02f * (most * (3.9e-6f + (float)G * 5.9604645e-8f) + steps * (6.f * 1.1920929e-7f)) + 1.0e-42f;
+        const float err = 1.02f * (most * (3.9e-6f + (float)G * 5.9604645e-8f) + steps * (18.f * 1.1920929e-7f)) + 2.0e-35f;
         s.choose[warp].run(p, r, keys + row * KS, err, unsafe, lane);
     }
 }

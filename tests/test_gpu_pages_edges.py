@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_pages import BF, DEV, F32, PAGE, Step, like_lists, names
+from tests.test_gpu_pages import BF, DEV, F32, PAGE, Step, check_selection, like_lists, names
 
 pytestmark = pytest.mark.gpu
 
@@ -209,3 +209,20 @@ def test_scores_that_are_all_the_lowest_show_in_a_prompt(ops):
     looks_up(s)
     s.dev["k_plane"][:, :, :, 0] = -math.inf
     assert attend_all(ops, s).isnan().all() and ops.tc5_status() == 0
+
+
+# ---- scores whose sums lose most of what they add up -------------------------------------------
+@pytest.mark.parametrize("big", [300.0, 2e4, 1e6])
+@pytest.mark.parametrize("pages,new,d", [(300, 21, 128), (300, 9, 64), (300, 40, 48), (300, 2, 128), (100, 12, 256)])
+def test_select_pages_whose_scores_cancel_late(ops, big, pages, new, d):
+    """The first channel's bound carries a number through the whole sum that the last channel's takes off again."""
+    s = Step([(pages * PAGE - new + 1, new)], 2, 1, d, BF, seed=pages)
+    bounds = s.bounds_plane()
+    mine = s.table[s.slots[0]].long()
+    for side in (0, 1):
+        bounds[mine, 0, side, 0] = big
+        bounds[mine, 0, side, d - 1] = -big
+    q = s.wide[:, :2 * d].view(-1, 2, d)
+    q[:, :, 0] = q[:, :, d - 1] = 0.75
+    s.q = s.wide[:, :2 * d].cpu()
+    check_selection(s, s.select(ops, bounds, 17), bounds, 17, 1, 2)
