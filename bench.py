@@ -416,6 +416,48 @@ def design_bench(args):
     return 0
 
 
+def fill_bounds(engine, torch, ops):
+    """The bounds of every page of the cache, where a model selects pages by them (as the steps that write the keys leave them)."""
+    for key, bounds in engine.cache._bounds.items():
+        pages = bounds.shape[1]
+        ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=engine.device)
+        ops.page_bounds(engine.cache._k[key], bounds, torch.arange(pages, dtype=torch.int32, device=engine.device).view(1, -1), ints(0),
+                        ints(64 * pages), ints(64 * pages), 1, 64 * pages)
+
+
+def sparse_bench(args):
+    """``--sparse-pages N``: whole decode steps that read N pages of 64 tokens a sequence beside the same steps reading everything; one
+    JSON line."""
+    import torch
+    from gophonic_b200 import ops
+    from gophonic_b200.config import PageSelection
+    from gophonic_b200.engine import Engine, Model
+    from gophonic_b200.sampling import DeviceSampler
+    cfg = config_of(args.model, args.layers, args.context)
+    batches = sorted({args.batch, *(int(b) for b in args.points.split(",") if b)})
+    clocks = ClockSampler()
+    clocks.start()
+    line = {"model": f"Qwen3-{args.model.upper()}-shaped", "layers": args.layers or sizes(args.model)["layers"], "dtype": "bf16", "context": args.context,
+            "pages": args.sparse_pages, "timing": "CUDA events around the steps, captured and replayed, sampling included",
+            "data": "synthetic: seeded random weights, random token ids, cache pre-filled with random keys/values and their bounds"}
+    for key, selection in (("everything", None), ("selected", PageSelection(args.sparse_pages))):
+        model = Model.from_random(cfg, seed=0, dtype="bfloat16", device="cuda:0", selection=selection)
+        for b in batches:
+            engine = Engine(model, max_tokens=b * args.context, max_slots=b, max_seq_tokens=args.context)
+            fill_cache_random(engine, torch)
+            fill_bounds(engine, torch, ops)
+            sampler = DeviceSampler(cfg.vocab_size, b, engine.device)
+            d = time_decode(engine, sampler, b, args.steps, max(16, args.warmup), torch, ops)
+            line[f"{key}_b{b}_ms"], line[f"{key}_b{b}_tok_s"] = round(d["ms"], 4), round(b / (d["ms"] * 1e-3), 1)
+            del engine, sampler
+            torch.cuda.empty_cache()
+        del model
+        torch.cuda.empty_cache()
+    line["clocks"] = clocks.stop()
+    print(json.dumps(line))
+    return 0
+
+
 def probe(name, **opts):
     """Run one kernel of the step a few times on a small, fixed workload (operands larger than L2
     where the kernel is bound by memory), for profilers.  Prints the kernel's own timing."""
@@ -852,9 +894,14 @@ def main():
     ap.add_argument("--prompt-tokens", type=int, default=PREFILL_TOKENS, help="prompt length of --probe prefill_step")
     ap.add_argument("--design", default="", help="instead of the headline run: a named configuration of another design "
                     f"({', '.join(sorted(DESIGN_TWINS))}) beside the closest Qwen3-shaped one, --layers layers each (default 8)")
+    ap.add_argument("--sparse-pages", type=int, default=0,
+                    help="instead of the headline run: decode steps that read so many pages of 64 tokens a sequence beside steps that read "
+                         "everything (with --model, --batch, --points, --context)")
     args = ap.parse_args()
     if args.design:
         return design_bench(args)
+    if args.sparse_pages:
+        return sparse_bench(args)
     if args.probe:
         return probe(args.probe, model=args.model, batch=args.batch, context=args.context, prompt_tokens=args.prompt_tokens)
     if args.profile:

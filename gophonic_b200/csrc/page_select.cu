@@ -1001,7 +1001,7 @@ GB_API int gb_select_pages(const PagesParams* pp, int dtype, cudaStream_t stream
     if (p.nseq <= 0 || p.max_q_len <= 0) return 0;
     if (int rc = check(p, dtype, "select_pages")) return rc;
     if (p.heads <= 0 || p.heads % p.kv_heads) GB_REFUSE("select_pages: %d heads over %d kv heads", p.heads, p.kv_heads);
-    if (p.first < 0 || p.last < 1 || p.first + p.last > p.top) GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
+    if (p.first < 0 || p.last < 1 || (int64_t)p.first + p.last > p.top) GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
     if (p.bt_stride > MAX_PAGES) GB_REFUSE("select_pages: sequences of up to %d pages; this kernel takes %d", p.bt_stride, MAX_PAGES);
     if (dtype == GB_BF16 && p.max_q_len >= TILE_MIN_ROWS && p.d % 16 == 0) {
         if (p.max_q_len > 16 && tile_smem<8>(p, 32) <= HALF_TILE_SMEM) return launch_tiles<2, 8>(p, stream);

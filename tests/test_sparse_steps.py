@@ -74,3 +74,14 @@ def test_a_run_that_selects_reads_no_cache_without_bounds():
                 Cache([(owner, None), (bounded, 0)] + more, 256, "cpu", torch.float32)
     c = Cache([(bounded, None), (bounded, 0), (plain, 0)], 256, "cpu", torch.float32)
     assert c.view(1).bounds.data_ptr() == c.view(0).bounds.data_ptr()
+
+
+@pytest.mark.parametrize("first,last", [(2 ** 31 - 1, 1), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 30, 2 ** 30), (1, 2 ** 31 - 1)])
+def test_more_pages_always_chosen_than_numbers_hold(first, last):
+    """Their sum passes 31 bits: refused ahead of any launch, as every sum above the list's length is."""
+    import ctypes
+    ops = pytest.importorskip("gophonic_b200.ops")
+    p = ops._PagesParams(q=4096, q_row_stride=256, bounds=4096, block_table=4096, bt_stride=8, seq_slot=4096, seq_q_start=4096, seq_q_len=4096,
+                         seq_kv_len=4096, nseq=1, heads=4, kv_heads=2, d=64, max_q_len=1, list=4096, top=4, first=first, last=last, pages=8, max_slots=2, rows=1)
+    rc = ops._lib.gb_select_pages(ctypes.byref(p), ctypes.c_int(ops.BF16), ctypes.c_void_p(0))
+    assert rc == -1 and "always chosen" in ops._lib.gb_last_error().decode()
