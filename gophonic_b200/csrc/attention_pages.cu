@@ -10,7 +10,8 @@
 // Neither these kernels nor the selection ahead of them let the kernel behind them start early: its CTAs took the SMs that clusters
 // were waiting for (36 layers of one token behind 32768, 64 pages: 5.2 ms a step with early starts, 3.7 without).
 // Scores, the softmax and the sums are float32; with bfloat16 the probabilities are rounded to bfloat16 for the second product, as
-// the values are.
+// the values are (tensor cores take both operands in one type): 0.0021 to 0.0023 of the result's size against 64 bits, where rounding
+// the result alone leaves 0.0017.
 #include "mma.cuh"
 #include "api.h"
 
@@ -29,7 +30,8 @@ constexpr int THREADS = 128;
 constexpr int MAX_TOP = 1024;     // entries of a list
 // Rows times key heads from which on runs of rows go to tcgen05 (attention_pages_tc5.cu), us here / there, 32 pages behind 20000: 8
 // key heads, one sequence of 4 rows 11.7 / 14.0, of 8 rows 16.8 / 15.6, of 16 rows 28 / 18; eight sequences of 2 rows 28 / 20; two
-// key heads, one sequence of 16 rows 13 / 18, of 32 rows 18 / 19, of 48 rows 28 / 21.
+// key heads, one sequence of 16 rows 13 / 18, of 32 rows 18 / 19, of 48 rows 28 / 21.  Rows are counted as the longest sequence's times
+// the sequences, of which the launch is made.
 constexpr int TC5_MIN_UNITS = 64;
 
 // The row's listed pages that it can see, in the list's order, packed into `to`, and behind them (from to[p.top] on) where they are in
@@ -474,10 +476,10 @@ __global__ void __launch_bounds__(THREADS) attn_pages_f32_kernel(PagesParams p) 
     join<float>(&ml[0][0], Os, at.nh, d, (float*)p.out + (int64_t)at.row * p.out_row_stride + (int64_t)at.h0 * d, n_all > 0);
 }
 
-// Into how many pieces a row's list is cut: the CTAs of a cluster, a power of two (sixteen where the GPU holds all of the clusters).  As many as run at once (one token over eight key heads, 32 pages:
-// 34 us in one piece, 19 in two, 12 in four, 8.4 in eight, 8.1 in sixteen); where not even two pieces each do, two if their waves end sooner than
-// those of whole rows (50 sequences over eight key heads, 64 pages: 173 us in one piece, 147 in two, 158 in four, 197 in eight;
-// 139 in two since a list's places are looked up at once).
+// Into how many pieces a row's list is cut: the CTAs of a cluster, a power of two (sixteen where the GPU holds all of the clusters).  As many
+// as run at once (one token over eight key heads, 32 pages: 34 us in one piece, 19 in two, 12 in four, 8.4 in eight, 8.1 in
+// sixteen); where not even two pieces each do, two if their waves end sooner than those of whole rows (50 sequences over eight key
+// heads, 64 pages: 173 us in one piece, 147 in two, 158 in four, 197 in eight; 139 in two since a list's places are looked up at once).
 int pieces_for(const PagesParams& p, int chunks, int per_sm, int wide) {
     const int64_t units = (int64_t)p.nseq * p.max_q_len * p.kv_heads * chunks;
     int pieces = 1;
@@ -491,7 +493,8 @@ int pieces_for(const PagesParams& p, int chunks, int per_sm, int wide) {
 template <typename K>
 int launch(K kernel, const PagesParams& p, int chunks, int pieces, int smem, cudaStream_t stream) {
     const int64_t x = (int64_t)p.nseq * p.max_q_len * pieces;
-    if (x > 0x7fffffff || p.kv_heads * chunks > 65535) GB_REFUSE("attention_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
+    if (x > 0x7fffffff || p.kv_heads * chunks > 65535)
+        GB_REFUSE("attention_pages: %d sequences of up to %d rows, %d kv heads exceed one launch", p.nseq, p.max_q_len, p.kv_heads);
     launch_pdl_cluster(kernel, dim3((unsigned)x, p.kv_heads * chunks), dim3(THREADS), (size_t)smem, stream, pieces, 1, p);
     GB_CHECK_LAUNCH("attention_pages");
     return 0;

@@ -20,8 +20,9 @@
 // The heads of a group are rows of the tile (a group of G heads takes the next power of two: a tensor map of three dimensions
 // brings token after token, head after head), so that they share every page too.
 //
-// A weight of zero times an infinite or NaN value is NaN, and stays one in the row's sums: a row whose sums are not all finite is
-// computed once more at the end, over its own keys alone, which gives what it gives if the value was the row's own.
+// The probabilities are rounded to bfloat16 for the second product, whose operands have one type.  A weight of zero times an infinite or
+// NaN value is NaN, and stays one in the row's sums: a row whose sums are not all finite is computed once more at the end, over
+// its own keys alone, which gives what it gives if the value was the row's own.
 // (A warp that looked through every page's values instead cost 11 %.)
 //
 // Where there are few tiles, a cluster of CTAs shares one: each takes a stretch of the pages, and they join their rows through
@@ -566,7 +567,8 @@ int gb_attention_pages_tc5(const PagesParams& p, cudaStream_t stream) {
     pieces = pieces < 1 ? 1 : pieces > MAX_PIECES ? MAX_PIECES : pieces;
     const dim3 grid(ceil_div(p.max_q_len, tok) * pieces, p.kv_heads, p.nseq);
     if (grid.y > 65535 || grid.z > 65535) GB_REFUSE("attention_pages: grid (%u, %u, %u) exceeds one launch", grid.x, grid.y, grid.z);
-    const cudaError_t e = launch_pdl_cluster(attn_pages_tc5_kernel, grid, dim3(THREADS), (size_t)(TILE_BYTES + 1024 + list_bytes(p)), stream, pieces, 1, map_q, map_k, map_v, p);
+    const cudaError_t e = launch_pdl_cluster(attn_pages_tc5_kernel, grid, dim3(THREADS), (size_t)(TILE_BYTES + 1024 + list_bytes(p)), stream,
+                                             pieces, 1, map_q, map_k, map_v, p);
     if (e != cudaSuccess) GB_REFUSE("attention_pages: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }

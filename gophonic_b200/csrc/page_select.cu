@@ -907,13 +907,18 @@ __global__ void __launch_bounds__(TILE_WARPS * 32, 16 / TILE_WARPS) select_tile_
 constexpr int MAX_PAGES = 32768;        // of a sequence: their scores stand in shared memory
 constexpr int MAX_TILE_SMEM = 232448;   // what a CTA can have
 constexpr int HALF_TILE_SMEM = 115712;  // what a CTA can have where two share an SM
-constexpr int TILE_MIN_ROWS = 8;        // rows of a sequence from which on they are scored as tiles
+// Rows of a sequence from which on they are scored as tiles, us row by row / in tiles, 32 pages behind 20000: 8 key heads, one sequence of
+// 4 rows 7.7 / 11.2, of 8 rows 13.9 / 11.4, of 16 rows 18 / 13, of 32 rows 21 / 25 (two tiles of 16 as one of 32); eight sequences of
+// 2 rows 17 / 12, of 8 rows 30 / 13; two key heads, one sequence of 8 rows 9.1 / 11.9, of 32 rows 14 / 24, eight of 16 rows 23 / 13.  By the
+// longest sequence: 50 single rows beside one of 8, 33 / 32.
+constexpr int TILE_MIN_ROWS = 8;
 
 int check(const PagesParams& p, int dtype, const char* who) {
     if (dtype != GB_F32 && dtype != GB_BF16) GB_REFUSE("%s: dtype code %d", who, dtype);
     const int E = dtype == GB_F32 ? 4 : 8;
     if (p.d <= 0 || p.d % E || p.d > 256) GB_REFUSE("%s: head_dim %d is not a multiple of %d up to 256", who, p.d, E);
-    if (p.kv_heads <= 0 || p.pages <= 0 || p.bt_stride <= 0 || p.max_slots <= 0) GB_REFUSE("%s: %d kv heads, %d pages, block table %d x %d", who, p.kv_heads, p.pages, p.max_slots, p.bt_stride);
+    if (p.kv_heads <= 0 || p.pages <= 0 || p.bt_stride <= 0 || p.max_slots <= 0)
+        GB_REFUSE("%s: %d kv heads, %d pages, block table %d x %d", who, p.kv_heads, p.pages, p.max_slots, p.bt_stride);
     if ((uintptr_t)p.bounds & 15) GB_REFUSE("%s: the page bounds must be 16-byte aligned", who);
     return 0;
 }
@@ -1001,7 +1006,8 @@ GB_API int gb_select_pages(const PagesParams* pp, int dtype, cudaStream_t stream
     if (p.nseq <= 0 || p.max_q_len <= 0) return 0;
     if (int rc = check(p, dtype, "select_pages")) return rc;
     if (p.heads <= 0 || p.heads % p.kv_heads) GB_REFUSE("select_pages: %d heads over %d kv heads", p.heads, p.kv_heads);
-    if (p.first < 0 || p.last < 1 || (int64_t)p.first + p.last > p.top) GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
+    if (p.first < 0 || p.last < 1 || (int64_t)p.first + p.last > p.top)
+        GB_REFUSE("select_pages: %d pages of which the first %d and the last %d are always chosen", p.top, p.first, p.last);
     if (p.bt_stride > MAX_PAGES) GB_REFUSE("select_pages: sequences of up to %d pages; this kernel takes %d", p.bt_stride, MAX_PAGES);
     if (dtype == GB_BF16 && p.max_q_len >= TILE_MIN_ROWS && p.d % 16 == 0) {
         if (p.max_q_len > 16 && tile_smem<8>(p, 32) <= HALF_TILE_SMEM) return launch_tiles<2, 8>(p, stream);

@@ -526,9 +526,8 @@ def checked_status():
     found out of bounds since the last call (the access was skipped or redirected, nothing faulted).
     Always None in the ordinary build, whose kernels carry no checks.  Synchronises."""
     out = (c_int * 4)()
-    for name in ("rows", "cache", "attention_simt", "attention_mma", "attention_tc5", "linear_state", "delta_state", "attention_sigmoid", "hyper", "postnorm", "attention_latent", "sandwich",
-                 "short_conv", "gated_delta", "page_select", "attention_pages",
-                 "attention_pages_tc5"):
+    for name in ("rows", "cache", "attention_simt", "attention_mma", "attention_tc5", "linear_state", "delta_state", "attention_sigmoid", "hyper",
+                 "postnorm", "attention_latent", "sandwich", "short_conv", "gated_delta", "page_select", "attention_pages", "attention_pages_tc5"):
         code = int(getattr(_lib, "gb_checked_status_" + name)(out))
         if code or out[3]:
             return name, _CHECK_NAMES.get(code, f"code {code}"), out[1], out[2], out[3]
@@ -940,8 +939,9 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v
     """Causal GQA over a part of the paged cache: row r's heads of kv head g attend to the keys, at positions up to the row's own, of
     the logical pages that ``pages[r, g]`` lists (int32 [rows, kv_heads, top], top up to ``MAX_LISTED_PAGES``; each page once, as
     ``select_pages`` leaves them; negative entries and pages behind the row's own name nothing).  A row that sees no key
-    gives zeros, one that sees a score of NaN or +inf, or scores of -inf alone, NaN; rows of no sequence keep what they had.  q and out are [rows, >= heads * head_dim] views (row strides free) that do not
-    overlap.  What a row does not see may hold Inf or NaN."""
+    gives zeros, one that sees a score of NaN or +inf, or scores of -inf alone, NaN; rows of no sequence keep what they had.  q and out
+    are [rows, >= heads * head_dim] views (row strides free; bfloat16 rows of q begin on 16 bytes) that do not overlap.  What a row
+    does not see may hold anything, Inf and NaN too."""
     dtype, dev, wide = q.dtype, q.get_device(), heads * head_dim
     table, listed, plane, shape, to = block_table.shape, pages.shape, k_plane.shape, q.shape, out.shape
     ok = dev >= 0 and len(shape) == 2 and len(to) == 2 and len(table) == 2 and len(listed) == 3
