@@ -442,7 +442,7 @@ __device__ __forceinline__ void prefill_tc5(const CUtensorMap& map_q, const CUte
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             // a sink adds one unit to the denominator: a key of score 0, in the scale the sums are kept in
             // (a sum so scaled that the unit overflows gives 1 / inf = 0, which is the limit)
-            if (!sig && p.sink && m_used != -INFINITY) l += exp2f((p.sinks ? p.sinks[head] * LOG2E : 0.f) - m_used);
+            if (!sig && p.sink) l += exp2f((p.sinks ? p.sinks[head] * LOG2E : 0.f) - m_used);
             // a NaN score's weight is 0 where the polynomial has it; and of a score of +inf, beside which the others weigh nothing, so
             // is its own, inf - inf
             if (!sig && !(m_run < INFINITY)) l = NAN;

@@ -211,6 +211,21 @@ def test_scores_that_are_all_the_lowest_show_in_a_prompt(ops):
     assert attend_all(ops, s).isnan().all() and ops.tc5_status() == 0
 
 
+@pytest.mark.parametrize("algo", ["prefill_tc5", "prefill_mma"])
+@pytest.mark.parametrize("own", [False, True], ids=["a unit", "a score a head"])
+def test_a_sink_takes_all_where_the_scores_are_the_lowest(ops, algo, own):
+    """0 / exp(sink): zeros, where without a sink it is 0 / 0."""
+    s = Step([(0, 150)], 4, 2, 128, BF, seed=3)
+    looks_up(s)
+    s.dev["k_plane"][:, :, :, 0] = -math.inf
+    out = torch.full((150, 512), 9.0, dtype=BF, device=DEV)
+    slot, start, q_len, kv_len = s.seq
+    sinks = torch.tensor([0.5, -3.0, 2.0, 0.0], device=DEV) if own else None
+    ops.attention(s.q_dev, out, s.dev["k_plane"], s.dev["v_plane"], s.dev["table"], slot, start, q_len, kv_len, 1, 150, 4, 2, 128, 128 ** -0.5, algo=algo,
+                  sink=True, sinks=sinks)
+    assert (out == 0).all() and ops.tc5_status() == 0
+
+
 # ---- scores whose sums lose most of what they add up -------------------------------------------
 @pytest.mark.parametrize("big", [300.0, 2e4, 1e6])
 @pytest.mark.parametrize("pages,new,d", [(300, 21, 128), (300, 9, 64), (300, 40, 48), (300, 2, 128), (100, 12, 256)])
